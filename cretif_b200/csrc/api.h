@@ -561,6 +561,28 @@ int cretif_sample(const float* logits, int ld, int rows, int V, float temperatur
 float cretif_uniform01(unsigned long long seed, long long request, int draw);
 int cretif_max_top_k(void);
 
+// Which of a sequence's drafts stand, and the token behind them (verify.cu).  logits [n_rows, V]: rows
+// cu[b] .. cu[b + 1] - 1 are sequence b's, one more than its drafts (at most K, drafts [B, K]).
+// draft_logits (may be null): place j of sequence b at b * ld_seq + j * ld_place.  accept_u [B, K],
+// next_u [B] in [0, 1).  accepted [B]; tokens [B, K + 1]: the drafts that stand, the token, then -1.
+int cretif_verify_drafts(const float* logits, int ld, int n_rows, const int* cu, const int* drafts,
+                         int ld_drafts, int K, const float* draft_logits, long long ld_seq,
+                         long long ld_place, const float* accept_u, int ld_u, const float* next_u,
+                         int B, int V, double temperature, int top_k, int* accepted, int* tokens,
+                         int ld_tokens, unsigned int* fault, void* stream);
+
+// Attention of few new tokens a sequence where groups of sequences share prefixes (attn_shared.cu).
+// plan: int32, n_pre prefix items of 8, n_own own items of 4, n_rows token rows of the groups, [T]
+// prefix pieces and [T] sequence of a token, [B] prefix of a sequence.  part_o
+// [max_pieces, T * nh, hd], part_ml [max_pieces, T * nh, 2]: scratch.
+int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int ldo, const void* kc,
+                       const void* vc, long long n_blocks, const int* table, int table_stride,
+                       int n_slots, const int* tok_pos, const int* cu, const int* seq_slot,
+                       const int* plan, int n_pre, int n_own, int own_splits, int max_pieces,
+                       int n_rows, int B, int T, int nh, int nkv, int hd, int bt, float scale,
+                       const float* sink, float* part_o, float* part_ml, unsigned int* fault,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,79 @@
+// What the kernels of the attention over a shared prefix have in common (attn_shared.cu).
+//
+// The keys of a batch's queries are cut into pieces: a prefix that a group of sequences shares in
+// ranges of whole blocks, each walked once for all the group's rows, and every sequence's own keys
+// behind it.  A piece leaves, for each of its rows (a token and a query head), the largest scaled
+// score m (times log2 e), l = sum 2^(s - m) and o = sum 2^(s - m) v; a row's output is
+//   sum_i 2^(m_i - m) o_i / (sum_i 2^(m_i - m) l_i + 2^(sink - m)),   m = max_i m_i.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+
+namespace cretif {
+
+constexpr int kShBlk = 64;                 // tokens of a cache block
+
+// A range of blocks of a group's prefix for some of the group's rows.  Row r of a key/value head is
+// query head kvh * g + r % g of token rows[row_base + r / g].
+struct SharedPrefixItem {
+  int row_base, row0, n_rows;
+  int seq;                                 // a member: its table is read
+  int blk0, blk1;                          // blocks [blk0, blk1)
+  int piece;                               // the piece's index among the rows' pieces
+  int pad;
+};
+// Some rows of one sequence over its own keys: row r is head kvh * g + r % g of token cu[seq] + r / g.
+struct SharedOwnItem {
+  int seq, row0, n_rows, pad;
+};
+
+// What every kernel of a call reads.
+struct SharedArgs {
+  const void *q, *kc, *vc;
+  void* out;
+  int ldq, ldo;
+  long long n_blocks;
+  const int* table;
+  int table_stride, n_slots;
+  const int *tok_pos, *cu, *seq_slot;
+  // the plan: prefix items, own items, the rows of the groups, [T] prefix pieces and sequence of a
+  // token, [B] prefix of a sequence
+  const SharedPrefixItem* pre;
+  const SharedOwnItem* own;
+  const int *rows, *tok_pieces, *tok_seq, *seq_prefix;
+  int n_pre, n_own, own_splits, max_pieces, T;
+  int nh, nkv, hd;
+  float scale_log2;
+  const float* sink;
+  float* part_o;                           // [pieces][T * nh][hd]
+  float2* part_ml;                         // [pieces][T * nh]
+  unsigned int* fault;
+};
+
+// The physical block at place `at` of a sequence's table; 0 and a fault bit where there is none.
+__device__ __forceinline__ int shared_block(const SharedArgs& a, int seq, int at) {
+  const int slot = a.seq_slot[seq];
+  int blk = -1;
+  if (slot >= 0 && slot < a.n_slots && at >= 0 && at < a.table_stride)
+    blk = a.table[(size_t)slot * a.table_stride + at];
+  if (blk < 0 || blk >= a.n_blocks) {
+    atomicOr(a.fault, (unsigned)kFaultBlockTable);
+    blk = 0;
+  }
+  return blk;
+}
+
+// A sequence's own keys: first block, and one past the last position that a row at `last` sees.  A
+// position inside the prefix is a caller's mistake: the fault bit is set and there are none.
+__device__ __forceinline__ int shared_own_end(const SharedArgs& a, int seq, int last) {
+  const int prefix = a.seq_prefix[seq];
+  if (last < prefix) {
+    atomicOr(a.fault, (unsigned)kFaultBlockTable);
+    return prefix;
+  }
+  return last + 1;
+}
+
+}  // namespace cretif

@@ -1521,6 +1521,70 @@ def sample(logits, out, temperature: float, top_k: int, seed: int, request=None,
                                _p(request), _p(draw), _p(out), _stream()), "sample")
 
 
+def verify_drafts(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens, temperature: float,
+                  top_k: int = 0, draft_logits=None, fault=None) -> None:
+    """Which drafted tokens the model's probabilities let stand, and the token behind the last of
+    them, from given uniform numbers.  ``logits`` [rows, V] float32: rows ``cu_rows[b]`` to
+    ``cu_rows[b + 1] - 1`` (int32 [B + 1]) are sequence b's, one more than its drafts, which are the
+    first entries of ``drafts[b]`` (int32 [B, K]); row j holds what follows the tokens before draft j.
+    ``temperature`` and ``top_k`` as in :func:`sample`; ``draft_logits`` [B, K, V] float32: the logits
+    that the drafts were drawn from with the same two, None: the drafts stand for certain (looked up).
+    ``accept_u`` [B, K] and ``next_u`` [B] float32 in [0, 1).  Results: ``accepted`` int32 [B], how
+    many stand, and ``tokens`` int32 [B, K + 1]: those drafts, the new token, -1 behind it.
+
+    Draft j stands while ``accept_u q_j(x) < p_j(x)``; the token is drawn from max(p - q, 0) at the
+    first that does not, from p behind them all, as the first id whose cumulative sum in id order
+    exceeds ``next_u`` of the total.  ``temperature <= 0``: a draft stands where it is the arg max (lowest
+    id among equals) and the token is the arg max.  NaN counts as -infinity; a row whose largest
+    entries are infinite is uniform over them.  A draft outside the vocabulary does not stand, a
+    sequence without rows or with more than K drafts gives no token (-1); both set the token bit of
+    ``fault``."""
+    _need(logits, "logits", torch.float32, 2); _need(cu_rows, "cu_rows", torch.int32, 1)
+    _need(drafts, "drafts", torch.int32, 2); _need(accept_u, "accept_u", torch.float32, 2)
+    _need(next_u, "next_u", torch.float32, 1); _need(accepted, "accepted", torch.int32, 1)
+    _need(tokens, "tokens", torch.int32, 2)
+    R, V = logits.shape
+    B, K = drafts.shape
+    dev = logits.device
+    if fault is None:
+        fault = fault_word(dev)
+    _need(fault, "fault", torch.int32)
+    if any(t.device != dev for t in (cu_rows, drafts, accept_u, next_u, accepted, tokens, fault)) \
+            or dev.index != torch.cuda.current_device():
+        raise KernelError("verify_drafts: all tensors must be on the current device")
+    if cu_rows.shape[0] != B + 1 or tuple(accept_u.shape) != (B, K) or next_u.shape[0] != B \
+            or accepted.shape[0] != B or tuple(tokens.shape) != (B, K + 1) or V < 1:
+        raise KernelError(f"verify_drafts: for {B} sequences of up to {K} drafts cu_rows is [{B + 1}], "
+                          f"accept_u [{B}, {K}], next_u and accepted [{B}], tokens [{B}, {K + 1}]")
+    if not (cu_rows.is_contiguous() and next_u.is_contiguous() and accepted.is_contiguous()) \
+            or (K > 0 and (drafts.stride(1) != 1 or accept_u.stride(1) != 1)) \
+            or (K > 0 and tokens.stride(1) != 1):
+        raise KernelError("verify_drafts: rows must be dense")
+    if not temperature == temperature:
+        raise KernelError("verify_drafts: the temperature is NaN")
+    if top_k < 0 or (temperature > 0 and 0 < top_k < V and top_k > lib().cretif_max_top_k()):
+        raise KernelError(f"verify_drafts: top_k {top_k} is below zero or exceeds the kernel's limit "
+                          f"{lib().cretif_max_top_k()}")
+    ld_seq = ld_place = V
+    if draft_logits is not None:
+        _need(draft_logits, "draft_logits", torch.float32, 3)
+        if tuple(draft_logits.shape) != (B, K, V) or (V > 1 and draft_logits.stride(2) != 1) \
+                or draft_logits.device != dev:
+            raise KernelError(f"verify_drafts: draft_logits must be [{B}, {K}, {V}] with dense rows")
+        ld_seq, ld_place = draft_logits.stride(0), draft_logits.stride(1)
+        if temperature <= 0 or K == 0:
+            draft_logits = None                # (a greedy draft is judged by the arg max alone)
+    if not B:
+        return
+    if not R:
+        raise KernelError("verify_drafts: every sequence has one row of logits at least")
+    _check(lib().cretif_verify_drafts(
+        _p(logits), _rows(logits, "logits"), R, _p(cu_rows), _p(drafts), max(K, drafts.stride(0)), K,
+        _p(draft_logits), ctypes.c_longlong(ld_seq), ctypes.c_longlong(max(V, ld_place)), _p(accept_u),
+        accept_u.stride(0), _p(next_u), B, V, ctypes.c_double(temperature), int(top_k), _p(accepted),
+        _p(tokens), max(K + 1, tokens.stride(0)), _p(fault), _stream()), "verify_drafts")
+
+
 def uniform01(seed: int, request: int, draw: int) -> float:
     """The uniform number the sampling kernel uses for (seed, request, draw)."""
     return float(lib().cretif_uniform01(ctypes.c_ulonglong(seed & 0xFFFFFFFFFFFFFFFF),
@@ -1745,6 +1809,145 @@ def attn_decode(q, out, kc, vc, table, tok_pos, tok_seq, seq_slot, nh: int, nkv:
         table.stride(0), _p(tok_pos), _p(tok_seq), _p(seq_slot), nh, nkv, hd,
         ctypes.c_float(scale), window, block_tokens, B, n_splits, _p(part_o), _p(part_ml),
         _p(counters), _p(fault), _stream()), "attn_decode")
+
+
+# ------------------------------------------------------------------ attention over shared prefixes
+class SharedPrefixPlan:
+    """How a step's rows and keys are dealt out, made by :func:`shared_prefix_plan`: device index
+    arrays and launch sizes that depend on how many tokens the sequences bring and on what they
+    share, not on slots, positions or values.  One plan serves every layer, and every later step of
+    the same make-up."""
+
+    __slots__ = ("data", "n_pre", "n_own", "own_splits", "max_pieces", "n_rows", "B", "T", "nh", "nkv",
+                 "hd", "dtype", "prefix_blocks", "device")
+
+
+def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_rows: int, ctas: int):
+    """The host side of a plan: (prefix items, own items, splits of the own keys, most pieces, rows,
+    pieces of a token, sequence of a token, prefix of a sequence), lists of integers."""
+    if nh <= 0 or nkv <= 0 or nh % nkv:
+        raise KernelError(f"shared prefix: {nh} heads cannot share {nkv} key/value heads")
+    news, starts = [int(n) for n in news], [int(n) for n in starts]
+    B, g = len(news), nh // nkv
+    if not B or len(starts) != B:
+        raise KernelError("shared prefix: a number of new and of cached tokens for every sequence")
+    if min(news) < 1 or min(starts) < 0:
+        raise KernelError("shared prefix: every sequence brings at least one token")
+    cu = [0]
+    for n in news:
+        cu.append(cu[-1] + n)
+    prefix_of = [0] * B
+    grouped = []                        # (blocks, tokens of the members, a member)
+    rows, seen = [], set()
+    for prefix, members in ((int(p), [int(b) for b in m]) for m, p in groups):
+        if prefix < 0 or prefix % 64:
+            raise KernelError(f"shared prefix: {prefix} tokens are not whole blocks of 64")
+        for b in members:
+            if not 0 <= b < B or b in seen:
+                raise KernelError(f"shared prefix: sequence {b} is not one of the step's {B}, or in "
+                                  "two groups")
+            if starts[b] < prefix:
+                raise KernelError(f"shared prefix: sequence {b} has {starts[b]} cached tokens, its "
+                                  f"group shares {prefix}")
+            seen.add(b)
+            prefix_of[b] = prefix
+        if prefix and members:
+            toks = [t for b in members for t in range(cu[b], cu[b + 1])]
+            grouped.append((prefix // 64, len(rows), toks, members[0]))
+            rows += toks
+    tok_pieces = [0] * cu[-1]
+    pre = []
+    # blocks an item: as many items as the chip holds at once, where there are blocks enough
+    units = sum(blocks * -(-len(toks) * g // tile_rows) for blocks, _, toks, _ in grouped) * nkv
+    per = max(1, -(-units // ctas))
+    for blocks, base, toks, member in grouped:
+        pieces = -(-blocks // per)
+        for t in toks:
+            tok_pieces[t] = pieces
+        n_rows = len(toks) * g
+        for piece in range(pieces):
+            blk0, blk1 = blocks * piece // pieces, blocks * (piece + 1) // pieces
+            for row0 in range(0, n_rows, tile_rows):
+                pre += [base, row0, min(tile_rows, n_rows - row0), member, blk0, blk1, piece, 0]
+    own = []
+    for b in range(B):
+        for row0 in range(0, news[b] * g, own_rows):
+            own += [b, row0, min(own_rows, news[b] * g - row0), 0]
+    own_blocks = max(-(-(starts[b] + news[b] - prefix_of[b]) // 64) for b in range(B))
+    splits = max(1, min(own_blocks, ctas // max(1, len(own) // 4 * nkv), 8))
+    tok_seq = [b for b in range(B) for _ in range(news[b])]
+    return pre, own, splits, max(tok_pieces) + splits, rows, tok_pieces, tok_seq, prefix_of
+
+
+def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, device) -> SharedPrefixPlan:
+    """The plan of a step for :func:`attn_shared`.  ``groups``: (sequences of the step, tokens they
+    share) pairs; the shared tokens are whole cache blocks of 64 that the members' tables name alike.
+    A sequence is in one group at most.  ``news``: the tokens every sequence brings, ``starts``: its
+    cached tokens (at least the shared ones).  How many ranges a sequence's own keys are cut into goes
+    by ``starts``; a plan stays right, if not best, while they grow."""
+    if dtype not in _DT:
+        raise KernelError(f"shared prefix: tensors of dtype {dtype} have no kernel")
+    if hd % 16 or not 16 <= hd <= 128:
+        raise KernelError(f"shared prefix: head_dim {hd} is not a multiple of 16 up to 128")
+    dev = torch.device(device)
+    ctas = 2 * (sm_count(dev) if dev.type == "cuda" else 148)
+    pre, own, splits, pieces, rows, tok_pieces, tok_seq, prefix_of = _shared_items(
+        groups, news, starts, nh, nkv, 32, 32, ctas)
+    plan = SharedPrefixPlan()
+    packed = torch.tensor(pre + own + rows + tok_pieces + tok_seq + prefix_of, dtype=torch.int32)
+    plan.data = packed.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else packed
+    plan.n_pre, plan.n_own, plan.own_splits, plan.max_pieces = len(pre) // 8, len(own) // 4, splits, pieces
+    plan.n_rows, plan.B, plan.T = len(rows), len(prefix_of), len(tok_seq)
+    plan.nh, plan.nkv, plan.hd, plan.dtype, plan.device = nh, nkv, hd, dtype, plan.data.device
+    plan.prefix_blocks = max(prefix_of) // 64
+    return plan
+
+
+def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: SharedPrefixPlan,
+                scale: float, block_tokens: int, fault, sink=None) -> None:
+    """Causal attention of a step whose sequences bring a few tokens each, with the keys of the
+    prefixes that they share read once a group (``plan``, from :func:`shared_prefix_plan`).  ``q``
+    rows start with the query heads; ``out`` [T, heads · head_dim], row t for token t.  The step's own
+    keys and values are in the cache already.  ``sink`` (float32 [heads], optional): exp(sink_h)
+    joins head h's softmax denominator.  bfloat16 or float32, head sizes in multiples of 16 up to 128,
+    any number of query heads on a key/value head.  A table entry that names no block, or a position
+    inside the shared tokens, sets the block-table bit of ``fault``."""
+    nh, nkv, hd, T, B = plan.nh, plan.nkv, plan.hd, plan.T, plan.B
+    _need(q, "q", plan.dtype, 2); _need(out, "out", plan.dtype, 2)
+    _need(kc, "k cache", plan.dtype, 4); _need(vc, "v cache", plan.dtype, 4)
+    _need(table, "table", torch.int32, 2); _need(tok_pos, "tok_pos", torch.int32, 1)
+    _need(cu_seqlens, "cu_seqlens", torch.int32, 1); _need(seq_slot, "seq_slot", torch.int32, 1)
+    _need(fault, "fault", torch.int32)
+    dev = plan.device
+    if not (dev == q.device == out.device == kc.device == vc.device == table.device == tok_pos.device
+            == cu_seqlens.device == seq_slot.device == fault.device) or dev.index != torch.cuda.current_device():
+        raise KernelError("attn_shared: the plan and all tensors must be on the current device")
+    if q.shape[0] < T or out.shape[0] < T or q.shape[1] < nh * hd or out.shape[1] < nh * hd:
+        raise KernelError(f"attn_shared: q and out must have at least {T} rows of {nh * hd}")
+    if tok_pos.shape[0] < T or cu_seqlens.shape[0] < B + 1 or seq_slot.shape[0] < B \
+            or not (tok_pos.is_contiguous() and cu_seqlens.is_contiguous() and seq_slot.is_contiguous()):
+        raise KernelError("attn_shared: a position per token, a slot per sequence and their offsets")
+    if kc.shape != vc.shape or tuple(kc.shape[1:]) != (nkv, 64, hd) or block_tokens != 64 \
+            or not kc.is_contiguous() or not vc.is_contiguous():
+        raise KernelError(f"attn_shared: cache must be contiguous [blocks, {nkv}, 64, {hd}], got "
+                          f"{tuple(kc.shape)} with blocks of {block_tokens}")
+    if table.shape[1] < plan.prefix_blocks:
+        raise KernelError("attn_shared: the table is shorter than the shared prefix")
+    if sink is not None:
+        _need(sink, "sink", torch.float32, 1)
+        if sink.shape[0] != nh or not sink.is_contiguous() or sink.device != dev:
+            raise KernelError("attn_shared: the sink has one number per query head")
+    if not scale > 0:
+        raise KernelError("attn_shared: the scale must be above zero")
+    scratch = torch.empty(plan.max_pieces * T * nh * (hd + 2), dtype=torch.float32, device=dev)
+    part_o = scratch.data_ptr()
+    _check(lib().cretif_attn_shared(
+        _p(q), _rows(q, "q"), _DT[plan.dtype], _p(out), _rows(out, "out"), _p(kc), _p(vc),
+        ctypes.c_longlong(kc.shape[0]), _p(table), _rows(table, "table"), table.shape[0], _p(tok_pos),
+        _p(cu_seqlens), _p(seq_slot), _p(plan.data), plan.n_pre, plan.n_own, plan.own_splits,
+        plan.max_pieces, plan.n_rows, B, T, nh, nkv, hd, block_tokens, ctypes.c_float(scale), _p(sink),
+        ctypes.c_void_p(part_o), ctypes.c_void_p(part_o + 4 * plan.max_pieces * T * nh * hd), _p(fault),
+        _stream()), "attn_shared", 2)
 
 
 _COUNTERS = {}

@@ -1,4 +1,4 @@
-"""Sampling: parameters and the device sampler."""
-from .sampler import Sampler, SamplingParams, uniform01
+"""Sampling: parameters, the device sampler, and the verification of drafted tokens."""
+from .sampler import DraftVerifier, Sampler, SamplingParams, uniform01
 
-__all__ = ["Sampler", "SamplingParams", "uniform01"]
+__all__ = ["DraftVerifier", "Sampler", "SamplingParams", "uniform01"]

@@ -78,6 +78,29 @@ class Sampler:
         return out
 
 
+class DraftVerifier:
+    """Verifies drafted tokens against the model's probabilities at the options a
+    :class:`Sampler` of the same parameters draws with, so that what is kept is distributed as
+    the sampler's tokens are (greedy: is what it would have chosen).  The uniform numbers are the
+    caller's (``SamplingParams.seed`` is not used)."""
+
+    def __init__(self, params: SamplingParams, vocab_size: int):
+        params.validate(vocab_size)
+        self.params, self.vocab_size = params, int(vocab_size)
+
+    def __call__(self, logits: torch.Tensor, cu_rows: torch.Tensor, drafts: torch.Tensor,
+                 accept_u: torch.Tensor, next_u: torch.Tensor, accepted: torch.Tensor,
+                 tokens: torch.Tensor, draft_logits: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """As :func:`cretif_b200.csrc.ops.verify_drafts`: what ``Engine.step`` gives for steps that
+        bring a last token and its drafts (``want="all"``) are the rows of ``logits``."""
+        if logits.shape[-1] != self.vocab_size:
+            raise ValueError(f"the logits have {logits.shape[-1]} columns, the vocabulary "
+                             f"{self.vocab_size}")
+        ops.verify_drafts(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens,
+                          self.params.temperature, self.params.top_k, draft_logits)
+        return tokens
+
+
 def _as_int64(seed: int) -> int:
     """The 64 bits of ``seed`` as a signed value (what an int64 tensor holds)."""
     seed &= 0xFFFFFFFFFFFFFFFF

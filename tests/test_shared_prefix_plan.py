@@ -1,0 +1,82 @@
+"""The host side of a shared-prefix plan: every row meets every key it sees exactly once."""
+import pytest
+import torch
+
+from cretif_b200.csrc import ops
+
+
+def walk(groups, news, starts, nh, nkv, tile_rows, own_rows, ctas):
+    pre, own, splits, pieces, rows, tok_pieces, tok_seq, prefix = ops._shared_items(
+        groups, news, starts, nh, nkv, tile_rows, own_rows, ctas)
+    g = nh // nkv
+    cu = [0]
+    for n in news:
+        cu.append(cu[-1] + n)
+    seen = {}
+    for i in range(0, len(pre), 8):
+        base, row0, n, member, b0, b1, piece, _ = pre[i:i + 8]
+        assert 0 < n <= tile_rows and b0 < b1
+        for r in range(row0, row0 + n):
+            t = rows[base + r // g]
+            assert piece < tok_pieces[t] <= pieces - splits
+            assert prefix[tok_seq[t]] == prefix[member]
+            for blk in range(b0, b1):
+                key = (t, r % g, blk)
+                assert key not in seen
+                seen[key] = piece
+    for t, b in enumerate(tok_seq):
+        assert cu[b] <= t < cu[b + 1]
+        for h in range(g):
+            for blk in range(prefix[b] // 64):
+                assert (t, h, blk) in seen
+    assert len(seen) == g * sum(prefix[b] // 64 * news[b] for b in range(len(news)))
+    mine = set()
+    for i in range(0, len(own), 4):
+        b, row0, n, _ = own[i:i + 4]
+        assert 0 < n <= own_rows
+        for r in range(row0, row0 + n):
+            assert (b, r) not in mine
+            mine.add((b, r))
+    assert len(mine) == g * sum(news)
+    return pre, own, splits, pieces
+
+
+@pytest.mark.parametrize("tile_rows, own_rows", [(32, 32), (128, 16)])
+@pytest.mark.parametrize("ctas", [1, 7, 296])
+def test_every_row_meets_every_key_once(tile_rows, own_rows, ctas):
+    walk([([0, 3, 1], 640), ([2, 5], 64)], [1, 4, 2, 1, 1, 9], [700, 640, 64, 641, 9, 100], 12, 4, tile_rows, own_rows,
+         ctas)
+    walk([(list(range(50)), 1024)], [1 + b % 3 for b in range(50)], [1024 + b for b in range(50)], 9, 3, tile_rows,
+         own_rows, ctas)
+    walk([], [1, 2], [0, 5], 4, 1, tile_rows, own_rows, ctas)
+    walk([([0], 0), ([1], 64)], [1, 2], [0, 64], 4, 1, tile_rows, own_rows, ctas)
+
+
+def test_items_fill_the_chip_without_going_far_beyond_it():
+    for batch, blocks in ((2, 3), (8, 31), (64, 125), (64, 469)):
+        pre, *_ = walk([(list(range(batch)), 64 * blocks)], [1] * batch, [64 * blocks] * batch, 9, 3, 32, 32, 296)
+        tiles = -(-batch * 3 // 32)
+        assert len(pre) // 8 * 3 <= max(296 + tiles * 3, 3 * tiles)
+
+
+def test_refusals():
+    plan = ops.shared_prefix_plan
+    ok = dict(groups=[([0, 1], 64)], news=[1, 1], starts=[64, 70], nh=4, nkv=2, hd=64, dtype=torch.bfloat16,
+              device="cpu")
+    assert plan(**ok).T == 2
+    for change in (dict(groups=[([0, 1], 65)]), dict(groups=[([0, 1], -64)]), dict(groups=[([0, 2], 64)]),
+                   dict(groups=[([0, -1], 64)]), dict(groups=[([0], 64), ([0, 1], 64)]), dict(groups=[([0, 0], 64)]),
+                   dict(groups=[([0, 1], 128)]), dict(news=[1, 0]), dict(news=[]), dict(starts=[64]),
+                   dict(starts=[64, -1]), dict(nh=3), dict(nkv=0), dict(hd=72), dict(hd=144), dict(hd=0),
+                   dict(dtype=torch.float16)):
+        with pytest.raises(ops.KernelError):
+            plan(**{**ok, **change})
+
+
+def test_cpu_tensors_are_refused():
+    plan = ops.shared_prefix_plan([([0, 1], 64)], [1, 1], [64, 70], 4, 2, 64, torch.float32, "cpu")
+    z = torch.zeros
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.attn_shared(z(2, 256), z(2, 256), z(4, 2, 64, 64), z(4, 2, 64, 64), z(2, 4, dtype=torch.int32),
+                        z(2, dtype=torch.int32), z(3, dtype=torch.int32), z(2, dtype=torch.int32), plan, 0.125, 64,
+                        z(1, dtype=torch.int32))
