@@ -176,15 +176,22 @@ __global__ void __launch_bounds__(kShThreads) shared_join_kernel(const SharedArg
       static_cast<T*>(a.out)[(size_t)t * a.ldo + (size_t)h * a.hd + lane + 32 * c] = from_float<T>(acc[c] * inv);
 }
 
+int launch_shared_bf16(const SharedArgs& a, cudaStream_t st);        // attn_shared_tc.cu
+
 template <typename T>
-static int launch_shared(const SharedArgs& a, cudaStream_t st) {
-  const size_t smem = ((size_t)(kShRows + kShBlk) * (a.hd + 4) + (size_t)kShBlk * a.hd + kShRows * 65) * 4;
-  cudaError_t e = cudaFuncSetAttribute(shared_pieces_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
-  launch_dependent(shared_pieces_kernel<T>, dim3(a.n_pre + a.n_own * a.own_splits, a.nkv), dim3(kShThreads),
-                   smem, st, a);
+static int launch_join(const SharedArgs& a, cudaStream_t st) {
   launch_dependent(shared_join_kernel<T>, dim3((a.T * a.nh + 7) / 8), dim3(kShThreads), 0, st, a);
   return launch_status();
+}
+
+static int launch_shared_f32(const SharedArgs& a, cudaStream_t st) {
+  const size_t smem = ((size_t)(kShRows + kShBlk) * (a.hd + 4) + (size_t)kShBlk * a.hd + kShRows * 65) * 4;
+  cudaError_t e = cudaFuncSetAttribute(shared_pieces_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  launch_dependent(shared_pieces_kernel<float>, dim3(a.n_pre + a.n_own * a.own_splits, a.nkv), dim3(kShThreads),
+                   smem, st, a);
+  return launch_join<float>(a, st);
 }
 
 }  // namespace cretif
@@ -220,6 +227,7 @@ extern "C" int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int
   a.n_pre = n_pre; a.n_own = n_own; a.own_splits = own_splits; a.max_pieces = max_pieces; a.T = T;
   a.nh = nh; a.nkv = nkv; a.hd = hd; a.scale_log2 = scale * 1.4426950408889634f; a.sink = sink;
   a.part_o = part_o; a.part_ml = reinterpret_cast<float2*>(part_ml); a.fault = fault;
-  return dt == kF32 ? launch_shared<float>(a, (cudaStream_t)stream)
-                    : launch_shared<__nv_bfloat16>(a, (cudaStream_t)stream);
+  if (dt == kF32) return launch_shared_f32(a, (cudaStream_t)stream);
+  const int e = launch_shared_bf16(a, (cudaStream_t)stream);
+  return e || own_splits == 1 ? e : launch_join<__nv_bfloat16>(a, (cudaStream_t)stream);
 }

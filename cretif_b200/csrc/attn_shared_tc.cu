@@ -1,0 +1,623 @@
+// The bfloat16 kernels of the attention over shared prefixes (attn_shared.h has the formula).
+//
+// shared_prefix_tc: the prefix's keys against all rows of a group on the tcgen05 tensor cores.
+// shared_own_mma: a sequence's own keys against its few rows, and the joining of a row's pieces.
+#include <cuda.h>
+
+#include "api.h"
+#include "attn_decode_mma.cuh"
+#include "attn_shared.h"
+#include "tc_common.cuh"
+
+namespace cretif {
+
+// ---------------------------------------------------------------------------------------
+// Prefix: a CTA takes up to 128 rows (tokens x heads of a key/value head) and a range of the
+// prefix's blocks, 64 keys a step; two CTAs fit an SM and fill each other's gaps.
+//   warps 0-3  softmax: a thread owns a row (a lane of tensor memory);
+//   warp 4     TMA producer: K and V tiles straight out of the block cache;
+//   warp 5     one thread issues S = Q K^T and O += P V.
+// Tensor memory: two score tiles of 64 columns, O.  A row's thread writes its probabilities as
+// bfloat16 over the scores it has read, from where the product P V takes them as its A operand; it
+// adds into O itself, since a row's reference for the exponentials moves only when a score exceeds
+// it by 2^8 (then the row's thread waits for the product before and scales O).
+// The tiles come in pairs: {K_0, K_1}, then {V_j, K_{j+2}}: one barrier to wait for a step, and one
+// commit a step, behind P V of step j and the scores of step j + 2, which tells the softmax threads
+// that the scores are there and the producer that the pair may be replaced.
+//
+// Few rows (FOLD = 2 or 4: up to 64 or 32): the rows lie in tensor memory FOLD times, and each copy
+// takes its share of every step's keys (zeros stand for the others), so that all four warps work;
+// the copies are joined at the end.
+constexpr int kSpThreads = 192, kSpRows = 128, kSpTile = kShBlk * 128;   // a 64 x 64 tile's bytes
+constexpr int kSpDone = 8;                // commit c arrives on barrier c % 8 (see the producer)
+
+struct SpSmem {
+  int q, ring, pairs, bars, xch, total;
+  __host__ __device__ explicit SpSmem(int n_sub) {
+    pairs = n_sub == 1 ? 5 : 2;
+    q = 0;
+    ring = n_sub * kSpRows * 128;
+    bars = ring + pairs * 2 * n_sub * kSpTile;
+    xch = bars + (kSpDone + 5 + 3) * 8 + 16;
+    total = xch + kSpRows * 8 + 1024;
+  }
+};
+
+__device__ __forceinline__ float sp_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float sp_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// MN-major operand (V): a key is a row of 128 bytes, 64-wide column groups are a tile apart.
+__device__ __forceinline__ uint64_t sp_desc_v(const void* tile) {
+  uint64_t d = 0;
+  d |= (uint64_t)((tc::smem_u32(tile) & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(kSpTile >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+template <int FOLD>
+__device__ __forceinline__ void sp_softmax(uint32_t lane_addr, int hd, int n_steps, int copy, float scale_log2,
+                                           uint64_t* done, uint64_t* p_full, volatile int* abort, float& m_out,
+                                           float& l_out) {
+  constexpr int NK = kShBlk / FOLD;       // this thread's keys of a step
+  constexpr uint32_t kColO = 128;
+  float m = -INFINITY, l = 0.f;
+  for (int j = 0; j < n_steps; ++j) {
+    tc::mbar_wait(&done[j % kSpDone], (uint32_t)((j / kSpDone) & 1), abort);
+    tc::tc_fence_after();
+    const uint32_t s_addr = lane_addr + (uint32_t)(j & 1) * 64;
+    uint32_t r[NK];
+    if constexpr (FOLD == 1) {
+      uint32_t (&lo)[32] = *reinterpret_cast<uint32_t (*)[32]>(&r[0]);
+      uint32_t (&hi)[32] = *reinterpret_cast<uint32_t (*)[32]>(&r[32]);
+      tc::tmem_load_32(s_addr, lo);
+      tc::tmem_load_32(s_addr + 32, hi);
+    } else if constexpr (FOLD == 2) {
+      tc::tmem_load_32(s_addr + copy * 32, r);
+    } else {
+      tc::tmem_load_16(s_addr + copy * 16, r);
+    }
+    tc::tmem_load_wait();
+    float mx[4] = {__uint_as_float(r[0]), __uint_as_float(r[1]), __uint_as_float(r[2]), __uint_as_float(r[3])};
+#pragma unroll
+    for (int c = 4; c + 3 < NK; c += 4) {
+      const int i = (c >> 2) & 1;
+      mx[2 * i] = sp_max3(mx[2 * i], __uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+      mx[2 * i + 1] = sp_max3(mx[2 * i + 1], __uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
+    }
+    // (the scale is positive: the largest raw score is the largest scaled one)
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+    if (j == 0) {
+      m = top;
+    } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+      const float m_new = fmaxf(m, top);
+      const float alpha = m == -INFINITY ? 0.f : sp_exp2(m - m_new);
+      // O is scaled in place, once the product of the step before has gone into it
+      tc::mbar_wait(&done[(j + 1) % kSpDone], (uint32_t)(((j + 1) / kSpDone) & 1), abort);
+      tc::tc_fence_after();
+      for (int c0 = 0; c0 < hd; c0 += 32) {
+        uint32_t o[32];
+        tc::tmem_load_32(lane_addr + kColO + (uint32_t)c0, o);
+        tc::tmem_load_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+        tc::tmem_store_32(lane_addr + kColO + (uint32_t)c0, o);
+      }
+      l *= alpha;
+      m = m_new;
+    }
+    const float neg_m = m == -INFINITY ? 0.f : -m;
+    const float2 scale2 = make_float2(scale_log2, scale_log2), neg2 = make_float2(neg_m, neg_m);
+    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+    uint32_t packed[NK / 2];
+#pragma unroll
+    for (int c = 0; c < NK; c += 2) {
+      const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, neg2);
+      const float2 p = make_float2(sp_exp2(x.x), sp_exp2(x.y));
+      sum[(c >> 1) & 1] = __fadd2_rn(sum[(c >> 1) & 1], p);
+      packed[c >> 1] = pack_bf16(p.x, p.y);
+    }
+    if constexpr (FOLD == 1) {
+      tc::tmem_store_32(s_addr, packed);
+    } else {
+      uint32_t all[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) all[e] = e / (NK / 2) == copy ? packed[e % (NK / 2)] : 0u;
+      tc::tmem_store_32(s_addr, all);
+    }
+    const float2 s2 = __fadd2_rn(sum[0], sum[1]);
+    l += s2.x + s2.y;
+    tc::tmem_store_wait();                 // P (and O) are in tensor memory, S has been read
+    tc::tc_fence_before();
+    tc::mbar_arrive(&p_full[j & 1]);
+  }
+  m_out = m;
+  l_out = l;
+}
+
+__global__ void __launch_bounds__(kSpThreads, 2)
+shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                        const __grid_constant__ SharedArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int hd = a.hd, n_sub = (hd + 63) >> 6;
+  const SpSmem L(n_sub);
+  uint64_t* done = reinterpret_cast<uint64_t*>(smem + L.bars);
+  uint64_t* full = done + kSpDone;
+  uint64_t* p_full = full + 5;
+  uint64_t* q_full = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float2* xch = reinterpret_cast<float2*>(smem + L.xch);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const SharedPrefixItem it = a.pre[blockIdx.x];
+  const int kvh = blockIdx.y, g = a.nh / a.nkv;
+  const int n = it.blk1 - it.blk0;
+  const int fold = it.n_rows <= 32 ? 4 : it.n_rows <= 64 ? 2 : 1;
+  const int span = kSpRows / fold;                       // lanes of a copy
+  // warps whose lanes hold rows: the others neither wait nor arrive
+  const int warps_a_copy = (it.n_rows + 31) >> 5;
+  constexpr uint32_t kColO = 128;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSpDone; ++i) tc::mbar_init(&done[i], 1);
+    for (int i = 0; i < L.pairs; ++i) tc::mbar_init(&full[i], 1);
+    tc::mbar_init(&p_full[0], 32 * warps_a_copy * fold);
+    tc::mbar_init(&p_full[1], 32 * warps_a_copy * fold);
+    tc::mbar_init(q_full, kSpRows);
+    *abort = 0;
+    tc::fence_barrier_init();
+    tc::tma_prefetch_descriptor(&map_k);
+    tc::tma_prefetch_descriptor(&map_v);
+  }
+  if (warp == 5) {
+    tc::tmem_alloc(tmem_slot, 256);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // Everything before this call's first kernel is done and visible behind the wait; the kernel
+  // behind this one may start only then, so that it may read the queries without a wait of its own.
+  dependent_wait();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (warp == 4) {
+    int mine = 0;
+    for (int p = 0; p <= n; ++p) {
+      // block ids of the range, 32 at a time: pair p needs block p (V is one pair behind its K)
+      // and the ones around it
+      const int s = p % L.pairs;
+      bool go = true;
+      if (lane == 0 && p >= L.pairs) {
+        // pair q has been read when commit q + 1 arrives; the one 8 commits later cannot arrive
+        // before pair q + L.pairs is loaded, which is this thread's next step
+        const int c = p - L.pairs + 1;
+        go = tc::mbar_wait(&done[c % kSpDone], (uint32_t)((c / kSpDone) & 1), abort);
+      }
+      go = __shfl_sync(0xffffffffu, go, 0);
+      if (!go) break;
+      if (lane < 2) {                                     // lane 0: the pair's first tile, 1: its second
+        const bool is_k = p == 0 || lane == 1;
+        const int j = p == 0 ? lane : lane == 0 ? p - 1 : p + 1;
+        const bool there = j < n;
+        mine = there ? shared_block(a, it.seq, it.blk0 + j) : 0;
+        const unsigned both = __ballot_sync(0x3u, there);
+        if (lane == 0) tc::mbar_expect_tx(&full[s], (uint32_t)(__popc(both) * n_sub * kSpTile));
+        __syncwarp(0x3u);
+        if (there) {
+          const int row = (mine * a.nkv + kvh) * kShBlk;
+          for (int sub = 0; sub < n_sub; ++sub)
+            tc::tma_load_2d(smem + L.ring + ((s * 2 + lane) * n_sub + sub) * kSpTile, is_k ? &map_k : &map_v,
+                            64 * sub, row, &full[s]);
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      const uint32_t idesc_qk = tc::instr_desc_bf16(kSpRows, kShBlk);
+      const uint32_t idesc_pv = tc::instr_desc_bf16(kSpRows, hd) | (1u << 16);   // B is MN-major
+      const int k_steps = hd >> 4;
+      const uint64_t qd = tc::smem_desc_k_sw128(smem + L.q);
+      auto scores = [&](int j) {
+        const int p = j < 2 ? 0 : j - 1;
+        const uint64_t kd =
+            tc::smem_desc_k_sw128(smem + L.ring + ((p % L.pairs) * 2 + (j == 0 ? 0 : 1)) * n_sub * kSpTile);
+        for (int kk = 0; kk < k_steps; ++kk)
+          tc::umma_bf16(tmem + (uint32_t)(j & 1) * 64, qd + (uint64_t)((kk >> 2) * ((kSpRows * 128) >> 4) + 2 * (kk & 3)),
+                        kd + (uint64_t)((kk >> 2) * (kSpTile >> 4) + 2 * (kk & 3)), idesc_qk, kk != 0);
+      };
+      bool ok = tc::mbar_wait(q_full, 0u, abort) && tc::mbar_wait(&full[0], 0u, abort);
+      if (ok) {
+        tc::tc_fence_after();
+        scores(0);
+        tc::umma_commit(&done[0]);
+        if (n > 1) scores(1);
+        tc::umma_commit(&done[1]);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const int p = j + 1;
+        ok = tc::mbar_wait(&full[p % L.pairs], (uint32_t)((p / L.pairs) & 1), abort) &&
+             tc::mbar_wait(&p_full[j & 1], (uint32_t)((j >> 1) & 1), abort);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint64_t vd = sp_desc_v(smem + L.ring + (p % L.pairs) * 2 * n_sub * kSpTile);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)                    // 16 keys: two 1,024-byte atoms of V
+          tc::umma_bf16_a_tmem(tmem + kColO, tmem + (uint32_t)((j & 1) * 64 + kk * 8), vd + (uint64_t)(kk * 128),
+                               idesc_pv, (j | kk) != 0);
+        if (j + 2 < n) scores(j + 2);
+        tc::umma_commit(&done[(j + 2) % kSpDone]);
+      }
+    }
+  } else {
+    // ---- the queries into shared memory, in the operand's swizzled layout
+    const int row = threadIdx.x, copy = row / span, r = row - copy * span;
+    {
+      const bool there = r < it.n_rows;
+      const int rr = it.row0 + r;
+      const __nv_bfloat16* src = nullptr;
+      if (there)
+        src = static_cast<const __nv_bfloat16*>(a.q) + (size_t)a.rows[it.row_base + rr / g] * a.ldq +
+              (size_t)(kvh * g + rr % g) * hd;
+      for (int ch = 0; ch < hd >> 3; ++ch) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (there) v = *reinterpret_cast<const uint4*>(src + 8 * ch);
+        *reinterpret_cast<uint4*>(smem + L.q + (ch >> 3) * kSpRows * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
+      }
+      tc::fence_proxy_async();
+      tc::mbar_arrive(q_full);
+    }
+    const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
+    const bool active = (warp * 32) % span < it.n_rows;
+    float m = -INFINITY, l = 0.f;
+    if (active) {
+      if (fold == 1) sp_softmax<1>(lane_addr, hd, n, 0, a.scale_log2, done, p_full, abort, m, l);
+      else if (fold == 2) sp_softmax<2>(lane_addr, hd, n, copy, a.scale_log2, done, p_full, abort, m, l);
+      else sp_softmax<4>(lane_addr, hd, n, copy, a.scale_log2, done, p_full, abort, m, l);
+      tc::mbar_wait(&done[(n + 1) % kSpDone], (uint32_t)(((n + 1) / kSpDone) & 1), abort);
+      tc::tc_fence_after();
+    }
+    auto part_row = [&](int rr) {
+      return (size_t)it.piece * a.T * a.nh + (size_t)a.rows[it.row_base + rr / g] * a.nh + kvh * g + rr % g;
+    };
+    if (fold == 1) {
+      const bool there = r < it.n_rows;
+      const size_t at = there ? part_row(it.row0 + r) : 0;
+      if (there) a.part_ml[at] = make_float2(m, l);
+      if (active)
+        for (int c0 = 0; c0 < hd; c0 += 32) {
+          uint32_t o[32];
+          tc::tmem_load_32(lane_addr + kColO + (uint32_t)c0, o);
+          tc::tmem_load_wait();
+          if (there) {
+            float4* dst = reinterpret_cast<float4*>(a.part_o + at * hd + c0);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c0 + e < hd)
+                dst[e >> 2] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                          __uint_as_float(o[e + 3]));
+          }
+        }
+    } else {
+      // the copies meet in shared memory (queries, keys and values have been read)
+      float* buf = reinterpret_cast<float*>(smem);
+      const int ld = hd + 4;
+      asm volatile("bar.sync 1, 128;" ::: "memory");      // all rows' products are done
+      if (active) {
+        xch[row] = make_float2(m, l);
+        for (int c0 = 0; c0 < hd; c0 += 32) {
+          uint32_t o[32];
+          tc::tmem_load_32(lane_addr + kColO + (uint32_t)c0, o);
+          tc::tmem_load_wait();
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (c0 + e < hd)
+              *reinterpret_cast<float4*>(buf + row * ld + c0 + e) =
+                  make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                              __uint_as_float(o[e + 3]));
+        }
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const int quads = hd >> 2;
+      for (int i = threadIdx.x; i < it.n_rows * quads; i += kSpRows) {
+        const int rr = i / quads, c = (i - rr * quads) * 4;
+        float mm = -INFINITY;
+        for (int f = 0; f < fold; ++f) mm = fmaxf(mm, xch[f * span + rr].x);
+        float den = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int f = 0; f < fold; ++f) {
+          const float2 ml = xch[f * span + rr];
+          const float w = ml.x == -INFINITY ? 0.f : sp_exp2(ml.x - mm);
+          const float4 o = *reinterpret_cast<const float4*>(buf + (f * span + rr) * ld + c);
+          den = fmaf(w, ml.y, den);
+          acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y);
+          acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
+        }
+        const size_t at = part_row(it.row0 + rr);
+        if (c == 0) a.part_ml[at] = make_float2(mm, den);
+        *reinterpret_cast<float4*>(a.part_o + at * hd + c) = acc;
+      }
+    }
+  }
+  if (*abort && threadIdx.x == 0) atomicOr(a.fault, (unsigned)kFaultWaitExpired);
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    __syncwarp();
+    tc::tmem_dealloc(tmem, 256);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Own keys: a CTA takes up to 16 rows of one sequence and key/value head; its warps take 16 keys of
+// every block (or of two blocks) each, straight from the cache into the operands' registers.
+//   S = Q K^T (m16n8k16): the channels of 32 are taken in an order in which a lane's 16 bytes of a
+//   key are its part of two products (channels 8c .. 8c + 7 of lane c: pairs 0 and 1 in the first,
+//   2 and 3 in the second), the same for the queries.
+//   O += P V: column n of product t is channel 8 n + t, so a lane's 16 bytes of a key are its part
+//   of eight products; two keys' values are brought together by byte permutes.
+// No shared memory and no barrier inside the loop; the next 16 keys are on their way meanwhile.
+// With JOIN the CTA holds all of the rows' own keys and joins the rows' prefix pieces itself (it is
+// launched while the prefix kernel runs and waits for it only then); else it leaves pieces.
+template <int HDG, int WARPS, bool JOIN>
+__global__ void __launch_bounds__(WARPS * 32)
+shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
+  extern __shared__ __align__(16) float so_smem[];
+  const int hd = a.hd, g = a.nh / a.nkv, kvh = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int split = JOIN ? 0 : blockIdx.x % a.own_splits, splits = JOIN ? 1 : a.own_splits;
+  // (the plan is never written by a kernel)
+  const SharedOwnItem it = a.own[JOIN ? blockIdx.x : blockIdx.x / a.own_splits];
+  if (!after_prefix) dependent_wait();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int seq = it.seq, cu0 = a.cu[seq];
+  const int prefix = a.seq_prefix[seq];
+  const int end = shared_own_end(a, seq, a.tok_pos[cu0 + (it.row0 + it.n_rows - 1) / g]);
+  // ---- queries: rows r and r + 8
+  uint32_t qa[HDG * 2][2][4];                             // [32 channels][row][pair]
+  int pos[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = r + 8 * i, rr = it.row0 + row;
+    const bool there = row < it.n_rows;
+    const int t = cu0 + (there ? rr / g : 0);
+    pos[i] = there ? a.tok_pos[t] : -1;
+    const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.ldq +
+                               (size_t)(kvh * g + (there ? rr % g : 0)) * hd;
+#pragma unroll
+    for (int d = 0; d < HDG * 2; ++d) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (there && 32 * d + 8 * c < hd) v = *reinterpret_cast<const uint4*>(src + 32 * d + 8 * c);
+      qa[d][i][0] = v.x; qa[d][i][1] = v.y; qa[d][i][2] = v.z; qa[d][i][3] = v.w;
+    }
+  }
+  float o[HDG][8][4];
+#pragma unroll
+  for (int v = 0; v < HDG; ++v)
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[v][t][e] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  // 16 keys a warp and step: 64 / 16 warps share a block, WARPS / 4 blocks a step
+  const int blocks = (end - prefix + kShBlk - 1) / kShBlk, blk0 = prefix / kShBlk;
+  constexpr int kStep = WARPS / 4;
+  const int first = split * kStep + (warp >> 2), stride = splits * kStep, key_in = (warp & 3) * 16;
+  uint4 kr[HDG * 2][2], vr[HDG][4];
+  auto load = [&](int i) {                                // keys key_in .. + 15 of own block i
+    const int key0 = prefix + i * kShBlk + key_in;
+    const size_t at = ((size_t)shared_block(a, seq, blk0 + i) * a.nkv + kvh) * kShBlk * hd;
+    const __nv_bfloat16* kp = static_cast<const __nv_bfloat16*>(a.kc) + at + (size_t)key_in * hd;
+    const __nv_bfloat16* vp = static_cast<const __nv_bfloat16*>(a.vc) + at + (size_t)key_in * hd;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int d = 0; d < HDG * 2; ++d)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        kr[d][x] = key0 + 8 * x + r < end && 32 * d + 8 * c < hd
+            ? __ldg(reinterpret_cast<const uint4*>(kp + (size_t)(8 * x + r) * hd + 32 * d + 8 * c)) : zero;
+#pragma unroll
+    for (int v = 0; v < HDG; ++v)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int key = 2 * c + (x & 1) + 8 * (x >> 1);
+        vr[v][x] = key0 + key < end && 64 * v + 8 * r < hd
+            ? __ldg(reinterpret_cast<const uint4*>(vp + (size_t)key * hd + 64 * v + 8 * r)) : zero;
+      }
+  };
+  auto has = [&](int i) { return i < blocks && prefix + i * kShBlk + key_in < end; };
+  if (has(first)) load(first);
+  for (int i = first; has(i); i += stride) {
+    const int key0 = prefix + i * kShBlk + key_in;
+    uint4 kn[HDG * 2][2], vn[HDG][4];
+#pragma unroll
+    for (int d = 0; d < HDG * 2; ++d) { kn[d][0] = kr[d][0]; kn[d][1] = kr[d][1]; }
+#pragma unroll
+    for (int v = 0; v < HDG; ++v)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) vn[v][x] = vr[v][x];
+    if (has(i + stride)) load(i + stride);
+    float s[2][4];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[x][e] = 0.f;
+#pragma unroll
+    for (int d = 0; d < HDG * 2; ++d)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        mma_16816_f32(s[x], qa[d][0][0], qa[d][1][0], qa[d][0][1], qa[d][1][1], kn[d][x].x, kn[d][x].y);
+        mma_16816_f32(s[x], qa[d][0][2], qa[d][1][2], qa[d][0][3], qa[d][1][3], kn[d][x].z, kn[d][x].w);
+      }
+    uint32_t pa[4];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {                         // rows r, r + 8
+      float t4[4], mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + 8 * (e >> 1) + 2 * c + (e & 1);
+        t4[e] = key <= pos[w] ? s[e >> 1][2 * w + (e & 1)] * a.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, t4[e]);
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float m_new = fmaxf(m[w], mx);
+      const float alpha = m[w] == -INFINITY ? 0.f : sp_exp2(m[w] - m_new);
+      float p[4], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[e] = t4[e] == -INFINITY ? 0.f : sp_exp2(t4[e] - m_new);
+        sum += p[e];
+      }
+      l[w] = l[w] * alpha + sum;
+      m[w] = m_new;
+      pa[w] = pack_bf16(p[0], p[1]);
+      pa[2 + w] = pack_bf16(p[2], p[3]);
+#pragma unroll
+      for (int v = 0; v < HDG; ++v)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) { o[v][t][2 * w] *= alpha; o[v][t][2 * w + 1] *= alpha; }
+    }
+#pragma unroll
+    for (int v = 0; v < HDG; ++v) {
+      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vn[v][0]);
+      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vn[v][1]);
+      const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vn[v][2]);
+      const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vn[v][3]);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const unsigned sel = t & 1 ? 0x7632u : 0x5410u;
+        mma_16816_f32(o[v][t], pa[0], pa[1], pa[2], pa[3], __byte_perm(w0[t >> 1], w1[t >> 1], sel),
+                      __byte_perm(w2[t >> 1], w3[t >> 1], sel));
+      }
+    }
+  }
+  // ---- the warps' parts meet in shared memory: a lane has channels 16c .. 16c + 15 of two rows
+  const int ld = hd + 4;
+  float* so = so_smem;                                    // [WARPS][16][hd + 4]
+  float2* sml = reinterpret_cast<float2*>(so + WARPS * 16 * ld);    // [WARPS][16]
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
+    l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
+    if (c == 0) sml[warp * 16 + r + 8 * w] = make_float2(m[w], l[w]);
+    if (r + 8 * w < it.n_rows) {
+#pragma unroll
+      for (int v = 0; v < HDG; ++v) {
+        float* dst = so + (warp * 16 + r + 8 * w) * ld + 64 * v + 16 * c;
+        if (64 * v + 16 * c < hd) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < 8; t += 4)
+              *reinterpret_cast<float4*>(dst + 8 * h + t) =
+                  make_float4(o[v][t][2 * w + h], o[v][t + 1][2 * w + h], o[v][t + 2][2 * w + h], o[v][t + 3][2 * w + h]);
+        }
+      }
+    }
+  }
+  // The prefix pieces are there; and this kernel ends behind the prefix kernel, so that what waits
+  // for this one need not wait for that one.
+  if (after_prefix) dependent_wait();
+  __syncthreads();
+  const int quads = hd >> 2;
+  const size_t rows_all = (size_t)a.T * a.nh;
+  for (int i = threadIdx.x; i < it.n_rows * quads; i += WARPS * 32) {
+    const int row = i / quads, ch = (i - row * quads) * 4, rr = it.row0 + row;
+    const int t = cu0 + rr / g, h = kvh * g + rr % g;
+    const size_t at = (size_t)t * a.nh + h;
+    const int n = JOIN ? a.tok_pieces[t] : 0;
+    float mm = -INFINITY;
+    const float sink = JOIN && a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
+    mm = fmaxf(mm, sink);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, sml[w * 16 + row].x);
+    for (int p = 0; p < n; ++p) mm = fmaxf(mm, __ldcg(&a.part_ml[p * rows_all + at]).x);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float den = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float2 ml, const float4& x) {
+      const float w = ml.x == -INFINITY ? 0.f : sp_exp2(ml.x - ref);
+      den = fmaf(w, ml.y, den);
+      acc.x = fmaf(w, x.x, acc.x); acc.y = fmaf(w, x.y, acc.y);
+      acc.z = fmaf(w, x.z, acc.z); acc.w = fmaf(w, x.w, acc.w);
+    };
+#pragma unroll 4
+    for (int p = 0; p < n; ++p)
+      add(__ldcg(&a.part_ml[p * rows_all + at]),
+          __ldcg(reinterpret_cast<const float4*>(a.part_o + (p * rows_all + at) * hd + ch)));
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+      add(sml[w * 16 + row], *reinterpret_cast<const float4*>(so + (w * 16 + row) * ld + ch));
+    if (JOIN) {
+      if (a.sink) den += sink == ref ? 1.0f : exp2f(sink - ref);
+      const float inv = den > 0.f ? 1.0f / den : 0.f;
+      uint2 packed = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)t * a.ldo + (size_t)h * hd + ch) = packed;
+    } else {
+      const size_t to = (size_t)(a.max_pieces - a.own_splits + split) * rows_all + at;
+      if (ch == 0) a.part_ml[to] = make_float2(mm, den);
+      *reinterpret_cast<float4*>(a.part_o + to * hd + ch) = acc;
+    }
+  }
+}
+
+template <typename... Params, typename... Args>
+static int sp_launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args&&... args) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = dependent_launch_enabled();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  return e == cudaSuccess ? launch_status() : (int)e;
+}
+
+template <int HDG, int WARPS>
+static int launch_own(const SharedArgs& a, cudaStream_t st) {
+  const size_t smem = (size_t)(WARPS * 16 * (a.hd + 4) + WARPS * 32) * 4;
+  const int after = a.n_pre > 0;
+  return a.own_splits == 1
+      ? sp_launch(shared_own_mma_kernel<HDG, WARPS, true>, dim3(a.n_own, a.nkv), WARPS * 32, smem, st, a, after)
+      : sp_launch(shared_own_mma_kernel<HDG, WARPS, false>, dim3(a.n_own * a.own_splits, a.nkv), WARPS * 32, smem, st, a,
+                  after);
+}
+
+// The prefix pieces and the own keys; joins the rows where the own keys are in one piece.
+int launch_shared_bf16(const SharedArgs& a, cudaStream_t st) {
+  if (((uintptr_t)a.q & 15) || a.ldq % 8 || ((uintptr_t)a.out & 7) || a.ldo % 4) return kMisaligned;
+  if (a.n_pre > 0) {
+    const long long cache_rows = a.n_blocks * a.nkv * kShBlk;
+    if (cache_rows > 0x7fffffffLL) return kBadArgument;
+    CUtensorMap mk, mv;
+    if (make_tile_map_bf16(&mk, a.kc, (int)cache_rows, a.hd, a.hd, kShBlk) ||
+        make_tile_map_bf16(&mv, a.vc, (int)cache_rows, a.hd, a.hd, kShBlk))
+      return kBadArgument;
+    const SpSmem L((a.hd + 63) / 64);
+    const int e = sp_launch(shared_prefix_tc_kernel, dim3(a.n_pre, a.nkv), kSpThreads, L.total, st, mk, mv, a);
+    if (e) return e;
+  }
+  return a.hd <= 64 ? launch_own<1, 4>(a, st) : launch_own<2, 4>(a, st);
+}
+
+}  // namespace cretif

@@ -1822,6 +1822,21 @@ class SharedPrefixPlan:
                  "hd", "dtype", "prefix_blocks", "device")
 
 
+def _blocks_an_item(tiles, ctas: int, begin: int = 4) -> int:
+    """How many blocks of its prefix an item walks: ``tiles`` are (blocks of a prefix, items that walk
+    each of its ranges at once) pairs; the fewest turns of ``ctas`` items times what one takes, which
+    is its blocks and some ``begin`` more for setting up."""
+    longest = max((blocks for blocks, _ in tiles), default=1)
+    best = (None, longest)
+    for pieces in range(1, min(longest, ctas) + 1):
+        per = -(-longest // pieces)
+        items = sum(-(-blocks // per) * n for blocks, n in tiles)
+        cost = -(-items // ctas) * (per + begin)
+        if best[0] is None or cost < best[0]:
+            best = (cost, per)
+    return best[1]
+
+
 def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_rows: int, ctas: int):
     """The host side of a plan: (prefix items, own items, splits of the own keys, most pieces, rows,
     pieces of a token, sequence of a token, prefix of a sequence), lists of integers."""
@@ -1857,9 +1872,7 @@ def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_r
             rows += toks
     tok_pieces = [0] * cu[-1]
     pre = []
-    # blocks an item: as many items as the chip holds at once, where there are blocks enough
-    units = sum(blocks * -(-len(toks) * g // tile_rows) for blocks, _, toks, _ in grouped) * nkv
-    per = max(1, -(-units // ctas))
+    per = _blocks_an_item([(blocks, -(-len(toks) * g // tile_rows) * nkv) for blocks, _, toks, _ in grouped], ctas)
     for blocks, base, toks, member in grouped:
         pieces = -(-blocks // per)
         for t in toks:
@@ -1874,7 +1887,7 @@ def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_r
         for row0 in range(0, news[b] * g, own_rows):
             own += [b, row0, min(own_rows, news[b] * g - row0), 0]
     own_blocks = max(-(-(starts[b] + news[b] - prefix_of[b]) // 64) for b in range(B))
-    splits = max(1, min(own_blocks, ctas // max(1, len(own) // 4 * nkv), 8))
+    splits = max(1, min(own_blocks // 8, ctas // max(1, len(own) // 4 * nkv), 8))
     tok_seq = [b for b in range(B) for _ in range(news[b])]
     return pre, own, splits, max(tok_pieces) + splits, rows, tok_pieces, tok_seq, prefix_of
 
@@ -1892,7 +1905,7 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
     dev = torch.device(device)
     ctas = 2 * (sm_count(dev) if dev.type == "cuda" else 148)
     pre, own, splits, pieces, rows, tok_pieces, tok_seq, prefix_of = _shared_items(
-        groups, news, starts, nh, nkv, 32, 32, ctas)
+        groups, news, starts, nh, nkv, *((128, 16) if dtype == torch.bfloat16 else (32, 32)), ctas)
     plan = SharedPrefixPlan()
     packed = torch.tensor(pre + own + rows + tok_pieces + tok_seq + prefix_of, dtype=torch.int32)
     plan.data = packed.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else packed

@@ -56,7 +56,7 @@ def test_items_fill_the_chip_without_going_far_beyond_it():
     for batch, blocks in ((2, 3), (8, 31), (64, 125), (64, 469)):
         pre, *_ = walk([(list(range(batch)), 64 * blocks)], [1] * batch, [64 * blocks] * batch, 9, 3, 32, 32, 296)
         tiles = -(-batch * 3 // 32)
-        assert len(pre) // 8 * 3 <= max(296 + tiles * 3, 3 * tiles)
+        assert len(pre) // 8 * 3 <= max(296, 3 * tiles)
 
 
 def test_refusals():
