@@ -565,11 +565,13 @@ int cretif_max_top_k(void);
 // cu[b] .. cu[b + 1] - 1 are sequence b's, one more than its drafts (at most K, drafts [B, K]).
 // draft_logits (may be null): place j of sequence b at b * ld_seq + j * ld_place.  accept_u [B, K],
 // next_u [B] in [0, 1).  accepted [B]; tokens [B, K + 1]: the drafts that stand, the token, then -1.
+// scratch: as many bytes as cretif_verify_scratch says, 8-byte aligned.
+long long cretif_verify_scratch(int n_rows, int B, int K, int V, int top_k, int draft_rows);
 int cretif_verify_drafts(const float* logits, int ld, int n_rows, const int* cu, const int* drafts,
                          int ld_drafts, int K, const float* draft_logits, long long ld_seq,
                          long long ld_place, const float* accept_u, int ld_u, const float* next_u,
                          int B, int V, double temperature, int top_k, int* accepted, int* tokens,
-                         int ld_tokens, unsigned int* fault, void* stream);
+                         int ld_tokens, void* scratch, unsigned int* fault, void* stream);
 
 // Attention of few new tokens a sequence where groups of sequences share prefixes (attn_shared.cu).
 // plan: int32, n_pre prefix items of 8, n_own own items of 4, n_rows token rows of the groups, [T]

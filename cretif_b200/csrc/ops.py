@@ -35,6 +35,7 @@ def lib():
         L = load_library()
         L.cretif_uniform01.restype = ctypes.c_float
         L.cretif_delta_chunk_row.restype = ctypes.c_longlong
+        L.cretif_verify_scratch.restype = ctypes.c_longlong
         L.cretif_uniform01.argtypes = [ctypes.c_ulonglong, ctypes.c_longlong, ctypes.c_int]
         _lib = L
     return _lib
@@ -1578,11 +1579,14 @@ def verify_drafts(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens, t
         return
     if not R:
         raise KernelError("verify_drafts: every sequence has one row of logits at least")
+    scratch = torch.empty(lib().cretif_verify_scratch(R, B, K, V, int(top_k) if temperature > 0 else 0,
+                                                      int(draft_logits is not None)),
+                          dtype=torch.uint8, device=dev)
     _check(lib().cretif_verify_drafts(
         _p(logits), _rows(logits, "logits"), R, _p(cu_rows), _p(drafts), max(K, drafts.stride(0)), K,
         _p(draft_logits), ctypes.c_longlong(ld_seq), ctypes.c_longlong(max(V, ld_place)), _p(accept_u),
         accept_u.stride(0), _p(next_u), B, V, ctypes.c_double(temperature), int(top_k), _p(accepted),
-        _p(tokens), max(K + 1, tokens.stride(0)), _p(fault), _stream()), "verify_drafts")
+        _p(tokens), max(K + 1, tokens.stride(0)), _p(scratch), _p(fault), _stream()), "verify_drafts", 2)
 
 
 def uniform01(seed: int, request: int, draw: int) -> float:

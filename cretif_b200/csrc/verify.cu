@@ -8,18 +8,59 @@
 // whose cumulative sum, in id order, exceeds u' times the total.  So the tokens are distributed as if
 // each had been drawn from its p.  T <= 0: a draft stands where it is the arg max.
 //
-// A row's terms are 2^((x - max) / T log2 e); an entry equal to the row's maximum counts 1 whatever
-// it is, so that a row of equal infinities is uniform; NaN counts as -infinity.  Sums are 64-bit: the
-// drawn id is decided at one of V borders, and sums that are off by 1e-8 of the total would draw
-// another id once in V * 1e-8 draws (1 in 2,000 at 49,152 ids).
+// A row's terms are 2^((x - max) log2 e / T); an entry equal to the row's maximum counts 1 whatever
+// it is, so that a row of equal infinities is uniform; NaN counts as -infinity.
+//
+// Two launches.  The first looks at all rows: what decides whether a draft stands are its row's
+// maximum and sum (32-bit terms, off by about 1e-8 of the sum: a draft is judged otherwise once in
+// 1e8), with top_k the kept entries themselves.  The second decides and draws.  An id is drawn at one
+// of V borders, so sums that are off by 1e-8 would draw another id once in V 1e-8 draws (1 in 2,000
+// at 49,152 ids): the one or two rows that a sequence draws from are summed again in 64 bits.
 //
 // The reference has no counterpart (its sampling: src/embedding.cu:343-406).
+#include <cooperative_groups.h>
+
 #include "api.h"
 #include "common.cuh"
 
 namespace cretif {
 
-constexpr int kVfThreads = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int kVfMaxTopK = 1024;
+
+struct VfArgs {
+  const float* logits;
+  int ld, n_rows;
+  const int* cu;
+  const int* drafts;
+  int ld_drafts, K, B, V;
+  const float* draft_logits;
+  long long ld_seq, ld_place;
+  const float* accept_u;
+  int ld_u;
+  const float* next_u;
+  double log2_t;                // log2 e / T, within what float32 holds
+  int top_k;
+  int* accepted;
+  int* tokens;
+  int ld_tokens;
+  unsigned int* fault;
+  // what the first launch leaves: rows 0 .. n_rows - 1 are the logits', n_rows + b K + j draft j's
+  void* stats;                  // [rows][slices] VfPart, with top_k [rows] VfKept, greedy [rows][slices] u64
+  int slices, slice_vectors;    // vectors of four a slice
+  float* list_v;                // top_k: [rows][top_k] kept values and ids
+  int* list_i;
+};
+struct VfPart {                 // of a slice of a row
+  float m, z;
+};
+struct VfKept {
+  double z;
+  unsigned long long thr;       // (key, ~id) of the last entry kept
+  float top;
+  int pad;
+};
 
 __device__ __forceinline__ unsigned int vf_key(float v) {
   if (v == 0.f) v = 0.f;                                   // the two zeros are equal
@@ -27,220 +68,776 @@ __device__ __forceinline__ unsigned int vf_key(float v) {
   const unsigned int b = __float_as_uint(v);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);       // larger float -> larger key
 }
+__device__ __forceinline__ float vf_value(unsigned int key) {
+  return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+}
+// Larger value first, of equals the lower id.
+__device__ __forceinline__ unsigned long long vf_rank(float v, int id) {
+  return ((unsigned long long)vf_key(v) << 32) | (0xffffffffu - (unsigned)id);
+}
+__device__ __forceinline__ float vf_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ VfPart vf_merge(VfPart a, VfPart b, float c) {
+  VfPart r;
+  r.m = fmaxf(a.m, b.m);
+  r.z = (a.m == r.m ? a.z : a.z * vf_ex2((a.m - r.m) * c)) + (b.m == r.m ? b.z : b.z * vf_ex2((b.m - r.m) * c));
+  return r;
+}
 
-template <typename V, typename Op>
-__device__ __forceinline__ V vf_reduce(V v, V* scratch, Op op) {
+// The drafts of sequence b and its first row; false where it has no such rows.
+__device__ __forceinline__ bool vf_sequence(const VfArgs& a, int b, int& row0, int& n) {
+  row0 = a.cu[b];
+  n = a.cu[b + 1] - row0 - 1;
+  return n >= 0 && n <= a.K && row0 >= 0 && row0 <= a.n_rows - 1 - n;
+}
+// Row i of the first launch, null where there is none to look at.
+__device__ __forceinline__ const float* vf_row(const VfArgs& a, int i) {
+  if (i < a.n_rows) return a.logits + (size_t)i * a.ld;
+  const int at = i - a.n_rows, b = at / a.K, j = at - b * a.K;
+  int row0, n;
+  if (!vf_sequence(a, b, row0, n) || j >= n) return nullptr;
+  return a.draft_logits + b * a.ld_seq + j * a.ld_place;
+}
+
+// ---- first launch: maximum and sum, or arg max, of a slice of a row.  A thread asks for all of its
+// NV vectors at once.  Rows may begin anywhere: the vectors begin at the first 16-byte boundary, the
+// up to three entries before it and behind the last vector are the first slice's.
+constexpr int kVsThreads = 256;
+
+template <int NV, bool GREEDY>
+__global__ void __launch_bounds__(kVsThreads)
+verify_rows_kernel(const __grid_constant__ VfArgs a) {
+  __shared__ VfPart part[kVsThreads / 32];
+  __shared__ unsigned long long best_s[kVsThreads / 32];
+  dependent_begin();
+  const int tid = threadIdx.x, slice = blockIdx.y;
+  const float* x = vf_row(a, blockIdx.x);
+  if (!x) return;
+  const int head = min(a.V, (int)((0u - (unsigned)((uintptr_t)x >> 2)) & 3u));
+  const int n4 = (a.V - head) >> 2;
+  const float4* x4 = reinterpret_cast<const float4*>(x + head);
+  const int v0 = slice * a.slice_vectors, v1 = min(n4, v0 + a.slice_vectors);
+  const float c = (float)a.log2_t;
+  const float ninf = -INFINITY;
+  VfPart mine{ninf, 0.f};
+  unsigned long long best = 0ull;
+  // (entries behind the slice are NaN: they count for nothing, not even in a row of -infinity)
+  const float none = __uint_as_float(0x7fffffffu);
+  for (int base = v0; base < v1; base += NV * kVsThreads) {
+    float v[4 * NV];
+    int n_mine = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = scratch[threadIdx.x & 31];                           // 32 warps
+    for (int i = 0; i < NV; ++i) {
+      const int at = base + i * kVsThreads + tid;
+      float4 f = make_float4(none, none, none, none);
+      if (at < v1) { f = __ldcs(x4 + at); n_mine += 4; }
+      v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+    }
+    if (GREEDY) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+      for (int i = 0; i < 4 * NV; ++i) {
+        const int at = base + (i >> 2) * kVsThreads + tid;
+        const unsigned long long k = at < v1 ? vf_rank(v[i], head + 4 * at + (i & 3)) : 0ull;
+        best = k > best ? k : best;
+      }
+    } else {
+      // NaN in place: fmaxf passes it over; its term must be nothing as well
+      float m = ninf;
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) m = fmaxf(m, v[i]);
+      VfPart p{m, 0.f};
+      if (fabsf(m) != INFINITY) {
+        float z[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4 * NV; ++i) z[i & 1] += vf_ex2((fmaxf(v[i], ninf) - m) * c);
+        p.z = z[0] + z[1];
+      } else if (n_mine) {
+        // equal infinities count 1 each (a NaN that is the row's as -infinity)
+        int equal = 0;
+#pragma unroll
+        for (int i = 0; i < 4 * NV; ++i)
+          equal += base + (i >> 2) * kVsThreads + tid < v1 && fmaxf(v[i], ninf) == m;
+        p.z = (float)equal;
+      }
+      if (n_mine) mine = vf_merge(mine, p, c);
+    }
+  }
+  if (slice == 0) {
+    const int tail = a.V - head - 4 * n4;
+    if (tid < head + tail) {
+      const int id = tid < head ? tid : 4 * n4 + tid;
+      const float v = x[id];
+      if (GREEDY) {
+        const unsigned long long k = vf_rank(v, id);
+        best = k > best ? k : best;
+      } else {
+        mine = vf_merge(mine, VfPart{fmaxf(v, ninf), 1.f}, c);
+      }
+    }
+  }
+  if (GREEDY) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
+      best = k > best ? k : best;
+    }
+    if ((tid & 31) == 0) best_s[tid >> 5] = best;
+  } else {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      VfPart p;
+      p.m = __shfl_xor_sync(0xffffffffu, mine.m, o);
+      p.z = __shfl_xor_sync(0xffffffffu, mine.z, o);
+      mine = vf_merge(mine, p, c);
+    }
+    if ((tid & 31) == 0) part[tid >> 5] = mine;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    const size_t at = (size_t)blockIdx.x * a.slices + slice;
+    if (GREEDY) {
+      for (int w = 1; w < kVsThreads / 32; ++w) best = best_s[w] > best ? best_s[w] : best;
+      static_cast<unsigned long long*>(a.stats)[at] = best;
+    } else {
+      for (int w = 1; w < kVsThreads / 32; ++w) mine = vf_merge(mine, part[w], c);
+      static_cast<VfPart*>(a.stats)[at] = mine;
+    }
+  }
+}
+
+// ---- second launch, greedy: a warp a sequence
+__global__ void __launch_bounds__(128) verify_greedy_kernel(const __grid_constant__ VfArgs a) {
+  dependent_begin();
+  const int b = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (b >= a.B) return;
+  int row0, n;
+  int* out = a.tokens + (size_t)b * a.ld_tokens;
+  if (!vf_sequence(a, b, row0, n)) {
+    for (int j = lane; j <= a.K; j += 32) out[j] = -1;
+    if (lane == 0) { a.accepted[b] = 0; atomicOr(a.fault, (unsigned)kFaultTokenRange); }
+    return;
+  }
+  // a lane a place: its row's arg max, and whether its draft is that
+  int accepted = n, next = 0;
+  bool found = false;
+  for (int j0 = 0; j0 <= n && !found; j0 += 32) {
+    const int j = j0 + lane;
+    int best = -1, d = -1;
+    if (j <= n) {
+      const unsigned long long* s = static_cast<const unsigned long long*>(a.stats) + (size_t)(row0 + j) * a.slices;
+      unsigned long long k = 0ull;
+      for (int i = 0; i < a.slices; ++i) k = s[i] > k ? s[i] : k;
+      best = (int)(0xffffffffu - (unsigned)k);
+      if (j < n) {
+        d = a.drafts[(size_t)b * a.ld_drafts + j];
+        if (d < 0 || d >= a.V) d = -2;
+      }
+    }
+    const unsigned stop = __ballot_sync(0xffffffffu, j <= n && (j == n || d != best));
+    if (stop) {
+      const int at = __ffs(stop) - 1;
+      accepted = j0 + at;
+      next = __shfl_sync(0xffffffffu, best, at);
+      if (lane == at && d == -2) atomicOr(a.fault, (unsigned)kFaultTokenRange);
+      found = true;
+    }
+  }
+  for (int j = lane; j <= a.K; j += 32)
+    out[j] = j < accepted ? a.drafts[(size_t)b * a.ld_drafts + j] : j == accepted ? next : -1;
+  if (lane == 0) a.accepted[b] = accepted;
+}
+
+// ---- second launch, whole vocabulary: a cluster a sequence, its CTAs share the vocabulary
+constexpr int kVdThreads = 512, kVdSeg = 128;             // entries a warp takes at once
+
+// 2^t, t <= 0, in 64 bits: t = n / 32 + f, 2^(n / 32) from a table of 32 and a power of two, 2^f by
+// its series to the fifth power (|f| <= 1/64: the sixth term is below 2.3e-15) (table-driven
+// exponential, P. T. P. Tang, 1989).  Nine 64-bit operations; the library's has about twice as many.
+__device__ __forceinline__ double vf_exp2(double t, const double* table) {
+  t = fmax(t, -1100.0);
+  const double magic = 6755399441055744.0;                // 1.5 * 2^52: rounds to an integer
+  const double big = fma(t, 32.0, magic);
+  const int n = __double2loint(big);
+  const double f = fma(big - magic, -1.0 / 32.0, t);
+  // ln2^k / k!
+  double p = fma(f, 0.0013333558146428441, 0.0096181291076284772);
+  p = fma(f, p, 0.055504108664821580);
+  p = fma(f, p, 0.24022650695910072);
+  p = fma(f, p, 0.69314718055994531);
+  p = fma(f, p, 1.0);
+  p *= table[n & 31];
+  const int e = n >> 5;
+  if (e < -1020) return 0.0;
+  return __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p));
+}
+
+struct VfTerm {                 // a row's terms in 64 bits
+  double c;                     // log2 e / T
+  float top;                    // the row's maximum
+  bool infinite;
+  __device__ __forceinline__ void set(float top_, double c_) {
+    top = top_;
+    c = c_;
+    infinite = fabsf(top_) == INFINITY;
+  }
+  __device__ __forceinline__ double operator()(float v, const double* table) const {
+    v = fmaxf(v, -INFINITY);                              // (NaN)
+    if (v == top) return 1.0;
+    if (infinite) return 0.0;
+    return vf_exp2(((double)v - (double)top) * c, table);
+  }
+};
+
+__device__ __forceinline__ double vf_warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-struct VfRow {                // a row's distribution: kept are (key, id) at or before the threshold
-  const float* x;
-  unsigned int top;           // key of the largest
-  float top_value;
-  unsigned int thr;           // key of the last one kept, and its largest kept id
-  int thr_id;
-  double total;
-};
-
-// A kept entry's term (0 where it is not kept).
-__device__ __forceinline__ double vf_term(const VfRow& r, int i, double inv_t) {
-  const float v = r.x[i];
-  const unsigned int k = vf_key(v);
-  if (k < r.thr || (k == r.thr && i > r.thr_id)) return 0.0;
-  return k == r.top ? 1.0 : v != v ? 0.0 : exp(((double)v - (double)r.top_value) * inv_t);
-}
-
-struct VfShared {
-  unsigned int u[32];
-  double d[32];
-  int i[32];
-  int hist[256];
-  unsigned int prefix;
-  int need;
-};
-
-__device__ void vf_row(VfRow& r, const float* x, int V, int top_k, double inv_t, VfShared& s) {
-  const int tid = threadIdx.x;
-  r.x = x;
-  unsigned int best = 0u;
-  for (int i = tid; i < V; i += kVfThreads) best = max(best, vf_key(x[i]));
-  best = vf_reduce(best, s.u, [](unsigned a, unsigned b) { return a > b ? a : b; });
-  r.top = best;
-  r.top_value = __uint_as_float((best & 0x80000000u) ? (best & 0x7fffffffu) : ~best);
-  r.thr = 0u;
-  r.thr_id = V - 1;
-  if (top_k > 0 && top_k < V) {
-    // the key of the k-th largest, 8 bits at a time, then the id of the last of its equals kept
-    if (tid == 0) { s.prefix = 0u; s.need = top_k; }
-    for (int pass = 0; pass < 4; ++pass) {
-      const int shift = 24 - 8 * pass;
-      if (tid < 256) s.hist[tid] = 0;
-      __syncthreads();
-      const unsigned int mask = pass == 0 ? 0u : 0xffffffffu << (shift + 8), prefix = s.prefix;
-      for (int i = tid; i < V; i += kVfThreads) {
-        const unsigned int k = vf_key(x[i]);
-        if ((k & mask) == prefix) atomicAdd(&s.hist[(k >> shift) & 255u], 1);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int need = s.need, b = 255;
-        for (; b > 0 && s.hist[b] < need; --b) need -= s.hist[b];
-        s.prefix = prefix | ((unsigned int)b << shift);
-        s.need = need;
-      }
-      __syncthreads();
-    }
-    r.thr = s.prefix;
-    // equals of the threshold in id order: the need-th one's id
-    int left = s.need, id = V - 1;
-    for (int i0 = 0; i0 < V && left > 0; i0 += kVfThreads) {
-      const bool eq = i0 + tid < V && vf_key(x[i0 + tid]) == r.thr;
-      const int n = __syncthreads_count(eq);
-      if (n >= left) {
-        const unsigned int mine = __ballot_sync(0xffffffffu, eq);
-        __syncthreads();
-        if ((tid & 31) == 0) s.i[tid >> 5] = __popc(mine);
-        __syncthreads();
-        int before = 0;
-        for (int w = 0; w < (tid >> 5); ++w) before += s.i[w];
-        before += __popc(mine & ((1u << (tid & 31)) - 1u));
-        if (eq && before == left - 1) s.need = i0 + tid;
-        __syncthreads();
-        id = s.need;
-      }
-      left -= n;
-    }
-    r.thr_id = id;
+// The entries 4 i .. 4 i + 3 of a row (NaN behind its end).
+__device__ __forceinline__ void vf_four(const float* x, int V, int i, bool aligned, float (&v)[4]) {
+  if (aligned && 4 * i + 3 < V) {
+    const float4 f = __ldg(reinterpret_cast<const float4*>(x) + i);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = 4 * i + e < V ? __ldg(x + 4 * i + e) : __uint_as_float(0x7fffffffu);
   }
-  double sum = 0.0;
-  for (int i = tid; i < V; i += kVfThreads) sum += vf_term(r, i, inv_t);
-  r.total = vf_reduce(sum, s.d, [](double a, double b) { return a + b; });
 }
 
-__global__ void __launch_bounds__(kVfThreads)
-verify_kernel(const float* __restrict__ logits, int ld, const int* __restrict__ cu, int n_rows,
-              const int* __restrict__ drafts, int ld_drafts, int K, const float* __restrict__ draft_logits,
-              long long ld_seq, long long ld_place, const float* __restrict__ accept_u, int ld_u,
-              const float* __restrict__ next_u, int V, double temperature, int top_k,
-              int* __restrict__ accepted, int* __restrict__ tokens, int ld_tokens,
-              unsigned int* __restrict__ fault) {
-  __shared__ VfShared s;
-  const int b = blockIdx.x, tid = threadIdx.x;
+__global__ void __launch_bounds__(kVdThreads)
+verify_draw_kernel(const __grid_constant__ VfArgs a) {
+  extern __shared__ double vd_smem[];                     // sums of the CTA's segments
+  __shared__ double table[32];
+  __shared__ double sums[kVdThreads / 32];
+  __shared__ double shared_tot[3];                        // this CTA's: p, q, what is drawn from
+  __shared__ int first_bad;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int kWarps = kVdThreads / 32;
+  if (tid < 32) table[tid] = exp2((double)tid / 32.0);
+  if (tid == 0) first_bad = 0x7fffffff;
   dependent_begin();
-  const int row0 = cu[b];
-  int n = cu[b + 1] - row0 - 1;
-  if (n < 0 || n > K || row0 < 0 || row0 + n >= n_rows) {      // no row of the logits, or more drafts than there are
-    if (tid == 0) {
-      atomicOr(fault, (unsigned)kFaultTokenRange);
-      accepted[b] = 0;
+  __syncthreads();
+  int row0, n;
+  int* out = a.tokens + (size_t)b * a.ld_tokens;
+  if (!vf_sequence(a, b, row0, n)) {                      // (all CTAs of the cluster alike)
+    if (rank == 0) {
+      for (int j = tid; j <= a.K; j += kVdThreads) out[j] = -1;
+      if (tid == 0) { a.accepted[b] = 0; atomicOr(a.fault, (unsigned)kFaultTokenRange); }
     }
-    for (int j = tid; j <= K; j += kVfThreads) tokens[(size_t)b * ld_tokens + j] = -1;
     return;
   }
-  const bool greedy = temperature <= 0.0;
-  const double inv_t = greedy ? 1.0 : 1.0 / temperature;
-  int j = 0, next = 0;
-  VfRow p, q;
-  for (;; ++j) {
-    const float* x = logits + (size_t)(row0 + j) * ld;
-    if (greedy) {
-      unsigned long long best = 0ull;
-      for (int i = tid; i < V; i += kVfThreads) {
-        const unsigned long long k = ((unsigned long long)vf_key(x[i]) << 32) | (0xffffffffu - (unsigned)i);
-        if (k > best) best = k;
+  // ---- which drafts stand: a warp a draft
+  const float cf = (float)a.log2_t;
+  const VfPart* stats = static_cast<const VfPart*>(a.stats);
+  auto whole = [&](int row) {                             // a row's maximum and sum
+    VfPart p{-INFINITY, 0.f};
+    for (int i = lane; i < a.slices; i += 32) p = vf_merge(p, stats[(size_t)row * a.slices + i], cf);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      VfPart q;
+      q.m = __shfl_xor_sync(0xffffffffu, p.m, o);
+      q.z = __shfl_xor_sync(0xffffffffu, p.z, o);
+      p = vf_merge(p, q, cf);
+    }
+    return p;
+  };
+  for (int j = warp; j < n; j += kWarps) {
+    const int d = a.drafts[(size_t)b * a.ld_drafts + j];
+    const bool in = d >= 0 && d < a.V;
+    bool stands = false;
+    if (in) {
+      VfTerm t;
+      const VfPart p = whole(row0 + j);
+      t.set(p.m, a.log2_t);
+      const double px = t(a.logits[(size_t)(row0 + j) * a.ld + d], table) / (double)p.z;
+      double qx = 1.0;
+      if (a.draft_logits) {
+        const VfPart q = whole(a.n_rows + b * a.K + j);
+        t.set(q.m, a.log2_t);
+        qx = t(a.draft_logits[b * a.ld_seq + j * a.ld_place + d], table) / (double)q.z;
       }
-      best = vf_reduce(best, reinterpret_cast<unsigned long long*>(s.d),
-                       [](unsigned long long a, unsigned long long c) { return a > c ? a : c; });
-      next = (int)(0xffffffffu - (unsigned)best);
-    } else {
-      vf_row(p, x, V, top_k, inv_t, s);
+      stands = (double)a.accept_u[(size_t)b * a.ld_u + j] * qx < px;
     }
-    if (j == n) break;
-    const int d = drafts[(size_t)b * ld_drafts + j];
-    const bool in = d >= 0 && d < V;
-    if (!in && tid == 0) atomicOr(fault, (unsigned)kFaultTokenRange);
-    bool stands;
-    if (greedy) {
-      stands = in && d == next;
-    } else {
-      if (draft_logits) vf_row(q, draft_logits + b * ld_seq + j * ld_place, V, top_k, inv_t, s);
-      const double u = accept_u[(size_t)b * ld_u + j];
-      const double px = in ? vf_term(p, d, inv_t) / p.total : 0.0;
-      const double qx = !in ? 0.0 : draft_logits ? vf_term(q, d, inv_t) / q.total : 1.0;
-      stands = in && u * qx < px;
-    }
-    if (!stands) break;
+    if (!stands && lane == 0) atomicMin(&first_bad, j);
   }
-  if (!greedy) {
-    // the token: from max(p - q, 0) behind a draft that did not stand, else (and where nothing is
-    // left of p) from p
-    const bool rest = j < n;
-    const int d = rest ? drafts[(size_t)b * ld_drafts + j] : -1;
-    const double wq = rest && draft_logits ? p.total / q.total : 0.0;
-    auto term = [&](int i, bool minus) {
-      double v = vf_term(p, i, inv_t);
-      if (!minus) return v;
-      if (draft_logits) return fmax(v - wq * vf_term(q, i, inv_t), 0.0);
-      return i == d ? 0.0 : v;
+  __syncthreads();
+  const int j = min(first_bad, n);
+  const bool rest = j < n;
+  const int d = rest ? a.drafts[(size_t)b * a.ld_drafts + j] : -1;
+  if (rest && (d < 0 || d >= a.V) && rank == 0 && tid == 0) atomicOr(a.fault, (unsigned)kFaultTokenRange);
+  // ---- the row (two rows) to draw from
+  const bool minus_q = rest && a.draft_logits != nullptr;
+  const float* xp = a.logits + (size_t)(row0 + j) * a.ld;
+  const float* xq = minus_q ? a.draft_logits + b * a.ld_seq + j * a.ld_place : xp;
+  const bool ap = ((uintptr_t)xp & 15) == 0, aq = ((uintptr_t)xq & 15) == 0;
+  VfTerm tp, tq;
+  tp.set(whole(row0 + j).m, a.log2_t);
+  tq = tp;
+  if (minus_q) tq.set(whole(a.n_rows + b * a.K + j).m, a.log2_t);
+  const int segs = (a.V + kVdSeg - 1) / kVdSeg;
+  const int s0 = (int)((long long)segs * rank / C), s1 = (int)((long long)segs * (rank + 1) / C);
+  auto block_total = [&](double v, double* where) {       // into *where of this CTA
+    v = vf_warp_sum(v);
+    if (lane == 0) sums[warp] = v;
+    __syncthreads();
+    if (tid == 0) {
+      double t = 0.0;
+      for (int w = 0; w < kWarps; ++w) t += sums[w];
+      *where = t;
+    }
+    __syncthreads();
+  };
+  double weight = 0.0;                                    // of q's terms beside p's
+  if (minus_q) {
+    double zp = 0.0, zq = 0.0;
+    for (int s = s0 + warp; s < s1; s += kWarps) {
+      float vp[4], vq[4];
+      vf_four(xp, a.V, s * 32 + lane, ap, vp);
+      vf_four(xq, a.V, s * 32 + lane, aq, vq);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool there = s * kVdSeg + 4 * lane + e < a.V;
+        zp += there ? tp(vp[e], table) : 0.0;
+        zq += there ? tq(vq[e], table) : 0.0;
+      }
+    }
+    block_total(zp, &shared_tot[0]);
+    block_total(zq, &shared_tot[1]);
+    cluster.sync();
+    double all_p = 0.0, all_q = 0.0;
+    for (int r = 0; r < C; ++r) {
+      const double* there = cluster.map_shared_rank(shared_tot, r);
+      all_p += there[0];
+      all_q += there[1];
+    }
+    weight = all_p / all_q;
+  }
+  for (int turn = rest ? 0 : 1; turn < 2; ++turn) {       // (the second where p and q leave nothing)
+    const bool minus = turn == 0;
+    // the four terms of a lane in a segment
+    auto terms = [&](int s, double (&v)[4]) {
+      float vp[4], vq[4];
+      vf_four(xp, a.V, s * 32 + lane, ap, vp);
+      if (minus && minus_q) vf_four(xq, a.V, s * 32 + lane, aq, vq);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int id = s * kVdSeg + 4 * lane + e;
+        double t = id < a.V ? tp(vp[e], table) : 0.0;
+        if (minus) {
+          if (minus_q) t = id < a.V ? fmax(t - weight * tq(vq[e], table), 0.0) : 0.0;
+          else if (id == d) t = 0.0;
+        }
+        v[e] = t;
+      }
     };
-    const int chunk = (V + kVfThreads - 1) / kVfThreads, lo = min(V, tid * chunk), hi = min(V, lo + chunk);
-    for (int turn = rest ? 0 : 1; turn < 2; ++turn) {
-      double mine = 0.0;
-      for (int i = lo; i < hi; ++i) mine += term(i, turn == 0);
-      double inc = mine;
+    double mine = 0.0;
+    for (int s = s0 + warp; s < s1; s += kWarps) {
+      double v[4];
+      terms(s, v);
+      const double sum = vf_warp_sum((v[0] + v[1]) + (v[2] + v[3]));
+      if (lane == 0) {
+        vd_smem[s - s0] = sum;
+        mine += sum;
+      }
+    }
+    block_total(mine, &shared_tot[2]);
+    cluster.sync();
+    double total = 0.0, base = 0.0;
+    int last_rank = -1;
+    for (int r = 0; r < C; ++r) {
+      const double t = cluster.map_shared_rank(shared_tot, r)[2];
+      if (r == rank) base = total;
+      if (t > 0.0) last_rank = r;
+      total += t;
+    }
+    cluster.sync();                                       // nobody leaves, or writes again, before all have read
+    if (!(total > 0.0)) continue;
+    // (a number that is not in [0, 1) counts as the nearest that is)
+    double goal = (double)a.next_u[b] * total;
+    if (!(goal >= 0.0)) goal = 0.0;
+    const bool past = goal >= total;                      // the last id with any
+    const bool here = past ? rank == last_rank : base <= goal && goal < base + shared_tot[2];
+    if (here && warp == 0) {
+      // the segment, 32 at a time, and the place in it
+      double run = base;
+      int seg = -1, last_seg = -1;
+      double seg_base = 0.0;
+      for (int i0 = 0; i0 < s1 - s0 && seg < 0; i0 += 32) {
+        const double v = i0 + lane < s1 - s0 ? vd_smem[i0 + lane] : 0.0;
+        double inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double w = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += w;
+        }
+        const unsigned any = __ballot_sync(0xffffffffu, v > 0.0);
+        const unsigned hit = past ? 0u : __ballot_sync(0xffffffffu, v > 0.0 && run + inc > goal);
+        if (hit) {
+          seg = i0 + __ffs(hit) - 1;
+          double before = __shfl_up_sync(0xffffffffu, inc, 1);
+          if (lane == 0) before = 0.0;
+          seg_base = run + __shfl_sync(0xffffffffu, before, __ffs(hit) - 1);
+        }
+        if (any) last_seg = i0 + 31 - __clz(any);
+        run += __shfl_sync(0xffffffffu, inc, 31);
+      }
+      const bool take_last = seg < 0;                     // (rounding passed the last border)
+      if (take_last) seg = last_seg;
+      double v[4];
+      terms(s0 + seg, v);
+      const double four = (v[0] + v[1]) + (v[2] + v[3]);
+      double inc = four;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, inc, o);
-        if ((tid & 31) >= o) inc += v;
+        const double w = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += w;
       }
-      // a thread's interval [before, after): each begins exactly where the one before it ends
-      double prev = __shfl_up_sync(0xffffffffu, inc, 1);
-      if ((tid & 31) == 0) prev = 0.0;
-      __syncthreads();
-      if ((tid & 31) == 31) s.d[tid >> 5] = inc;
-      if (tid == 0) s.need = -1;
-      __syncthreads();
-      double base = 0.0, total = 0.0;
-      for (int w = 0; w < 32; ++w) {
-        if (w == (tid >> 5)) base = total;
-        total += s.d[w];
-      }
-      if (!(total > 0.0)) continue;
-      const double goal = (double)next_u[b] * total;
-      if (base + prev <= goal && goal < base + inc) {
-        double run = base + prev;
-        int at = -1;
-        for (int i = lo; i < hi; ++i) {
-          const double v = term(i, turn == 0);
-          if (v > 0.0) at = i;                 // (the chunk's last one where rounding passes its end)
-          run += v;
-          if (run > goal) break;
+      double run4 = seg_base + inc - four;
+      int first = 0x7fffffff, last = -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int id = (s0 + seg) * kVdSeg + 4 * lane + e;
+        run4 += v[e];
+        if (v[e] > 0.0) {
+          last = id;
+          if (!take_last && run4 > goal && first == 0x7fffffff) first = id;
         }
-        s.need = at;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+        last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+      }
+      const int next = first != 0x7fffffff ? first : last;
+      for (int i = lane; i <= a.K; i += 32)
+        out[i] = i < j ? a.drafts[(size_t)b * a.ld_drafts + i] : i == j ? next : -1;
+      if (lane == 0) a.accepted[b] = j;
+    }
+    break;
+  }
+}
+
+// ---- top_k: a CTA a row finds the kept entries.
+// The k-th largest of the threads' own maxima is at most the row's k-th largest; the entries at or
+// above it are few more than k.  They are listed in a second look at the row (from L2) and sorted by
+// (value, id).  Where they are too many for the list (equal logits in masses) the k-th largest is
+// found digit by digit over the whole row.
+constexpr int kVkThreads = 1024, kVkList = 4096;
+
+struct VkShared {
+  unsigned long long list[kVkList];
+  double sums[32];
+  unsigned int hist[256];
+  unsigned int digit, need, count;
+  unsigned int best[32];
+};
+
+// The key of the need-th largest of what `each` hands to its argument, 8 bits at a time; `need` is
+// left as how many equals of it are among them.
+template <typename Each>
+__device__ __forceinline__ unsigned int vk_select(VkShared& s, unsigned int need, unsigned int& equal_need, Each each) {
+  const int tid = threadIdx.x;
+  unsigned int prefix = 0u;
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    const unsigned int mask = pass == 0 ? 0u : 0xffffffffu << (shift + 8);
+    if (tid < 256) s.hist[tid] = 0u;
+    __syncthreads();
+    each([&](unsigned int k) {
+      if ((k & mask) == prefix) atomicAdd(&s.hist[(k >> shift) & 255u], 1u);
+    });
+    __syncthreads();
+    if (tid < 32) {                        // lane l: digits 255 - 8 l down to 248 - 8 l
+      unsigned int c[8], sum = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { c[i] = s.hist[255 - 8 * tid - i]; sum += c[i]; }
+      unsigned int inc = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (tid >= o) inc += v;
+      }
+      unsigned int before = inc - sum;
+      if (before < need && inc >= need) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (before < need && before + c[i] >= need) {
+            s.digit = 255 - 8 * tid - i;
+            s.need = need - before;
+          }
+          before += c[i];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= s.digit << shift;
+    need = s.need;
+    __syncthreads();
+  }
+  equal_need = need;
+  return prefix;
+}
+
+__global__ void __launch_bounds__(kVkThreads)
+verify_kept_kernel(const __grid_constant__ VfArgs a) {
+  __shared__ VkShared s;
+  dependent_begin();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V, k = a.top_k;
+  const float* x = vf_row(a, blockIdx.x);
+  if (!x) return;
+  const int head = min(V, (int)((0u - (unsigned)((uintptr_t)x >> 2)) & 3u));
+  const int n4 = (V - head) >> 2, tail = V - head - 4 * n4;
+  const float4* x4 = reinterpret_cast<const float4*>(x + head);
+  // f(value, id) for every entry of the row, a thread's in ascending order of id but the odd ones
+  auto each = [&](auto f) {
+    constexpr int U = 4;
+    for (int i0 = tid; i0 < n4; i0 += U * kVkThreads) {
+      float4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * kVkThreads < n4) v[u] = __ldg(x4 + i0 + u * kVkThreads);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kVkThreads;
+        if (i < n4) {
+          f(v[u].x, head + 4 * i); f(v[u].y, head + 4 * i + 1); f(v[u].z, head + 4 * i + 2); f(v[u].w, head + 4 * i + 3);
+        }
+      }
+    }
+    if (tid < head + tail) {
+      const int id = tid < head ? tid : 4 * n4 + tid;
+      f(x[id], id);
+    }
+  };
+  unsigned int mine = 0u;
+  each([&](float v, int) { mine = max(mine, vf_key(v)); });
+  unsigned int best = __reduce_max_sync(0xffffffffu, mine);
+  if (lane == 0) s.best[warp] = best;
+  if (tid == 0) s.count = 0u;
+  __syncthreads();
+  best = __reduce_max_sync(0xffffffffu, s.best[lane]);
+  const float top = vf_value(best);
+  // (threads without entries hold key 0, below every entry's; there are at least k entries, and where
+  // V < 1,024 some of the k largest maxima may be such: everything is listed then)
+  unsigned int equal;
+  const unsigned int floor_key = vk_select(s, (unsigned)k, equal, [&](auto f) { f(mine); });
+  each([&](float v, int id) {
+    if (vf_key(v) >= floor_key) {
+      const unsigned int at = atomicAdd(&s.count, 1u);
+      if (at < kVkList) s.list[at] = vf_rank(v, id);
+    }
+  });
+  __syncthreads();
+  unsigned int n = s.count;
+  if (n > kVkList) {
+    // list the larger ones and the equals with the lowest ids: the equals' ids are taken in the row's order
+    const unsigned int kth = vk_select(s, (unsigned)k, equal, [&](auto f) { each([&](float v, int) { f(vf_key(v)); }); });
+    if (tid == 0) s.count = 0u;
+    __syncthreads();
+    each([&](float v, int id) {
+      if (vf_key(v) > kth) s.list[atomicAdd(&s.count, 1u)] = vf_rank(v, id);
+    });
+    __syncthreads();
+    unsigned int left = equal;
+    const unsigned int at0 = (unsigned)k - equal;
+    for (int i0 = 0; i0 < V && left > 0u; i0 += kVkThreads) {
+      const bool eq = i0 + tid < V && vf_key(x[i0 + tid]) == kth;
+      const unsigned int votes = __ballot_sync(0xffffffffu, eq);
+      if (lane == 0) s.best[warp] = __popc(votes);
+      __syncthreads();
+      unsigned int before = __popc(votes & ((1u << lane) - 1u)), all = 0u;
+      for (int w = 0; w < 32; ++w) {
+        if (w < warp) before += s.best[w];
+        all += s.best[w];
+      }
+      if (eq && before < left) s.list[at0 + (equal - left) + before] = vf_rank(x[i0 + tid], i0 + tid);
+      left -= min(left, all);
+      __syncthreads();
+    }
+    n = (unsigned)k;
+    __syncthreads();
+  }
+  // sort: the largest first
+  int np2 = 1;
+  while (np2 < (int)n) np2 <<= 1;
+  for (int i = (int)n + tid; i < np2; i += kVkThreads) s.list[i] = 0ull;
+  __syncthreads();
+  for (int size = 2; size <= np2; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      for (int i = tid; i < np2; i += kVkThreads) {
+        const int p = i ^ stride;
+        if (p > i) {
+          const unsigned long long u = s.list[i], v = s.list[p];
+          if ((u > v) != ((i & size) == 0)) { s.list[i] = v; s.list[p] = u; }
+        }
       }
       __syncthreads();
-      next = s.need;
-      if (next < 0) {                          // the number was not in [0, 1): the last id with any
-        __syncthreads();
-        int last = -1;
-        for (int i = lo; i < hi; ++i)
-          if (term(i, turn == 0) > 0.0) last = i;
-        next = vf_reduce(last, s.i, [](int a, int c) { return a > c ? a : c; });
-      }
-      break;
     }
+  // the kept ones, their sum in 64 bits
+  const double c = a.log2_t;
+  double z = 0.0;
+  if (tid < k) {
+    const unsigned long long r = s.list[tid];
+    const float v = vf_value((unsigned int)(r >> 32));
+    const size_t at = (size_t)blockIdx.x * k + tid;
+    a.list_v[at] = v;
+    a.list_i[at] = (int)(0xffffffffu - (unsigned)r);
+    z = v == top ? 1.0 : fabsf(top) == INFINITY ? 0.0 : exp2(((double)v - (double)top) * c);
   }
-  for (int i = tid; i <= K; i += kVfThreads)
-    tokens[(size_t)b * ld_tokens + i] = i < j ? drafts[(size_t)b * ld_drafts + i] : i == j ? next : -1;
-  if (tid == 0) accepted[b] = j;
+  z = vf_warp_sum(z);
+  if (lane == 0) s.sums[warp] = z;
+  __syncthreads();
+  if (tid == 0) {
+    double t = 0.0;
+    for (int w = 0; w < 32; ++w) t += s.sums[w];
+    static_cast<VfKept*>(a.stats)[blockIdx.x] = VfKept{t, s.list[k - 1], top, 0};
+  }
+}
+
+// ---- second launch, top_k: a CTA a sequence
+constexpr int kVlThreads = 256;
+
+__global__ void __launch_bounds__(kVlThreads)
+verify_kept_draw_kernel(const __grid_constant__ VfArgs a) {
+  __shared__ unsigned long long order[kVfMaxTopK];         // (id, place in the list), by id
+  __shared__ double term[kVfMaxTopK];
+  __shared__ double sums[kVlThreads / 32];
+  __shared__ int first_bad, chosen;
+  dependent_begin();
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.top_k;
+  constexpr int kWarps = kVlThreads / 32;
+  int row0, n;
+  int* out = a.tokens + (size_t)b * a.ld_tokens;
+  if (!vf_sequence(a, b, row0, n)) {
+    for (int j = tid; j <= a.K; j += kVlThreads) out[j] = -1;
+    if (tid == 0) { a.accepted[b] = 0; atomicOr(a.fault, (unsigned)kFaultTokenRange); }
+    return;
+  }
+  if (tid == 0) { first_bad = 0x7fffffff; chosen = -1; }
+  __syncthreads();
+  const VfKept* kept = static_cast<const VfKept*>(a.stats);
+  const double c = a.log2_t;
+  auto value = [&](const VfKept& r, float v, int id) {     // the term of a row's entry, 0 where it is not kept
+    if (vf_rank(v, id) < r.thr) return 0.0;
+    v = fmaxf(v, -INFINITY);
+    return v == r.top ? 1.0 : fabsf(r.top) == INFINITY ? 0.0 : exp2(((double)v - (double)r.top) * c);
+  };
+  for (int j = tid; j < n; j += kVlThreads) {              // a thread a draft
+    const int d = a.drafts[(size_t)b * a.ld_drafts + j];
+    bool stands = false;
+    if (d >= 0 && d < a.V) {
+      const VfKept p = kept[row0 + j];
+      const double px = value(p, a.logits[(size_t)(row0 + j) * a.ld + d], d) / p.z;
+      double qx = 1.0;
+      if (a.draft_logits) {
+        const VfKept q = kept[a.n_rows + b * a.K + j];
+        qx = value(q, a.draft_logits[b * a.ld_seq + j * a.ld_place + d], d) / q.z;
+      }
+      stands = (double)a.accept_u[(size_t)b * a.ld_u + j] * qx < px;
+    }
+    if (!stands) atomicMin(&first_bad, j);
+  }
+  __syncthreads();
+  const int j = min(first_bad, n);
+  const bool rest = j < n, minus_q = rest && a.draft_logits != nullptr;
+  const int d = rest ? a.drafts[(size_t)b * a.ld_drafts + j] : -1;
+  if (rest && (d < 0 || d >= a.V) && tid == 0) atomicOr(a.fault, (unsigned)kFaultTokenRange);
+  const VfKept p = kept[row0 + j];
+  const VfKept q = minus_q ? kept[a.n_rows + b * a.K + j] : p;
+  const float* xq = minus_q ? a.draft_logits + b * a.ld_seq + j * a.ld_place : nullptr;
+  const double weight = p.z / q.z;
+  const size_t list = (size_t)(row0 + j) * k;
+  int np2 = 1;
+  while (np2 < k) np2 <<= 1;
+  for (int i = tid; i < np2; i += kVlThreads)
+    order[i] = i < k ? ((unsigned long long)(unsigned)a.list_i[list + i] << 32) | (unsigned)i : ~0ull;
+  __syncthreads();
+  for (int size = 2; size <= np2; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      for (int i = tid; i < np2; i += kVlThreads) {
+        const int o = i ^ stride;
+        if (o > i) {
+          const unsigned long long u = order[i], v = order[o];
+          if ((u < v) != ((i & size) == 0)) { order[i] = v; order[o] = u; }
+        }
+      }
+      __syncthreads();
+    }
+  int next = 0;
+  for (int turn = rest ? 0 : 1; turn < 2; ++turn) {
+    // a thread's entries lie together: `per` of them
+    const int per = (k + kVlThreads - 1) / kVlThreads, lo = min(k, tid * per), hi = min(k, lo + per);
+    double mine = 0.0;
+    for (int i = lo; i < hi; ++i) {
+      const int id = (int)(order[i] >> 32);
+      double t = value(p, a.list_v[list + (unsigned)order[i]], id);
+      if (turn == 0) {
+        if (minus_q) t = fmax(t - weight * value(q, xq[id], id), 0.0);
+        else if (id == d) t = 0.0;
+      }
+      term[i] = t;
+      mine += t;
+    }
+    double inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    double prev = __shfl_up_sync(0xffffffffu, inc, 1);
+    if (lane == 0) prev = 0.0;
+    __syncthreads();
+    if (lane == 31) sums[warp] = inc;
+    __syncthreads();
+    double base = 0.0, total = 0.0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) base = total;
+      total += sums[w];
+    }
+    if (!(total > 0.0)) continue;
+    double goal = (double)a.next_u[b] * total;
+    if (!(goal >= 0.0)) goal = 0.0;
+    if (base + prev <= goal && goal < base + inc) {
+      double run = base + prev;
+      int at = -1;
+      for (int i = lo; i < hi; ++i) {
+        if (term[i] > 0.0) at = (int)(order[i] >> 32);     // (the last one where rounding passes the end)
+        run += term[i];
+        if (run > goal) break;
+      }
+      chosen = at;
+    }
+    __syncthreads();
+    const bool past = chosen < 0;
+    __syncthreads();
+    if (past) {                                            // the number was not below 1: the last id with any
+      for (int i = lo; i < hi; ++i)
+        if (term[i] > 0.0) atomicMax(&chosen, (int)(order[i] >> 32));
+      __syncthreads();
+    }
+    next = chosen;
+    break;
+  }
+  for (int i = tid; i <= a.K; i += kVlThreads)
+    out[i] = i < j ? a.drafts[(size_t)b * a.ld_drafts + i] : i == j ? next : -1;
+  if (tid == 0) a.accepted[b] = j;
+}
+
+// How the first launch cuts rows: vectors of four a slice, and slices.  A CTA takes 12 vectors a
+// thread where there are rows enough to fill the chip with such CTAs, else 4.
+static void vf_cut(const VfArgs& a, int rows, int& vectors, int& slices) {
+  const long long n4 = a.V / 4 + 1;
+  const long long big = (n4 + 12 * kVsThreads - 1) / (12 * kVsThreads);
+  const bool few = big * rows < 2 * kSmCount;
+  const long long per = (few ? 4 : 12) * kVsThreads;
+  vectors = (int)per;
+  slices = (int)((n4 + per - 1) / per);
 }
 
 }  // namespace cretif
@@ -249,19 +846,71 @@ using namespace cretif;
 
 extern "C" int cretif_max_top_k();
 
+extern "C" long long cretif_verify_scratch(int n_rows, int B, int K, int V, int top_k, int draft_rows) {
+  if (n_rows <= 0 || B < 0 || K < 0 || V <= 0) return 0;
+  const long long rows = (long long)n_rows + (draft_rows ? (long long)B * K : 0);
+  if (top_k > 0 && top_k < V) return rows * (long long)(sizeof(VfKept) + 8LL * top_k);
+  return rows * 8LL * (V / 4 / (4 * kVsThreads) + 1);
+}
+
 extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, const int* cu,
                                     const int* drafts, int ld_drafts, int K, const float* draft_logits,
                                     long long ld_seq, long long ld_place, const float* accept_u,
                                     int ld_u, const float* next_u, int B, int V, double temperature,
                                     int top_k, int* accepted, int* tokens, int ld_tokens,
-                                    unsigned int* fault, void* stream) {
+                                    void* scratch, unsigned int* fault, void* stream) {
   if (B <= 0) return kOk;
   if (V <= 0 || ld < V || K < 0 || n_rows <= 0 || ld_tokens < K + 1 || top_k < 0 || temperature != temperature ||
-      (temperature > 0 && top_k > cretif_max_top_k() && top_k < V) || (K > 0 && ld_drafts < K) ||
-      (draft_logits && ld_place < V))
+      (temperature > 0 && top_k > kVfMaxTopK && top_k < V) || (K > 0 && ld_drafts < K) ||
+      (draft_logits && ld_place < V) || B > 65535 || !scratch)
     return kBadArgument;
-  launch_dependent(verify_kernel, dim3(B), dim3(kVfThreads), 0, (cudaStream_t)stream, logits, ld, cu, n_rows,
-                   drafts, ld_drafts, K, draft_logits, ld_seq, ld_place, accept_u, ld_u, next_u, V,
-                   temperature, top_k, accepted, tokens, ld_tokens, fault);
-  return launch_status();
+  const bool greedy = temperature <= 0.0;
+  if (greedy) draft_logits = nullptr;
+  const long long rows = (long long)n_rows + (draft_logits ? (long long)B * K : 0);
+  const bool kept = !greedy && top_k > 0 && top_k < V;
+  if (rows > 0x7fffffffLL) return kBadArgument;
+  cudaStream_t st = (cudaStream_t)stream;
+  VfArgs a{logits, ld, n_rows, cu, drafts, ld_drafts, K, B, V, draft_logits, ld_seq, ld_place, accept_u, ld_u, next_u,
+           greedy ? 1.0 : fmin(fmax(1.4426950408889634 / temperature, 1e-30), 3e38), top_k, accepted, tokens, ld_tokens, fault, scratch, 0, 0,
+           nullptr, nullptr};
+  if (kept) {
+    a.list_v = reinterpret_cast<float*>(static_cast<char*>(scratch) + rows * sizeof(VfKept));
+    a.list_i = reinterpret_cast<int*>(a.list_v + rows * top_k);
+    launch_dependent(verify_kept_kernel, dim3((unsigned)rows), dim3(kVkThreads), 0, st, a);
+    launch_dependent(verify_kept_draw_kernel, dim3(B), dim3(kVlThreads), 0, st, a);
+    return launch_status();
+  }
+  vf_cut(a, (int)rows, a.slice_vectors, a.slices);
+  const dim3 grid((unsigned)rows, a.slices);
+  const bool big = a.slice_vectors == 12 * kVsThreads;
+  if (greedy) {
+    launch_dependent(big ? verify_rows_kernel<12, true> : verify_rows_kernel<4, true>, grid, dim3(kVsThreads), 0, st, a);
+    launch_dependent(verify_greedy_kernel, dim3((B + 3) / 4), dim3(128), 0, st, a);
+    return launch_status();
+  }
+  launch_dependent(big ? verify_rows_kernel<12, false> : verify_rows_kernel<4, false>, grid, dim3(kVsThreads), 0, st, a);
+  // CTAs a sequence: enough to fill the chip about once, at least 1,024 entries each
+  int C = 8;
+  while (C > 1 && (B * C > 4 * kSmCount || V < 1024 * C)) C >>= 1;
+  const int segs = ((V + kVdSeg - 1) / kVdSeg + C - 1) / C + 1;
+  const size_t smem = (size_t)segs * 8;
+  if (smem > 200 * 1024) return kBadArgument;
+  cudaError_t e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = dependent_launch_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C, B);
+  cfg.blockDim = dim3(kVdThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, verify_draw_kernel, a);
+  return e == cudaSuccess ? launch_status() : (int)e;
 }
