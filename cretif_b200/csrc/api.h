@@ -574,14 +574,14 @@ int cretif_verify_drafts(const float* logits, int ld, int n_rows, const int* cu,
                          int ld_tokens, void* scratch, unsigned int* fault, void* stream);
 
 // Attention of few new tokens a sequence where groups of sequences share prefixes (attn_shared.cu).
-// plan: int32, n_pre prefix items of 8, n_own own items of 4, n_rows token rows of the groups, [T]
-// prefix pieces and [T] sequence of a token, [B] prefix of a sequence.  part_o
-// [max_pieces, T * nh, hd], part_ml [max_pieces, T * nh, 2]: scratch.
+// plan: int32, n_pre prefix items of 8, n_own own items of 8 (each of up to own_rows rows), n_rows
+// tokens of the groups, [T] prefix pieces of a token.  part_o [max_pieces, T * nh, hd], part_ml
+// [max_pieces, T * nh, 2]: scratch.
 int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int ldo, const void* kc,
                        const void* vc, long long n_blocks, const int* table, int table_stride,
-                       int n_slots, const int* tok_pos, const int* cu, const int* seq_slot,
-                       const int* plan, int n_pre, int n_own, int own_splits, int max_pieces,
-                       int n_rows, int B, int T, int nh, int nkv, int hd, int bt, float scale,
+                       int n_slots, const int* tok_pos, const int* seq_slot, const int* plan,
+                       int n_pre, int n_own, int own_rows, int own_splits, int max_pieces,
+                       int n_rows, int T, int nh, int nkv, int hd, int bt, float scale,
                        const float* sink, float* part_o, float* part_ml, unsigned int* fault,
                        void* stream);
 

@@ -26,7 +26,7 @@ shared_pieces_kernel(const SharedArgs a) {
   dependent_begin();
 
   // ---- this block's rows and keys
-  int seq, row0, n_rows, row_base = -1, key0, key_end, piece;
+  int seq, row0, n_rows, row_base = -1, tok0 = 0, key0, key_end, piece;
   if ((int)blockIdx.x < a.n_pre) {
     const SharedPrefixItem it = a.pre[blockIdx.x];
     seq = it.seq; row0 = it.row0; n_rows = it.n_rows; row_base = it.row_base;
@@ -34,16 +34,16 @@ shared_pieces_kernel(const SharedArgs a) {
   } else {
     const int x = blockIdx.x - a.n_pre, split = x % a.own_splits;
     const SharedOwnItem it = a.own[x / a.own_splits];
-    seq = it.seq; row0 = it.row0; n_rows = it.n_rows;
-    const int prefix = a.seq_prefix[seq];
-    const int end = shared_own_end(a, seq, a.tok_pos[a.cu[seq] + (row0 + n_rows - 1) / g]);
+    seq = it.seq; row0 = it.row0; n_rows = it.n_rows; tok0 = it.tok0;
+    const int prefix = it.prefix;
+    const int end = shared_own_end(a, prefix, a.tok_pos[tok0 + (row0 + n_rows - 1) / g]);
     const int blocks = (end - prefix + kShBlk - 1) / kShBlk;
     key0 = prefix + (int)((long long)blocks * split / a.own_splits) * kShBlk;
     key_end = min(end, prefix + (int)((long long)blocks * (split + 1) / a.own_splits) * kShBlk);
     piece = a.max_pieces - a.own_splits + split;
   }
   auto token = [&](int r) {
-    return row_base >= 0 ? a.rows[row_base + r / g] : a.cu[seq] + r / g;
+    return row_base >= 0 ? a.rows[row_base + r / g] : tok0 + r / g;
   };
   for (int i = tid; i < kShRows * hd; i += kShThreads) {
     const int r = i / hd, d = i - r * hd;
@@ -200,13 +200,13 @@ using namespace cretif;
 
 extern "C" int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int ldo, const void* kc,
                                   const void* vc, long long n_blocks, const int* table,
-                                  int table_stride, int n_slots, const int* tok_pos, const int* cu,
+                                  int table_stride, int n_slots, const int* tok_pos,
                                   const int* seq_slot, const int* plan, int n_pre, int n_own,
-                                  int own_splits, int max_pieces, int n_rows, int B, int T, int nh,
+                                  int own_rows, int own_splits, int max_pieces, int n_rows, int T, int nh,
                                   int nkv, int hd, int bt, float scale, const float* sink,
                                   float* part_o, float* part_ml, unsigned int* fault, void* stream) {
   if (T <= 0) return kOk;
-  if (nh <= 0 || nkv <= 0 || nh % nkv || hd % 16 || hd < 16 || hd > 128 || bt != kShBlk || B <= 0 ||
+  if (nh <= 0 || nkv <= 0 || nh % nkv || hd % 16 || hd < 16 || hd > 128 || bt != kShBlk || own_rows <= 0 ||
       n_pre < 0 || n_own <= 0 || own_splits <= 0 || max_pieces < own_splits || n_rows < 0 ||
       nkv > 65535 || (long long)T * nh > (1LL << 30) || n_blocks <= 0 || !(scale > 0.f) ||
       (long long)n_pre + (long long)n_own * own_splits > 0x7fffffffLL)
@@ -217,14 +217,12 @@ extern "C" int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int
   SharedArgs a{};
   a.q = q; a.kc = kc; a.vc = vc; a.out = out; a.ldq = ldq; a.ldo = ldo; a.n_blocks = n_blocks;
   a.table = table; a.table_stride = table_stride; a.n_slots = n_slots;
-  a.tok_pos = tok_pos; a.cu = cu; a.seq_slot = seq_slot;
+  a.tok_pos = tok_pos; a.seq_slot = seq_slot;
   a.pre = reinterpret_cast<const SharedPrefixItem*>(plan);
   a.own = reinterpret_cast<const SharedOwnItem*>(plan + 8 * (size_t)n_pre);
-  a.rows = plan + 8 * (size_t)n_pre + 4 * (size_t)n_own;
+  a.rows = plan + 8 * ((size_t)n_pre + n_own);
   a.tok_pieces = a.rows + n_rows;
-  a.tok_seq = a.tok_pieces + T;
-  a.seq_prefix = a.tok_seq + T;
-  a.n_pre = n_pre; a.n_own = n_own; a.own_splits = own_splits; a.max_pieces = max_pieces; a.T = T;
+  a.n_pre = n_pre; a.n_own = n_own; a.own_rows = own_rows; a.own_splits = own_splits; a.max_pieces = max_pieces; a.T = T;
   a.nh = nh; a.nkv = nkv; a.hd = hd; a.scale_log2 = scale * 1.4426950408889634f; a.sink = sink;
   a.part_o = part_o; a.part_ml = reinterpret_cast<float2*>(part_ml); a.fault = fault;
   if (dt == kF32) return launch_shared_f32(a, (cudaStream_t)stream);

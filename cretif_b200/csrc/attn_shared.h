@@ -24,9 +24,11 @@ struct SharedPrefixItem {
   int piece;                               // the piece's index among the rows' pieces
   int pad;
 };
-// Some rows of one sequence over its own keys: row r is head kvh * g + r % g of token cu[seq] + r / g.
+// Some rows of one sequence over its own keys: row r is head kvh * g + r % g of token tok0 + r / g.
 struct SharedOwnItem {
-  int seq, row0, n_rows, pad;
+  int seq, tok0, row0, n_rows;
+  int prefix, pieces;                      // tokens shared, and pieces they are in
+  int pad[2];
 };
 
 // What every kernel of a call reads.
@@ -37,13 +39,13 @@ struct SharedArgs {
   long long n_blocks;
   const int* table;
   int table_stride, n_slots;
-  const int *tok_pos, *cu, *seq_slot;
-  // the plan: prefix items, own items, the rows of the groups, [T] prefix pieces and sequence of a
-  // token, [B] prefix of a sequence
+  const int *tok_pos, *seq_slot;
+  // the plan: prefix items, own items (of up to own_rows rows), the tokens of the groups, [T] prefix
+  // pieces of a token
   const SharedPrefixItem* pre;
   const SharedOwnItem* own;
-  const int *rows, *tok_pieces, *tok_seq, *seq_prefix;
-  int n_pre, n_own, own_splits, max_pieces, T;
+  const int *rows, *tok_pieces;
+  int n_pre, n_own, own_rows, own_splits, max_pieces, T;
   int nh, nkv, hd;
   float scale_log2;
   const float* sink;
@@ -52,9 +54,8 @@ struct SharedArgs {
   unsigned int* fault;
 };
 
-// The physical block at place `at` of a sequence's table; 0 and a fault bit where there is none.
-__device__ __forceinline__ int shared_block(const SharedArgs& a, int seq, int at) {
-  const int slot = a.seq_slot[seq];
+// The physical block at place `at` of a slot's table; 0 and a fault bit where there is none.
+__device__ __forceinline__ int shared_block_of(const SharedArgs& a, int slot, int at) {
   int blk = -1;
   if (slot >= 0 && slot < a.n_slots && at >= 0 && at < a.table_stride)
     blk = a.table[(size_t)slot * a.table_stride + at];
@@ -64,16 +65,16 @@ __device__ __forceinline__ int shared_block(const SharedArgs& a, int seq, int at
   }
   return blk;
 }
+__device__ __forceinline__ int shared_block(const SharedArgs& a, int seq, int at) {
+  return shared_block_of(a, a.seq_slot[seq], at);
+}
 
-// A sequence's own keys: first block, and one past the last position that a row at `last` sees.  A
-// position inside the prefix is a caller's mistake: the fault bit is set and there are none.
-__device__ __forceinline__ int shared_own_end(const SharedArgs& a, int seq, int last) {
-  const int prefix = a.seq_prefix[seq];
-  if (last < prefix) {
-    atomicOr(a.fault, (unsigned)kFaultBlockTable);
-    return prefix;
-  }
-  return last + 1;
+// One past the last own key that a row at position `last` sees.  A position inside the prefix is a
+// caller's mistake: the fault bit is set and there are none.
+__device__ __forceinline__ int shared_own_end(const SharedArgs& a, int prefix, int last) {
+  if (last >= prefix && last < 0x7fffff00) return last + 1;
+  atomicOr(a.fault, (unsigned)kFaultBlockTable);
+  return prefix;
 }
 
 }  // namespace cretif

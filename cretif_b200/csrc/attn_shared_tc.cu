@@ -194,36 +194,39 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp == 4) {
-    int mine = 0;
+    // Block ids come 32 at a time, a lane each, and a window ahead of their use: read one by one they
+    // cost two dependent loads a step (64 answers at 8,000: WINDOW_BEFORE us with, WINDOW_AFTER without).
+    auto window = [&](int w) { return 32 * w + lane < n ? shared_block(a, it.seq, it.blk0 + 32 * w + lane) : 0; };
+    int here = window(0), next = window(1), s = 0;        // windows of V's block, and the one behind it
     for (int p = 0; p <= n; ++p) {
-      // block ids of the range, 32 at a time: pair p needs block p (V is one pair behind its K)
-      // and the ones around it
-      const int s = p % L.pairs;
+      const int jv = p - 1, jk = p + 1;                   // pair 0: K_0 and K_1; pair p: V_{p-1}, K_{p+1}
+      if (jv > 0 && (jv & 31) == 0) {
+        here = next;
+        next = window((jv >> 5) + 1);
+      }
+      const int from = (jk >> 5) > ((jv > 0 ? jv : 0) >> 5) ? next : here;
+      const int blk_k = __shfl_sync(0xffffffffu, from, jk & 31);
+      const int blk_first = __shfl_sync(0xffffffffu, here, p == 0 ? 0 : jv & 31);
       bool go = true;
       if (lane == 0 && p >= L.pairs) {
-        // pair q has been read when commit q + 1 arrives; the one 8 commits later cannot arrive
-        // before pair q + L.pairs is loaded, which is this thread's next step
+        // pair p - L.pairs has been read when commit p - L.pairs + 1 arrives (the one 8 commits later
+        // cannot arrive before this pair is loaded)
         const int c = p - L.pairs + 1;
         go = tc::mbar_wait(&done[c % kSpDone], (uint32_t)((c / kSpDone) & 1), abort);
       }
-      go = __shfl_sync(0xffffffffu, go, 0);
-      if (!go) break;
-      if (lane < 2) {                                     // lane 0: the pair's first tile, 1: its second
-        const bool is_k = p == 0 || lane == 1;
-        const int j = p == 0 ? lane : lane == 0 ? p - 1 : p + 1;
-        const bool there = j < n;
-        mine = there ? shared_block(a, it.seq, it.blk0 + j) : 0;
-        const unsigned both = __ballot_sync(0x3u, there);
-        if (lane == 0) tc::mbar_expect_tx(&full[s], (uint32_t)(__popc(both) * n_sub * kSpTile));
-        __syncwarp(0x3u);
-        if (there) {
-          const int row = (mine * a.nkv + kvh) * kShBlk;
-          for (int sub = 0; sub < n_sub; ++sub)
-            tc::tma_load_2d(smem + L.ring + ((s * 2 + lane) * n_sub + sub) * kSpTile, is_k ? &map_k : &map_v,
-                            64 * sub, row, &full[s]);
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      if (lane == 0) {
+        const bool second = jk < n;
+        tc::mbar_expect_tx(&full[s], (uint32_t)((second ? 2 : 1) * n_sub * kSpTile));
+        unsigned char* slot = smem + L.ring + s * 2 * n_sub * kSpTile;
+        for (int sub = 0; sub < n_sub; ++sub) {
+          tc::tma_load_2d(slot + sub * kSpTile, p == 0 ? &map_k : &map_v, 64 * sub,
+                          (blk_first * a.nkv + kvh) * kShBlk, &full[s]);
+          if (second)
+            tc::tma_load_2d(slot + (n_sub + sub) * kSpTile, &map_k, 64 * sub, (blk_k * a.nkv + kvh) * kShBlk, &full[s]);
         }
       }
-      __syncwarp();
+      if (++s == L.pairs) s = 0;
     }
   } else if (warp == 5) {
     if (lane == 0) {
@@ -231,10 +234,10 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       const uint32_t idesc_pv = tc::instr_desc_bf16(kSpRows, hd) | (1u << 16);   // B is MN-major
       const int k_steps = hd >> 4;
       const uint64_t qd = tc::smem_desc_k_sw128(smem + L.q);
-      auto scores = [&](int j) {
-        const int p = j < 2 ? 0 : j - 1;
-        const uint64_t kd =
-            tc::smem_desc_k_sw128(smem + L.ring + ((p % L.pairs) * 2 + (j == 0 ? 0 : 1)) * n_sub * kSpTile);
+      const uint64_t kd0 = tc::smem_desc_k_sw128(smem + L.ring), vd0 = sp_desc_v(smem + L.ring);
+      const uint64_t tile = (uint64_t)((n_sub * kSpTile) >> 4);   // a tile, in descriptor units
+      auto scores = [&](int j, int slot) {                // K_j is tile `slot` of the ring
+        const uint64_t kd = kd0 + slot * tile;
         for (int kk = 0; kk < k_steps; ++kk)
           tc::umma_bf16(tmem + (uint32_t)(j & 1) * 64, qd + (uint64_t)((kk >> 2) * ((kSpRows * 128) >> 4) + 2 * (kk & 3)),
                         kd + (uint64_t)((kk >> 2) * (kSpTile >> 4) + 2 * (kk & 3)), idesc_qk, kk != 0);
@@ -242,24 +245,24 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       bool ok = tc::mbar_wait(q_full, 0u, abort) && tc::mbar_wait(&full[0], 0u, abort);
       if (ok) {
         tc::tc_fence_after();
-        scores(0);
+        scores(0, 0);
         tc::umma_commit(&done[0]);
-        if (n > 1) scores(1);
+        if (n > 1) scores(1, 1);
         tc::umma_commit(&done[1]);
       }
-      for (int j = 0; j < n && ok; ++j) {
-        const int p = j + 1;
-        ok = tc::mbar_wait(&full[p % L.pairs], (uint32_t)((p / L.pairs) & 1), abort) &&
+      for (int j = 0, s = 1, turn = 0; j < n && ok; ++j) {   // pair j + 1 in slot s
+        ok = tc::mbar_wait(&full[s], (uint32_t)(turn & 1), abort) &&
              tc::mbar_wait(&p_full[j & 1], (uint32_t)((j >> 1) & 1), abort);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint64_t vd = sp_desc_v(smem + L.ring + (p % L.pairs) * 2 * n_sub * kSpTile);
+        const uint64_t vd = vd0 + 2 * s * tile;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)                    // 16 keys: two 1,024-byte atoms of V
           tc::umma_bf16_a_tmem(tmem + kColO, tmem + (uint32_t)((j & 1) * 64 + kk * 8), vd + (uint64_t)(kk * 128),
                                idesc_pv, (j | kk) != 0);
-        if (j + 2 < n) scores(j + 2);
+        if (j + 2 < n) scores(j + 2, 2 * s + 1);
         tc::umma_commit(&done[(j + 2) % kSpDone]);
+        if (++s == L.pairs) { s = 0; ++turn; }
       }
     }
   } else {
@@ -362,18 +365,21 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 }
 
 // ---------------------------------------------------------------------------------------
-// Own keys: a CTA takes up to 16 rows of one sequence and key/value head; its warps take 16 keys of
-// every block (or of two blocks) each, straight from the cache into the operands' registers.
+// Own keys: a CTA takes up to 16 rows of one sequence and key/value head; its four warps take 16 keys
+// of every block each, straight from the cache into the operands' registers.
 //   S = Q K^T (m16n8k16): the channels of 32 are taken in an order in which a lane's 16 bytes of a
 //   key are its part of two products (channels 8c .. 8c + 7 of lane c: pairs 0 and 1 in the first,
 //   2 and 3 in the second), the same for the queries.
 //   O += P V: column n of product t is channel 8 n + t, so a lane's 16 bytes of a key are its part
 //   of eight products; two keys' values are brought together by byte permutes.
-// No shared memory and no barrier inside the loop; the next 16 keys are on their way meanwhile.
+// No shared memory and no barrier inside the loop; a step's keys are asked for when the step before
+// has taken its own, its values likewise.  NR = 1: up to 8 rows, and the products' other 8 are empty.
 // With JOIN the CTA holds all of the rows' own keys and joins the rows' prefix pieces itself (it is
 // launched while the prefix kernel runs and waits for it only then); else it leaves pieces.
-template <int HDG, int WARPS, bool JOIN>
-__global__ void __launch_bounds__(WARPS * 32)
+constexpr int kSoWarps = 4, kSoThreads = kSoWarps * 32;
+
+template <int HDG, int NR, bool JOIN>
+__global__ void __launch_bounds__(kSoThreads)
 shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
   extern __shared__ __align__(16) float so_smem[];
   const int hd = a.hd, g = a.nh / a.nkv, kvh = blockIdx.y;
@@ -383,17 +389,17 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
   const SharedOwnItem it = a.own[JOIN ? blockIdx.x : blockIdx.x / a.own_splits];
   if (!after_prefix) dependent_wait();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int seq = it.seq, cu0 = a.cu[seq];
-  const int prefix = a.seq_prefix[seq];
-  const int end = shared_own_end(a, seq, a.tok_pos[cu0 + (it.row0 + it.n_rows - 1) / g]);
-  // ---- queries: rows r and r + 8
-  uint32_t qa[HDG * 2][2][4];                             // [32 channels][row][pair]
-  int pos[2];
+  const int prefix = it.prefix, blk0 = prefix / kShBlk, key_in = warp * 16;
+  const int slot = a.seq_slot[it.seq];
+  int pos[NR];
+  const int last = a.tok_pos[it.tok0 + (it.row0 + it.n_rows - 1) / g];
+  // ---- queries: row r (and r + 8)
+  uint32_t qa[HDG * 2][NR][4];                            // [32 channels][row][pair]
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < NR; ++i) {
     const int row = r + 8 * i, rr = it.row0 + row;
     const bool there = row < it.n_rows;
-    const int t = cu0 + (there ? rr / g : 0);
+    const int t = it.tok0 + (there ? rr / g : 0);
     pos[i] = there ? a.tok_pos[t] : -1;
     const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.ldq +
                                (size_t)(kvh * g + (there ? rr % g : 0)) * hd;
@@ -404,52 +410,55 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
       qa[d][i][0] = v.x; qa[d][i][1] = v.y; qa[d][i][2] = v.z; qa[d][i][3] = v.w;
     }
   }
-  float o[HDG][8][4];
+  const int end = shared_own_end(a, prefix, last);
+  float o[HDG][8][2 * NR];
 #pragma unroll
   for (int v = 0; v < HDG; ++v)
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[v][t][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  // 16 keys a warp and step: 64 / 16 warps share a block, WARPS / 4 blocks a step
-  const int blocks = (end - prefix + kShBlk - 1) / kShBlk, blk0 = prefix / kShBlk;
-  constexpr int kStep = WARPS / 4;
-  const int first = split * kStep + (warp >> 2), stride = splits * kStep, key_in = (warp & 3) * 16;
+      for (int e = 0; e < 2 * NR; ++e) o[v][t][e] = 0.f;
+  float m[NR], l[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
+  const int blocks = (end - prefix + kShBlk - 1) / kShBlk;
+  auto has = [&](int i) { return i < blocks && prefix + i * kShBlk + key_in < end; };
+  auto block = [&](int i) { return has(i) ? shared_block_of(a, slot, blk0 + i) : 0; };
   uint4 kr[HDG * 2][2], vr[HDG][4];
-  auto load = [&](int i) {                                // keys key_in .. + 15 of own block i
-    const int key0 = prefix + i * kShBlk + key_in;
-    const size_t at = ((size_t)shared_block(a, seq, blk0 + i) * a.nkv + kvh) * kShBlk * hd;
-    const __nv_bfloat16* kp = static_cast<const __nv_bfloat16*>(a.kc) + at + (size_t)key_in * hd;
-    const __nv_bfloat16* vp = static_cast<const __nv_bfloat16*>(a.vc) + at + (size_t)key_in * hd;
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  // keys key_in .. + 15 of own block i, which is physical block blk
+  auto tile = [&](const void* cache, int blk) {
+    return static_cast<const __nv_bfloat16*>(cache) + (((size_t)blk * a.nkv + kvh) * kShBlk + key_in) * hd;
+  };
+  auto load_k = [&](int i, int blk) {
+    const int n = end - (prefix + i * kShBlk + key_in);   // (nothing past the last key is looked at)
+    const __nv_bfloat16* p = tile(a.kc, blk);
 #pragma unroll
     for (int d = 0; d < HDG * 2; ++d)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        kr[d][x] = key0 + 8 * x + r < end && 32 * d + 8 * c < hd
-            ? __ldg(reinterpret_cast<const uint4*>(kp + (size_t)(8 * x + r) * hd + 32 * d + 8 * c)) : zero;
+        kr[d][x] = 8 * x + r < n && 32 * d + 8 * c < hd
+            ? __ldg(reinterpret_cast<const uint4*>(p + (8 * x + r) * hd + 32 * d + 8 * c)) : zero;
+  };
+  auto load_v = [&](int i, int blk) {
+    const int n = end - (prefix + i * kShBlk + key_in);
+    const __nv_bfloat16* p = tile(a.vc, blk);
 #pragma unroll
     for (int v = 0; v < HDG; ++v)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int key = 2 * c + (x & 1) + 8 * (x >> 1);
-        vr[v][x] = key0 + key < end && 64 * v + 8 * r < hd
-            ? __ldg(reinterpret_cast<const uint4*>(vp + (size_t)key * hd + 64 * v + 8 * r)) : zero;
+        vr[v][x] = key < n && 64 * v + 8 * r < hd
+            ? __ldg(reinterpret_cast<const uint4*>(p + key * hd + 64 * v + 8 * r)) : zero;
       }
   };
-  auto has = [&](int i) { return i < blocks && prefix + i * kShBlk + key_in < end; };
-  if (has(first)) load(first);
-  for (int i = first; has(i); i += stride) {
+  int blk = block(split), ahead = block(split + splits);
+  if (has(split)) { load_k(split, blk); load_v(split, blk); }
+  for (int i = split; has(i); i += splits) {
     const int key0 = prefix + i * kShBlk + key_in;
-    uint4 kn[HDG * 2][2], vn[HDG][4];
-#pragma unroll
-    for (int d = 0; d < HDG * 2; ++d) { kn[d][0] = kr[d][0]; kn[d][1] = kr[d][1]; }
-#pragma unroll
-    for (int v = 0; v < HDG; ++v)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) vn[v][x] = vr[v][x];
-    if (has(i + stride)) load(i + stride);
+    const bool more = has(i + splits);
+    blk = ahead;
+    ahead = block(i + 2 * splits);
     float s[2][4];
 #pragma unroll
     for (int x = 0; x < 2; ++x)
@@ -459,12 +468,15 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
     for (int d = 0; d < HDG * 2; ++d)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        mma_16816_f32(s[x], qa[d][0][0], qa[d][1][0], qa[d][0][1], qa[d][1][1], kn[d][x].x, kn[d][x].y);
-        mma_16816_f32(s[x], qa[d][0][2], qa[d][1][2], qa[d][0][3], qa[d][1][3], kn[d][x].z, kn[d][x].w);
+        mma_16816_f32(s[x], qa[d][0][0], NR == 2 ? qa[d][NR - 1][0] : 0u, qa[d][0][1], NR == 2 ? qa[d][NR - 1][1] : 0u,
+                      kr[d][x].x, kr[d][x].y);
+        mma_16816_f32(s[x], qa[d][0][2], NR == 2 ? qa[d][NR - 1][2] : 0u, qa[d][0][3], NR == 2 ? qa[d][NR - 1][3] : 0u,
+                      kr[d][x].z, kr[d][x].w);
       }
-    uint32_t pa[4];
+    if (more) load_k(i + splits, blk);
+    uint32_t pa[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {                         // rows r, r + 8
+    for (int w = 0; w < NR; ++w) {                        // rows r, r + 8
       float t4[4], mx = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -493,31 +505,35 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
     }
 #pragma unroll
     for (int v = 0; v < HDG; ++v) {
-      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vn[v][0]);
-      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vn[v][1]);
-      const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vn[v][2]);
-      const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vn[v][3]);
+      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[v][0]);
+      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[v][1]);
+      const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[v][2]);
+      const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vr[v][3]);
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
         const unsigned sel = t & 1 ? 0x7632u : 0x5410u;
-        mma_16816_f32(o[v][t], pa[0], pa[1], pa[2], pa[3], __byte_perm(w0[t >> 1], w1[t >> 1], sel),
+        float acc[4] = {o[v][t][0], o[v][t][1], NR == 2 ? o[v][t][2 * NR - 2] : 0.f, NR == 2 ? o[v][t][2 * NR - 1] : 0.f};
+        mma_16816_f32(acc, pa[0], pa[1], pa[2], pa[3], __byte_perm(w0[t >> 1], w1[t >> 1], sel),
                       __byte_perm(w2[t >> 1], w3[t >> 1], sel));
+#pragma unroll
+        for (int e = 0; e < 2 * NR; ++e) o[v][t][e] = acc[e];
       }
     }
+    if (more) load_v(i + splits, blk);
   }
-  // ---- the warps' parts meet in shared memory: a lane has channels 16c .. 16c + 15 of two rows
+  // ---- the warps' parts meet in shared memory: a lane has channels 16c .. 16c + 15 of its rows
   const int ld = hd + 4;
-  float* so = so_smem;                                    // [WARPS][16][hd + 4]
-  float2* sml = reinterpret_cast<float2*>(so + WARPS * 16 * ld);    // [WARPS][16]
+  float* so = so_smem;                                    // [warp][8 NR][hd + 4]
+  float2* sml = reinterpret_cast<float2*>(so + kSoWarps * 8 * NR * ld);    // [warp][8 NR]
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
+  for (int w = 0; w < NR; ++w) {
     l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
     l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
-    if (c == 0) sml[warp * 16 + r + 8 * w] = make_float2(m[w], l[w]);
+    if (c == 0) sml[warp * 8 * NR + r + 8 * w] = make_float2(m[w], l[w]);
     if (r + 8 * w < it.n_rows) {
 #pragma unroll
       for (int v = 0; v < HDG; ++v) {
-        float* dst = so + (warp * 16 + r + 8 * w) * ld + 64 * v + 16 * c;
+        float* dst = so + (warp * 8 * NR + r + 8 * w) * ld + 64 * v + 16 * c;
         if (64 * v + 16 * c < hd) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -533,43 +549,68 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
   // for this one need not wait for that one.
   if (after_prefix) dependent_wait();
   __syncthreads();
-  const int quads = hd >> 2;
+  const int quads = hd >> 2, n_pieces = JOIN ? it.pieces : 0;
   const size_t rows_all = (size_t)a.T * a.nh;
-  for (int i = threadIdx.x; i < it.n_rows * quads; i += WARPS * 32) {
+  for (int i = threadIdx.x; i < it.n_rows * quads; i += kSoThreads) {
     const int row = i / quads, ch = (i - row * quads) * 4, rr = it.row0 + row;
-    const int t = cu0 + rr / g, h = kvh * g + rr % g;
+    const int t = it.tok0 + rr / g, h = kvh * g + rr % g;
     const size_t at = (size_t)t * a.nh + h;
-    const int n = JOIN ? a.tok_pieces[t] : 0;
-    float mm = -INFINITY;
-    const float sink = JOIN && a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
-    mm = fmaxf(mm, sink);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, sml[w * 16 + row].x);
-    for (int p = 0; p < n; ++p) mm = fmaxf(mm, __ldcg(&a.part_ml[p * rows_all + at]).x);
-    const float ref = mm == -INFINITY ? 0.f : mm;
-    float den = 0.f;
+    float ref = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float2 ml, const float4& x) {
-      const float w = ml.x == -INFINITY ? 0.f : sp_exp2(ml.x - ref);
-      den = fmaf(w, ml.y, den);
-      acc.x = fmaf(w, x.x, acc.x); acc.y = fmaf(w, x.y, acc.y);
-      acc.z = fmaf(w, x.z, acc.z); acc.w = fmaf(w, x.w, acc.w);
-    };
-#pragma unroll 4
-    for (int p = 0; p < n; ++p)
-      add(__ldcg(&a.part_ml[p * rows_all + at]),
-          __ldcg(reinterpret_cast<const float4*>(a.part_o + (p * rows_all + at) * hd + ch)));
+    // N parts at a time: one wait for their loads, one move of the reference
+    auto add = [&](auto& ml, auto& x) {
+      constexpr int N = sizeof(ml) / sizeof(ml[0]);
+      float top = ref;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w)
-      add(sml[w * 16 + row], *reinterpret_cast<const float4*>(so + (w * 16 + row) * ld + ch));
+      for (int e = 0; e < N; ++e) top = fmaxf(top, ml[e].x);
+      if (top == -INFINITY) return;
+      const float keep = ref == -INFINITY ? 0.f : sp_exp2(ref - top);
+      den *= keep;
+      acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float w = ml[e].x == -INFINITY ? 0.f : sp_exp2(ml[e].x - top);
+        den = fmaf(w, ml[e].y, den);
+        acc.x = fmaf(w, x[e].x, acc.x); acc.y = fmaf(w, x[e].y, acc.y);
+        acc.z = fmaf(w, x[e].z, acc.z); acc.w = fmaf(w, x[e].w, acc.w);
+      }
+      ref = top;
+    };
+    constexpr int kAtOnce = 8;
+    for (int p0 = 0; p0 < n_pieces; p0 += kAtOnce) {
+      float2 ml[kAtOnce];
+      float4 x[kAtOnce];
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) {
+        const bool in = p0 + e < n_pieces;
+        const size_t from = (size_t)(in ? p0 + e : p0) * rows_all + at;
+        ml[e] = __ldcg(&a.part_ml[from]);
+        x[e] = __ldcg(reinterpret_cast<const float4*>(a.part_o + from * hd + ch));
+        if (!in) ml[e] = make_float2(-INFINITY, 0.f);
+      }
+      add(ml, x);
+    }
+    float2 ml[kSoWarps];
+    float4 x[kSoWarps];
+#pragma unroll
+    for (int w = 0; w < kSoWarps; ++w) {
+      ml[w] = sml[w * 8 * NR + row];
+      x[w] = *reinterpret_cast<const float4*>(so + (w * 8 * NR + row) * ld + ch);
+    }
+    add(ml, x);
     if (JOIN) {
-      if (a.sink) den += sink == ref ? 1.0f : exp2f(sink - ref);
+      if (a.sink) {
+        const float sink = a.sink[h] * 1.4426950408889634f, top = fmaxf(ref, sink);
+        const float keep = ref == -INFINITY ? 0.f : sp_exp2(ref - top);
+        den = den * keep + (sink == top ? 1.0f : exp2f(sink - top));
+        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+      }
       const float inv = den > 0.f ? 1.0f / den : 0.f;
-      uint2 packed = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+      const uint2 packed = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
       *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)t * a.ldo + (size_t)h * hd + ch) = packed;
     } else {
       const size_t to = (size_t)(a.max_pieces - a.own_splits + split) * rows_all + at;
-      if (ch == 0) a.part_ml[to] = make_float2(mm, den);
+      if (ch == 0) a.part_ml[to] = make_float2(ref, den);
       *reinterpret_cast<float4*>(a.part_o + to * hd + ch) = acc;
     }
   }
@@ -593,14 +634,13 @@ static int sp_launch(void (*kernel)(Params...), dim3 grid, int threads, size_t s
   return e == cudaSuccess ? launch_status() : (int)e;
 }
 
-template <int HDG, int WARPS>
+template <int HDG, int NR>
 static int launch_own(const SharedArgs& a, cudaStream_t st) {
-  const size_t smem = (size_t)(WARPS * 16 * (a.hd + 4) + WARPS * 32) * 4;
+  const size_t smem = (size_t)(kSoWarps * 8 * NR * (a.hd + 4) + kSoWarps * 8 * NR * 2) * 4;
   const int after = a.n_pre > 0;
-  return a.own_splits == 1
-      ? sp_launch(shared_own_mma_kernel<HDG, WARPS, true>, dim3(a.n_own, a.nkv), WARPS * 32, smem, st, a, after)
-      : sp_launch(shared_own_mma_kernel<HDG, WARPS, false>, dim3(a.n_own * a.own_splits, a.nkv), WARPS * 32, smem, st, a,
-                  after);
+  const dim3 grid(a.n_own * a.own_splits, a.nkv);
+  return a.own_splits == 1 ? sp_launch(shared_own_mma_kernel<HDG, NR, true>, grid, kSoThreads, smem, st, a, after)
+                           : sp_launch(shared_own_mma_kernel<HDG, NR, false>, grid, kSoThreads, smem, st, a, after);
 }
 
 // The prefix pieces and the own keys; joins the rows where the own keys are in one piece.
@@ -617,7 +657,8 @@ int launch_shared_bf16(const SharedArgs& a, cudaStream_t st) {
     const int e = sp_launch(shared_prefix_tc_kernel, dim3(a.n_pre, a.nkv), kSpThreads, L.total, st, mk, mv, a);
     if (e) return e;
   }
-  return a.hd <= 64 ? launch_own<1, 4>(a, st) : launch_own<2, 4>(a, st);
+  if (a.own_rows <= 8) return a.hd <= 64 ? launch_own<1, 1>(a, st) : launch_own<2, 1>(a, st);
+  return a.hd <= 64 ? launch_own<1, 2>(a, st) : launch_own<2, 2>(a, st);
 }
 
 }  // namespace cretif

@@ -1822,7 +1822,7 @@ class SharedPrefixPlan:
     share, not on slots, positions or values.  One plan serves every layer, and every later step of
     the same make-up."""
 
-    __slots__ = ("data", "n_pre", "n_own", "own_splits", "max_pieces", "n_rows", "B", "T", "nh", "nkv",
+    __slots__ = ("data", "n_pre", "n_own", "own_rows", "own_splits", "max_pieces", "n_rows", "B", "T", "nh", "nkv",
                  "hd", "dtype", "prefix_blocks", "device")
 
 
@@ -1842,8 +1842,8 @@ def _blocks_an_item(tiles, ctas: int, begin: int = 4) -> int:
 
 
 def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_rows: int, ctas: int):
-    """The host side of a plan: (prefix items, own items, splits of the own keys, most pieces, rows,
-    pieces of a token, sequence of a token, prefix of a sequence), lists of integers."""
+    """The host side of a plan: (prefix items, own items, splits of the own keys, most pieces, tokens
+    of the groups, pieces of a token, prefix of a sequence), lists of integers."""
     if nh <= 0 or nkv <= 0 or nh % nkv:
         raise KernelError(f"shared prefix: {nh} heads cannot share {nkv} key/value heads")
     news, starts = [int(n) for n in news], [int(n) for n in starts]
@@ -1889,11 +1889,10 @@ def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_r
     own = []
     for b in range(B):
         for row0 in range(0, news[b] * g, own_rows):
-            own += [b, row0, min(own_rows, news[b] * g - row0), 0]
+            own += [b, cu[b], row0, min(own_rows, news[b] * g - row0), prefix_of[b], tok_pieces[cu[b]], 0, 0]
     own_blocks = max(-(-(starts[b] + news[b] - prefix_of[b]) // 64) for b in range(B))
-    splits = max(1, min(own_blocks // 8, ctas // max(1, len(own) // 4 * nkv), 8))
-    tok_seq = [b for b in range(B) for _ in range(news[b])]
-    return pre, own, splits, max(tok_pieces) + splits, rows, tok_pieces, tok_seq, prefix_of
+    splits = max(1, min(own_blocks // 8, ctas // max(1, len(own) // 8 * nkv), 8))
+    return pre, own, splits, max(tok_pieces) + splits, rows, tok_pieces, prefix_of
 
 
 def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, device) -> SharedPrefixPlan:
@@ -1908,13 +1907,17 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
         raise KernelError(f"shared prefix: head_dim {hd} is not a multiple of 16 up to 128")
     dev = torch.device(device)
     ctas = 2 * (sm_count(dev) if dev.type == "cuda" else 148)
-    pre, own, splits, pieces, rows, tok_pieces, tok_seq, prefix_of = _shared_items(
-        groups, news, starts, nh, nkv, *((128, 16) if dtype == torch.bfloat16 else (32, 32)), ctas)
+    tile_rows, own_rows = (128, 16) if dtype == torch.bfloat16 else (32, 32)
+    if dtype == torch.bfloat16 and nkv > 0 and max(news, default=1) * nh // nkv <= 8:
+        own_rows = 8
+    pre, own, splits, pieces, rows, tok_pieces, prefix_of = _shared_items(groups, news, starts, nh, nkv, tile_rows,
+                                                                          own_rows, ctas)
     plan = SharedPrefixPlan()
-    packed = torch.tensor(pre + own + rows + tok_pieces + tok_seq + prefix_of, dtype=torch.int32)
+    packed = torch.tensor(pre + own + rows + tok_pieces, dtype=torch.int32)
     plan.data = packed.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else packed
-    plan.n_pre, plan.n_own, plan.own_splits, plan.max_pieces = len(pre) // 8, len(own) // 4, splits, pieces
-    plan.n_rows, plan.B, plan.T = len(rows), len(prefix_of), len(tok_seq)
+    plan.n_pre, plan.n_own, plan.own_rows = len(pre) // 8, len(own) // 8, own_rows
+    plan.own_splits, plan.max_pieces = splits, pieces
+    plan.n_rows, plan.B, plan.T = len(rows), len(prefix_of), len(tok_pieces)
     plan.nh, plan.nkv, plan.hd, plan.dtype, plan.device = nh, nkv, hd, dtype, plan.data.device
     plan.prefix_blocks = max(prefix_of) // 64
     return plan
@@ -1924,8 +1927,9 @@ def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: Shar
                 scale: float, block_tokens: int, fault, sink=None) -> None:
     """Causal attention of a step whose sequences bring a few tokens each, with the keys of the
     prefixes that they share read once a group (``plan``, from :func:`shared_prefix_plan`).  ``q``
-    rows start with the query heads; ``out`` [T, heads · head_dim], row t for token t.  The step's own
-    keys and values are in the cache already.  ``sink`` (float32 [heads], optional): exp(sink_h)
+    rows start with the query heads; ``out`` [T, heads · head_dim], row t for token t.  ``tok_pos`` ascends
+    within a sequence; ``cu_seqlens`` are the sums of the plan's ``news``.  The step's own keys and values
+    are in the cache already.  ``sink`` (float32 [heads], optional): exp(sink_h)
     joins head h's softmax denominator.  bfloat16 or float32, head sizes in multiples of 16 up to 128,
     any number of query heads on a key/value head.  A table entry that names no block, or a position
     inside the shared tokens, sets the block-table bit of ``fault``."""
@@ -1961,8 +1965,8 @@ def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: Shar
     _check(lib().cretif_attn_shared(
         _p(q), _rows(q, "q"), _DT[plan.dtype], _p(out), _rows(out, "out"), _p(kc), _p(vc),
         ctypes.c_longlong(kc.shape[0]), _p(table), _rows(table, "table"), table.shape[0], _p(tok_pos),
-        _p(cu_seqlens), _p(seq_slot), _p(plan.data), plan.n_pre, plan.n_own, plan.own_splits,
-        plan.max_pieces, plan.n_rows, B, T, nh, nkv, hd, block_tokens, ctypes.c_float(scale), _p(sink),
+        _p(seq_slot), _p(plan.data), plan.n_pre, plan.n_own, plan.own_rows, plan.own_splits,
+        plan.max_pieces, plan.n_rows, T, nh, nkv, hd, block_tokens, ctypes.c_float(scale), _p(sink),
         ctypes.c_void_p(part_o), ctypes.c_void_p(part_o + 4 * plan.max_pieces * T * nh * hd), _p(fault),
         _stream()), "attn_shared", 2)
 

@@ -253,41 +253,40 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const __grid_constan
 // ---- second launch, whole vocabulary: a cluster a sequence, its CTAs share the vocabulary
 constexpr int kVdThreads = 512, kVdSeg = 128;             // entries a warp takes at once
 
-// 2^t, t <= 0, in 64 bits: t = n / 32 + f, 2^(n / 32) from a table of 32 and a power of two, 2^f by
-// its series to the fifth power (|f| <= 1/64: the sixth term is below 2.3e-15) (table-driven
-// exponential, P. T. P. Tang, 1989).  Nine 64-bit operations; the library's has about twice as many.
-__device__ __forceinline__ double vf_exp2(double t, const double* table) {
-  t = fmax(t, -1100.0);
-  const double magic = 6755399441055744.0;                // 1.5 * 2^52: rounds to an integer
-  const double big = fma(t, 32.0, magic);
-  const int n = __double2loint(big);
-  const double f = fma(big - magic, -1.0 / 32.0, t);
-  // ln2^k / k!
-  double p = fma(f, 0.0013333558146428441, 0.0096181291076284772);
-  p = fma(f, p, 0.055504108664821580);
-  p = fma(f, p, 0.24022650695910072);
-  p = fma(f, p, 0.69314718055994531);
-  p = fma(f, p, 1.0);
-  p *= table[n & 31];
-  const int e = n >> 5;
-  if (e < -1020) return 0.0;
-  return __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p));
-}
-
-struct VfTerm {                 // a row's terms in 64 bits
-  double c;                     // log2 e / T
-  float top;                    // the row's maximum
-  bool infinite;
-  __device__ __forceinline__ void set(float top_, double c_) {
-    top = top_;
-    c = c_;
+// A row's terms 2^((v - top) c) in 64 bits.  32 (v - top) c = n + f with |f| <= 1/2; 2^(n / 32) from a
+// table of 32 and a power of two, 2^(f / 32) by its series to the fifth power (the sixth term is below
+// 2.3e-15) (table-driven exponential, P. T. P. Tang, 1989).  Some 20 instructions, ten of them 64-bit.
+struct VfTerm {
+  double c32, top;              // 32 log2 e / T, the row's maximum
+  float lo;                     // entries below it (2^-1000 of the largest) and NaN count 0
+  bool infinite;                // the maximum is: entries equal to it count 1, all others 0
+  __device__ __forceinline__ void set(float top_, double c) {
     infinite = fabsf(top_) == INFINITY;
+    top = top_;
+    c32 = 32.0 * c;
+    lo = top_;
+    if (!infinite) {
+      lo = (float)((double)top_ - 1000.0 / c);
+      // (rounded down too far, an entry's n would not fit an exponent)
+      while (lo < top_ && ((double)lo - (double)top_) * c < -1020.0) lo = nextafterf(lo, INFINITY);
+    }
   }
   __device__ __forceinline__ double operator()(float v, const double* table) const {
-    v = fmaxf(v, -INFINITY);                              // (NaN)
-    if (v == top) return 1.0;
-    if (infinite) return 0.0;
-    return vf_exp2(((double)v - (double)top) * c, table);
+    if (infinite) return fmaxf(v, -INFINITY) == (float)top ? 1.0 : 0.0;
+    const double magic = 6755399441055744.0;              // 1.5 * 2^52: rounds to an integer
+    const double d = (double)fmaxf(v, lo) - top;
+    const double big = fma(d, c32, magic);
+    const int n = __double2loint(big);
+    const double f = fma(d, c32, magic - big);
+    // (ln2 / 32)^k / k!
+    double p = fma(f, 3.9737099845494154e-11, 9.172562701824643e-09);
+    p = fma(f, p, 1.6938509724371819e-06);
+    p = fma(f, p, 0.00023459619820224677);
+    p = fma(f, p, 0.02166084939249829);
+    p = fma(f, p, 1.0);
+    p *= table[n & 31];
+    const bool any = v >= lo;
+    return __hiloint2double(any ? __double2hiint(p) + ((n >> 5) << 20) : 0, any ? __double2loint(p) : 0);
   }
 };
 
@@ -309,8 +308,9 @@ __device__ __forceinline__ void vf_four(const float* x, int V, int i, bool align
 }
 
 __global__ void __launch_bounds__(kVdThreads)
-verify_draw_kernel(const __grid_constant__ VfArgs a) {
-  extern __shared__ double vd_smem[];                     // sums of the CTA's segments
+verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
+  // sums of the CTA's segments; where they fit (cached) the terms of its share of both rows
+  extern __shared__ __align__(16) double vd_smem[];
   __shared__ double table[32];
   __shared__ double sums[kVdThreads / 32];
   __shared__ double shared_tot[3];                        // this CTA's: p, q, what is drawn from
@@ -393,18 +393,35 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
     }
     __syncthreads();
   };
+  double2* keep = reinterpret_cast<double2*>(vd_smem + seg_room);   // [segment][row][lane][2]
+  // the four terms of a lane in a segment of a row (0 behind the vocabulary)
+  auto look = [&](const VfTerm& row, const float* x, bool aligned, int s, double (&v)[4]) {
+    float f[4];
+    vf_four(x, a.V, s * 32 + lane, aligned, f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = row(f[e], table);
+    if ((s + 1) * kVdSeg > a.V) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (s * kVdSeg + 4 * lane + e >= a.V) v[e] = 0.0;
+    }
+  };
   double weight = 0.0;                                    // of q's terms beside p's
   if (minus_q) {
     double zp = 0.0, zq = 0.0;
+#pragma unroll 2
     for (int s = s0 + warp; s < s1; s += kWarps) {
-      float vp[4], vq[4];
-      vf_four(xp, a.V, s * 32 + lane, ap, vp);
-      vf_four(xq, a.V, s * 32 + lane, aq, vq);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool there = s * kVdSeg + 4 * lane + e < a.V;
-        zp += there ? tp(vp[e], table) : 0.0;
-        zq += there ? tq(vq[e], table) : 0.0;
+      double vp[4], vq[4];
+      look(tp, xp, ap, s, vp);
+      look(tq, xq, aq, s, vq);
+      zp += (vp[0] + vp[1]) + (vp[2] + vp[3]);
+      zq += (vq[0] + vq[1]) + (vq[2] + vq[3]);
+      if (cached) {
+        double2* at = keep + (size_t)(s - s0) * 128 + lane;
+        at[0] = make_double2(vp[0], vp[1]);
+        at[32] = make_double2(vp[2], vp[3]);
+        at[64] = make_double2(vq[0], vq[1]);
+        at[96] = make_double2(vq[2], vq[3]);
       }
     }
     block_total(zp, &shared_tot[0]);
@@ -420,20 +437,32 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
   }
   for (int turn = rest ? 0 : 1; turn < 2; ++turn) {       // (the second where p and q leave nothing)
     const bool minus = turn == 0;
-    // the four terms of a lane in a segment
+    // what is drawn from: the four terms of a lane in a segment (a warp reads what it kept itself, and
+    // the segment that is drawn from after a barrier)
     auto terms = [&](int s, double (&v)[4]) {
-      float vp[4], vq[4];
-      vf_four(xp, a.V, s * 32 + lane, ap, vp);
-      if (minus && minus_q) vf_four(xq, a.V, s * 32 + lane, aq, vq);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int id = s * kVdSeg + 4 * lane + e;
-        double t = id < a.V ? tp(vp[e], table) : 0.0;
-        if (minus) {
-          if (minus_q) t = id < a.V ? fmax(t - weight * tq(vq[e], table), 0.0) : 0.0;
-          else if (id == d) t = 0.0;
+      if (minus && minus_q) {
+        double vq[4];
+        if (cached) {
+          const double2* at = keep + (size_t)(s - s0) * 128 + lane;
+          const double2 p0 = at[0], p1 = at[32], q0 = at[64], q1 = at[96];
+          v[0] = p0.x; v[1] = p0.y; v[2] = p1.x; v[3] = p1.y;
+          vq[0] = q0.x; vq[1] = q0.y; vq[2] = q1.x; vq[3] = q1.y;
+        } else {
+          look(tp, xp, ap, s, v);
+          look(tq, xq, aq, s, vq);
         }
-        v[e] = t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double r = fma(-weight, vq[e], v[e]);
+          v[e] = r > 0.0 ? r : 0.0;
+        }
+        return;
+      }
+      look(tp, xp, ap, s, v);
+      if (minus) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (s * kVdSeg + 4 * lane + e == d) v[e] = 0.0;
       }
     };
     double mine = 0.0;
@@ -893,7 +922,10 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
   int C = 8;
   while (C > 1 && (B * C > 4 * kSmCount || V < 1024 * C)) C >>= 1;
   const int segs = ((V + kVdSeg - 1) / kVdSeg + C - 1) / C + 1;
-  const size_t smem = (size_t)segs * 8;
+  const int room = (segs + 1) & ~1;
+  // (two CTAs fit an SM with up to 100 KB of terms each)
+  const int cached = a.draft_logits && (size_t)segs * kVdSeg * 16 <= 100 * 1024;
+  const size_t smem = (size_t)room * 8 + (cached ? (size_t)segs * kVdSeg * 16 : 0);
   if (smem > 200 * 1024) return kBadArgument;
   cudaError_t e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
@@ -911,6 +943,6 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, verify_draw_kernel, a);
+  e = cudaLaunchKernelEx(&cfg, verify_draw_kernel, a, room, cached);
   return e == cudaSuccess ? launch_status() : (int)e;
 }

@@ -6,12 +6,13 @@ from cretif_b200.csrc import ops
 
 
 def walk(groups, news, starts, nh, nkv, tile_rows, own_rows, ctas):
-    pre, own, splits, pieces, rows, tok_pieces, tok_seq, prefix = ops._shared_items(
+    pre, own, splits, pieces, rows, tok_pieces, prefix = ops._shared_items(
         groups, news, starts, nh, nkv, tile_rows, own_rows, ctas)
     g = nh // nkv
     cu = [0]
     for n in news:
         cu.append(cu[-1] + n)
+    tok_seq = [b for b in range(len(news)) for _ in range(news[b])]
     seen = {}
     for i in range(0, len(pre), 8):
         base, row0, n, member, b0, b1, piece, _ = pre[i:i + 8]
@@ -31,9 +32,10 @@ def walk(groups, news, starts, nh, nkv, tile_rows, own_rows, ctas):
                 assert (t, h, blk) in seen
     assert len(seen) == g * sum(prefix[b] // 64 * news[b] for b in range(len(news)))
     mine = set()
-    for i in range(0, len(own), 4):
-        b, row0, n, _ = own[i:i + 4]
-        assert 0 < n <= own_rows
+    for i in range(0, len(own), 8):
+        b, tok0, row0, n, shared, mine_pieces = own[i:i + 6]
+        assert 0 < n <= own_rows and tok0 == cu[b] and shared == prefix[b]
+        assert all(tok_pieces[t] == mine_pieces for t in range(cu[b], cu[b + 1]))
         for r in range(row0, row0 + n):
             assert (b, r) not in mine
             mine.add((b, r))
