@@ -17,13 +17,18 @@ namespace cretif {
 //   warps 0-3  softmax: a thread owns a row (a lane of tensor memory);
 //   warp 4     TMA producer: K and V tiles straight out of the block cache;
 //   warp 5     one thread issues S = Q K^T and O += P V.
-// Tensor memory: two score tiles of 64 columns, O.  A row's thread writes its probabilities as
+// Tensor memory: two score tiles of 64 columns, O, and for head sizes up to 64 the queries (as A
+// operand in shared memory, read again for every 64 keys, they took the memory's bandwidth: a product
+// of 16 channels reads 6 KB instead of 2).  A row's thread writes its probabilities as
 // bfloat16 over the scores it has read, from where the product P V takes them as its A operand; it
 // adds into O itself, since a row's reference for the exponentials moves only when a score exceeds
 // it by 2^8 (then the row's thread waits for the product before and scales O).
 // The tiles come in pairs: {K_0, K_1}, then {V_j, K_{j+2}}: one barrier to wait for a step, and one
 // commit a step, behind P V of step j and the scores of step j + 2, which tells the softmax threads
 // that the scores are there and the producer that the pair may be replaced.
+// (An issuing thread pays 200 to 250 cycles for a wait, even one that is over, so the step's two are
+// polled together.  One thread for the scores and one for P V, which then wait for each other, was
+// slower: 135 us against 115 with 64 answers with drafts at 30,016.)
 //
 // Few rows (FOLD = 2 or 4: up to 64 or 32): the rows lie in tensor memory FOLD times, and each copy
 // takes its share of every step's keys (zeros stand for the others), so that all four warps work;
@@ -34,11 +39,11 @@ constexpr int kSpDone = 8;                // commit c arrives on barrier c % 8 (
 struct SpSmem {
   int q, ring, pairs, bars, xch, total;
   __host__ __device__ explicit SpSmem(int n_sub) {
-    pairs = n_sub == 1 ? 5 : 2;
+    pairs = n_sub == 1 ? 6 : 2;
     q = 0;
-    ring = n_sub * kSpRows * 128;
+    ring = n_sub == 1 ? 0 : n_sub * kSpRows * 128;
     bars = ring + pairs * 2 * n_sub * kSpTile;
-    xch = bars + (kSpDone + 5 + 3) * 8 + 16;
+    xch = bars + (kSpDone + 6 + 4) * 8 + 16;
     total = xch + kSpRows * 8 + 1024;
   }
 };
@@ -62,6 +67,28 @@ __device__ __forceinline__ uint64_t sp_desc_v(const void* tile) {
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
   return d;
+}
+
+// Wait for two barriers at once: the polls of both are in flight together.
+__device__ __forceinline__ bool sp_wait_both(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, volatile int* abort) {
+  const uint32_t aa = tc::smem_u32(a), ab = tc::smem_u32(b);
+  for (unsigned spin = 0; spin < tc::kSpinLimit; ++spin) {
+    uint32_t oa, ob;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%2], %3;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 q, [%4], %5;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "selp.u32 %1, 1, 0, q;\n\t}"
+        : "=r"(oa), "=r"(ob)
+        : "r"(aa), "r"(pa), "r"(ab), "r"(pb)
+        : "memory");
+    if (oa & ob) return true;
+    if (!oa) { if (!tc::mbar_wait(a, pa, abort)) return false; }
+    else if (!tc::mbar_wait(b, pb, abort)) return false;
+  }
+  *abort = 1;
+  return false;
 }
 
 template <int FOLD>
@@ -153,7 +180,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const SpSmem L(n_sub);
   uint64_t* done = reinterpret_cast<uint64_t*>(smem + L.bars);
   uint64_t* full = done + kSpDone;
-  uint64_t* p_full = full + 5;
+  uint64_t* p_full = full + 6;
   uint64_t* q_full = p_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -167,7 +194,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const int span = kSpRows / fold;                       // lanes of a copy
   // warps whose lanes hold rows: the others neither wait nor arrive
   const int warps_a_copy = (it.n_rows + 31) >> 5;
-  constexpr uint32_t kColO = 128;
+  constexpr uint32_t kColO = 128, kColQ = 192;            // (kColQ: up to 64 channels)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSpDone; ++i) tc::mbar_init(&done[i], 1);
@@ -238,9 +265,16 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       const uint64_t tile = (uint64_t)((n_sub * kSpTile) >> 4);   // a tile, in descriptor units
       auto scores = [&](int j, int slot) {                // K_j is tile `slot` of the ring
         const uint64_t kd = kd0 + slot * tile;
-        for (int kk = 0; kk < k_steps; ++kk)
-          tc::umma_bf16(tmem + (uint32_t)(j & 1) * 64, qd + (uint64_t)((kk >> 2) * ((kSpRows * 128) >> 4) + 2 * (kk & 3)),
-                        kd + (uint64_t)((kk >> 2) * (kSpTile >> 4) + 2 * (kk & 3)), idesc_qk, kk != 0);
+        const uint32_t d = tmem + (uint32_t)(j & 1) * 64;
+        if (n_sub == 1) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk < k_steps) tc::umma_bf16_a_tmem(d, tmem + kColQ + 8 * kk, kd + 2 * kk, idesc_qk, kk != 0);
+        } else {
+          for (int kk = 0; kk < k_steps; ++kk)
+            tc::umma_bf16(d, qd + (uint64_t)((kk >> 2) * ((kSpRows * 128) >> 4) + 2 * (kk & 3)),
+                          kd + (uint64_t)((kk >> 2) * (kSpTile >> 4) + 2 * (kk & 3)), idesc_qk, kk != 0);
+        }
       };
       bool ok = tc::mbar_wait(q_full, 0u, abort) && tc::mbar_wait(&full[0], 0u, abort);
       if (ok) {
@@ -251,8 +285,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         tc::umma_commit(&done[1]);
       }
       for (int j = 0, s = 1, turn = 0; j < n && ok; ++j) {   // pair j + 1 in slot s
-        ok = tc::mbar_wait(&full[s], (uint32_t)(turn & 1), abort) &&
-             tc::mbar_wait(&p_full[j & 1], (uint32_t)((j >> 1) & 1), abort);
+        ok = sp_wait_both(&full[s], (uint32_t)(turn & 1), &p_full[j & 1], (uint32_t)((j >> 1) & 1), abort);
         if (!ok) break;
         tc::tc_fence_after();
         const uint64_t vd = vd0 + 2 * s * tile;
@@ -266,7 +299,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       }
     }
   } else {
-    // ---- the queries into shared memory, in the operand's swizzled layout
+    // ---- the queries into tensor memory, or into shared memory
     const int row = threadIdx.x, copy = row / span, r = row - copy * span;
     {
       const bool there = r < it.n_rows;
@@ -275,12 +308,24 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       if (there)
         src = static_cast<const __nv_bfloat16*>(a.q) + (size_t)a.rows[it.row_base + rr / g] * a.ldq +
               (size_t)(kvh * g + rr % g) * hd;
-      for (int ch = 0; ch < hd >> 3; ++ch) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (there) v = *reinterpret_cast<const uint4*>(src + 8 * ch);
-        *reinterpret_cast<uint4*>(smem + L.q + (ch >> 3) * kSpRows * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      if (n_sub == 1) {                                   // two channels a column
+        uint32_t all[32];
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
+          const uint4 v = there && 8 * ch < hd ? *reinterpret_cast<const uint4*>(src + 8 * ch) : zero;
+          all[4 * ch] = v.x; all[4 * ch + 1] = v.y; all[4 * ch + 2] = v.z; all[4 * ch + 3] = v.w;
+        }
+        tc::tmem_store_32(tmem + ((uint32_t)(warp * 32) << 16) + kColQ, all);
+        tc::tmem_store_wait();
+        tc::tc_fence_before();
+      } else {                                            // the operand's swizzled layout
+        for (int ch = 0; ch < hd >> 3; ++ch) {
+          const uint4 v = there ? *reinterpret_cast<const uint4*>(src + 8 * ch) : zero;
+          *reinterpret_cast<uint4*>(smem + L.q + (ch >> 3) * kSpRows * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
+        }
+        tc::fence_proxy_async();
       }
-      tc::fence_proxy_async();
       tc::mbar_arrive(q_full);
     }
     const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
@@ -365,8 +410,8 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 }
 
 // ---------------------------------------------------------------------------------------
-// Own keys: a CTA takes up to 16 rows of one sequence and key/value head; its four warps take 16 keys
-// of every block each, straight from the cache into the operands' registers.
+// Own keys: up to 16 rows of one sequence and key/value head are an item; its warps take 16 keys each
+// in turn, straight from the cache into the operands' registers.
 //   S = Q K^T (m16n8k16): the channels of 32 are taken in an order in which a lane's 16 bytes of a
 //   key are its part of two products (channels 8c .. 8c + 7 of lane c: pairs 0 and 1 in the first,
 //   2 and 3 in the second), the same for the queries.
@@ -374,22 +419,33 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 //   of eight products; two keys' values are brought together by byte permutes.
 // No shared memory and no barrier inside the loop; a step's keys are asked for when the step before
 // has taken its own, its values likewise.  NR = 1: up to 8 rows, and the products' other 8 are empty.
-// With JOIN the CTA holds all of the rows' own keys and joins the rows' prefix pieces itself (it is
-// launched while the prefix kernel runs and waits for it only then); else it leaves pieces.
+// WPI warps share an item, a CTA has four.  Four an item where there are few; one where there are items
+// enough to fill the chip with warps (64 sequences on 32 key/value heads, some 95 own keys: AN_ITEM4 us with
+// four, AN_ITEM1 with one, and no barrier between them).
+// With JOIN the item's warps hold all of the rows' own keys and join the rows' prefix pieces (the kernel is
+// launched while the prefix kernel runs and waits for it only then); else they leave pieces.
 constexpr int kSoWarps = 4, kSoThreads = kSoWarps * 32;
 
-template <int HDG, int NR, bool JOIN>
+template <int HDG, int NR, int WPI, bool JOIN>
 __global__ void __launch_bounds__(kSoThreads)
 shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
   extern __shared__ __align__(16) float so_smem[];
   const int hd = a.hd, g = a.nh / a.nkv, kvh = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int split = JOIN ? 0 : blockIdx.x % a.own_splits, splits = JOIN ? 1 : a.own_splits;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int of_cta = (threadIdx.x >> 5) / WPI, warp = (threadIdx.x >> 5) % WPI;   // item, warp of the item
+  const int index = blockIdx.x * (kSoWarps / WPI) + of_cta;
+  const int split = JOIN ? 0 : index % a.own_splits, splits = JOIN ? 1 : a.own_splits;
+  const int which = JOIN ? index : index / a.own_splits;
+  const bool none = which >= a.n_own;                     // (a warp of its own: WPI is 1)
   // (the plan is never written by a kernel)
-  const SharedOwnItem it = a.own[JOIN ? blockIdx.x : blockIdx.x / a.own_splits];
+  const SharedOwnItem it = a.own[none ? 0 : which];
   if (!after_prefix) dependent_wait();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int prefix = it.prefix, blk0 = prefix / kShBlk, key_in = warp * 16;
+  if (none) {
+    if (after_prefix) dependent_wait();
+    return;
+  }
+  const int prefix = it.prefix, blk0 = prefix / kShBlk;
   const int slot = a.seq_slot[it.seq];
   int pos[NR];
   const int last = a.tok_pos[it.tok0 + (it.row0 + it.n_rows - 1) / g];
@@ -421,18 +477,19 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
   float m[NR], l[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
-  const int blocks = (end - prefix + kShBlk - 1) / kShBlk;
-  auto has = [&](int i) { return i < blocks && prefix + i * kShBlk + key_in < end; };
-  auto block = [&](int i) { return has(i) ? shared_block_of(a, slot, blk0 + i) : 0; };
+  // 16 keys a warp and step, from key 16 i of the own ones on
+  const int first = split * WPI + warp, stride = splits * WPI;
+  auto has = [&](int i) { return prefix + 16 * i < end; };
+  auto block = [&](int i) { return has(i) ? shared_block_of(a, slot, blk0 + (i >> 2)) : 0; };
   uint4 kr[HDG * 2][2], vr[HDG][4];
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  // keys key_in .. + 15 of own block i, which is physical block blk
-  auto tile = [&](const void* cache, int blk) {
-    return static_cast<const __nv_bfloat16*>(cache) + (((size_t)blk * a.nkv + kvh) * kShBlk + key_in) * hd;
+  // (they lie in physical block blk)
+  auto tile = [&](const void* cache, int i, int blk) {
+    return static_cast<const __nv_bfloat16*>(cache) + (((size_t)blk * a.nkv + kvh) * kShBlk + (i & 3) * 16) * hd;
   };
   auto load_k = [&](int i, int blk) {
-    const int n = end - (prefix + i * kShBlk + key_in);   // (nothing past the last key is looked at)
-    const __nv_bfloat16* p = tile(a.kc, blk);
+    const int n = end - (prefix + 16 * i);                // (nothing past the last key is looked at)
+    const __nv_bfloat16* p = tile(a.kc, i, blk);
 #pragma unroll
     for (int d = 0; d < HDG * 2; ++d)
 #pragma unroll
@@ -441,8 +498,8 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
             ? __ldg(reinterpret_cast<const uint4*>(p + (8 * x + r) * hd + 32 * d + 8 * c)) : zero;
   };
   auto load_v = [&](int i, int blk) {
-    const int n = end - (prefix + i * kShBlk + key_in);
-    const __nv_bfloat16* p = tile(a.vc, blk);
+    const int n = end - (prefix + 16 * i);
+    const __nv_bfloat16* p = tile(a.vc, i, blk);
 #pragma unroll
     for (int v = 0; v < HDG; ++v)
 #pragma unroll
@@ -452,13 +509,13 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
             ? __ldg(reinterpret_cast<const uint4*>(p + key * hd + 64 * v + 8 * r)) : zero;
       }
   };
-  int blk = block(split), ahead = block(split + splits);
-  if (has(split)) { load_k(split, blk); load_v(split, blk); }
-  for (int i = split; has(i); i += splits) {
-    const int key0 = prefix + i * kShBlk + key_in;
-    const bool more = has(i + splits);
+  int blk = block(first), ahead = block(first + stride);
+  if (has(first)) { load_k(first, blk); load_v(first, blk); }
+  for (int i = first; has(i); i += stride) {
+    const int key0 = prefix + 16 * i;
+    const bool more = has(i + stride);
     blk = ahead;
-    ahead = block(i + 2 * splits);
+    ahead = block(i + 2 * stride);
     float s[2][4];
 #pragma unroll
     for (int x = 0; x < 2; ++x)
@@ -473,7 +530,7 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
         mma_16816_f32(s[x], qa[d][0][2], NR == 2 ? qa[d][NR - 1][2] : 0u, qa[d][0][3], NR == 2 ? qa[d][NR - 1][3] : 0u,
                       kr[d][x].z, kr[d][x].w);
       }
-    if (more) load_k(i + splits, blk);
+    if (more) load_k(i + stride, blk);
     uint32_t pa[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int w = 0; w < NR; ++w) {                        // rows r, r + 8
@@ -519,12 +576,12 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
         for (int e = 0; e < 2 * NR; ++e) o[v][t][e] = acc[e];
       }
     }
-    if (more) load_v(i + splits, blk);
+    if (more) load_v(i + stride, blk);
   }
   // ---- the warps' parts meet in shared memory: a lane has channels 16c .. 16c + 15 of its rows
   const int ld = hd + 4;
-  float* so = so_smem;                                    // [warp][8 NR][hd + 4]
-  float2* sml = reinterpret_cast<float2*>(so + kSoWarps * 8 * NR * ld);    // [warp][8 NR]
+  float* so = so_smem + of_cta * WPI * 8 * NR * ld;       // [warp][8 NR][hd + 4]
+  float2* sml = reinterpret_cast<float2*>(so_smem + kSoWarps * 8 * NR * ld) + of_cta * WPI * 8 * NR;   // [warp][8 NR]
 #pragma unroll
   for (int w = 0; w < NR; ++w) {
     l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
@@ -548,10 +605,11 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
   // The prefix pieces are there; and this kernel ends behind the prefix kernel, so that what waits
   // for this one need not wait for that one.
   if (after_prefix) dependent_wait();
-  __syncthreads();
+  if (WPI == 1) __syncwarp();
+  else __syncthreads();
   const int quads = hd >> 2, n_pieces = JOIN ? it.pieces : 0;
   const size_t rows_all = (size_t)a.T * a.nh;
-  for (int i = threadIdx.x; i < it.n_rows * quads; i += kSoThreads) {
+  for (int i = warp * 32 + lane; i < it.n_rows * quads; i += WPI * 32) {
     const int row = i / quads, ch = (i - row * quads) * 4, rr = it.row0 + row;
     const int t = it.tok0 + rr / g, h = kvh * g + rr % g;
     const size_t at = (size_t)t * a.nh + h;
@@ -590,10 +648,10 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
       }
       add(ml, x);
     }
-    float2 ml[kSoWarps];
-    float4 x[kSoWarps];
+    float2 ml[WPI];
+    float4 x[WPI];
 #pragma unroll
-    for (int w = 0; w < kSoWarps; ++w) {
+    for (int w = 0; w < WPI; ++w) {
       ml[w] = sml[w * 8 * NR + row];
       x[w] = *reinterpret_cast<const float4*>(so + (w * 8 * NR + row) * ld + ch);
     }
@@ -638,9 +696,13 @@ template <int HDG, int NR>
 static int launch_own(const SharedArgs& a, cudaStream_t st) {
   const size_t smem = (size_t)(kSoWarps * 8 * NR * (a.hd + 4) + kSoWarps * 8 * NR * 2) * 4;
   const int after = a.n_pre > 0;
-  const dim3 grid(a.n_own * a.own_splits, a.nkv);
-  return a.own_splits == 1 ? sp_launch(shared_own_mma_kernel<HDG, NR, true>, grid, kSoThreads, smem, st, a, after)
-                           : sp_launch(shared_own_mma_kernel<HDG, NR, false>, grid, kSoThreads, smem, st, a, after);
+  if (a.own_splits > 1)
+    return sp_launch(shared_own_mma_kernel<HDG, NR, 4, false>, dim3(a.n_own * a.own_splits, a.nkv), kSoThreads, smem, st,
+                     a, after);
+  if ((long long)a.n_own * a.nkv * kSoWarps > 32LL * kSmCount)
+    return sp_launch(shared_own_mma_kernel<HDG, NR, 1, true>, dim3((a.n_own + 3) / 4, a.nkv), kSoThreads, smem, st, a,
+                     after);
+  return sp_launch(shared_own_mma_kernel<HDG, NR, 4, true>, dim3(a.n_own, a.nkv), kSoThreads, smem, st, a, after);
 }
 
 // The prefix pieces and the own keys; joins the rows where the own keys are in one piece.
