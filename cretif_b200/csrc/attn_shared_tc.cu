@@ -411,34 +411,47 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 
 // ---------------------------------------------------------------------------------------
 // Own keys: up to 16 rows of one sequence and key/value head are an item; its warps take 16 keys each
-// in turn, straight from the cache into the operands' registers.
-//   S = Q K^T (m16n8k16): the channels of 32 are taken in an order in which a lane's 16 bytes of a
-//   key are its part of two products (channels 8c .. 8c + 7 of lane c: pairs 0 and 1 in the first,
-//   2 and 3 in the second), the same for the queries.
-//   O += P V: column n of product t is channel 8 n + t, so a lane's 16 bytes of a key are its part
-//   of eight products; two keys' values are brought together by byte permutes.
-// No shared memory and no barrier inside the loop; a step's keys are asked for when the step before
-// has taken its own, its values likewise.  NR = 1: up to 8 rows, and the products' other 8 are empty.
+// in turn.  A warp fetches its own keys and values (boxes of 16 keys, TMA, 128-byte swizzle) into a ring
+// of its own and needs no other warp until the end: scores and P V are m16n8k16 products with the
+// rows as their rows (NR = 1: up to 8 rows, and the products' other 8 are empty).
+// (Keys and values straight into the operands' registers, with no shared memory, took 120 registers and
+// kept 4 KB a warp in flight: 22 us against NOW_OWN for 64 sequences on 32 heads with 95 own keys.)
 // WPI warps share an item, a CTA has four.  Four an item where there are few; one where there are items
-// enough to fill the chip with warps (64 sequences on 32 key/value heads, some 95 own keys: AN_ITEM4 us with
-// four, AN_ITEM1 with one, and no barrier between them).
+// enough to fill the chip with warps.
 // With JOIN the item's warps hold all of the rows' own keys and join the rows' prefix pieces (the kernel is
 // launched while the prefix kernel runs and waits for it only then); else they leave pieces.
-constexpr int kSoWarps = 4, kSoThreads = kSoWarps * 32;
+constexpr int kSoWarps = 4, kSoThreads = kSoWarps * 32, kSoKeys = 16, kSoStages = 3;
+template <int HDG>
+constexpr int kSoStage = 2 * HDG * kSoKeys * 128;         // bytes: keys, then values
 
 template <int HDG, int NR, int WPI, bool JOIN>
 __global__ void __launch_bounds__(kSoThreads)
-shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
-  extern __shared__ __align__(16) float so_smem[];
+shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ SharedArgs a, int after_prefix) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int hd = a.hd, g = a.nh / a.nkv, kvh = blockIdx.y;
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int of_cta = (threadIdx.x >> 5) / WPI, warp = (threadIdx.x >> 5) % WPI;   // item, warp of the item
+  const int cta_warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int of_cta = cta_warp / WPI, warp = cta_warp % WPI;   // item, warp of the item
   const int index = blockIdx.x * (kSoWarps / WPI) + of_cta;
   const int split = JOIN ? 0 : index % a.own_splits, splits = JOIN ? 1 : a.own_splits;
   const int which = JOIN ? index : index / a.own_splits;
   const bool none = which >= a.n_own;                     // (a warp of its own: WPI is 1)
   // (the plan is never written by a kernel)
   const SharedOwnItem it = a.own[none ? 0 : which];
+  constexpr int kRing = kSoStages * kSoStage<HDG>;
+  unsigned char* ring = smem + cta_warp * kRing;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kSoWarps * kRing) + cta_warp * kSoStages;
+  int* abort_word = reinterpret_cast<int*>(smem + kSoWarps * kRing + kSoWarps * kSoStages * 8) + cta_warp;
+  volatile int* abort = abort_word;                       // (of the warp)
+  if (lane == 0) {
+    for (int i = 0; i < kSoStages; ++i) tc::mbar_init(&full[i], 1);
+    *abort = 0;
+    tc::fence_barrier_init();
+    tc::tma_prefetch_descriptor(&map_k);
+    tc::tma_prefetch_descriptor(&map_v);
+  }
+  __syncwarp();
   if (!after_prefix) dependent_wait();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (none) {
@@ -447,10 +460,36 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
   }
   const int prefix = it.prefix, blk0 = prefix / kShBlk;
   const int slot = a.seq_slot[it.seq];
-  int pos[NR];
   const int last = a.tok_pos[it.tok0 + (it.row0 + it.n_rows - 1) / g];
+  const int end = shared_own_end(a, prefix, last);
+  // 16 keys a warp and step: keys 16 i .. of the own ones, i = first, first + stride, ...
+  const int first = split * WPI + warp, stride = splits * WPI;
+  const int chunks = (end - prefix + kSoKeys - 1) / kSoKeys;
+  const int steps = chunks > first ? (chunks - first + stride - 1) / stride : 0;
+  // the physical blocks of 32 steps, a lane each
+  auto window = [&](int k0) {
+    return k0 + lane < steps ? shared_block_of(a, slot, blk0 + ((first + (k0 + lane) * stride) >> 2)) : 0;
+  };
+  int blocks = window(0);
+  auto fetch = [&](int k) {                               // step k into the ring
+    if (k > 0 && (k & 31) == 0) blocks = window(k);
+    const int blk = __shfl_sync(0xffffffffu, blocks, k & 31);
+    if (lane == 0) {
+      const int s = k % kSoStages, i = first + k * stride;
+      const int row = (blk * a.nkv + kvh) * kShBlk + (i & 3) * kSoKeys;
+      unsigned char* at = ring + s * kSoStage<HDG>;
+      tc::mbar_expect_tx(&full[s], (uint32_t)kSoStage<HDG>);
+#pragma unroll
+      for (int sub = 0; sub < HDG; ++sub) {
+        tc::tma_load_2d(at + sub * kSoKeys * 128, &map_k, 64 * sub, row, &full[s]);
+        tc::tma_load_2d(at + (HDG + sub) * kSoKeys * 128, &map_v, 64 * sub, row, &full[s]);
+      }
+    }
+  };
+  for (int k = 0; k < kSoStages && k < steps; ++k) fetch(k);
   // ---- queries: row r (and r + 8)
-  uint32_t qa[HDG * 2][NR][4];                            // [32 channels][row][pair]
+  uint32_t qa[HDG * 4][NR][2];                            // [16 channels][row][half]
+  int pos[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const int row = r + 8 * i, rr = it.row0 + row;
@@ -460,77 +499,43 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
     const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.ldq +
                                (size_t)(kvh * g + (there ? rr % g : 0)) * hd;
 #pragma unroll
-    for (int d = 0; d < HDG * 2; ++d) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (there && 32 * d + 8 * c < hd) v = *reinterpret_cast<const uint4*>(src + 32 * d + 8 * c);
-      qa[d][i][0] = v.x; qa[d][i][1] = v.y; qa[d][i][2] = v.z; qa[d][i][3] = v.w;
+    for (int d = 0; d < HDG * 4; ++d) {
+      const bool in = there && 16 * d < hd;
+      qa[d][i][0] = in ? *reinterpret_cast<const uint32_t*>(src + 16 * d + 2 * c) : 0u;
+      qa[d][i][1] = in ? *reinterpret_cast<const uint32_t*>(src + 16 * d + 8 + 2 * c) : 0u;
     }
   }
-  const int end = shared_own_end(a, prefix, last);
-  float o[HDG][8][2 * NR];
+  float o[HDG * 8][2 * NR];                               // [8 channels][row: 2c, 2c + 1]
 #pragma unroll
-  for (int v = 0; v < HDG; ++v)
+  for (int t = 0; t < HDG * 8; ++t)
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-#pragma unroll
-      for (int e = 0; e < 2 * NR; ++e) o[v][t][e] = 0.f;
+    for (int e = 0; e < 2 * NR; ++e) o[t][e] = 0.f;
   float m[NR], l[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
-  // 16 keys a warp and step, from key 16 i of the own ones on
-  const int first = split * WPI + warp, stride = splits * WPI;
-  auto has = [&](int i) { return prefix + 16 * i < end; };
-  auto block = [&](int i) { return has(i) ? shared_block_of(a, slot, blk0 + (i >> 2)) : 0; };
-  uint4 kr[HDG * 2][2], vr[HDG][4];
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  // (they lie in physical block blk)
-  auto tile = [&](const void* cache, int i, int blk) {
-    return static_cast<const __nv_bfloat16*>(cache) + (((size_t)blk * a.nkv + kvh) * kShBlk + (i & 3) * 16) * hd;
-  };
-  auto load_k = [&](int i, int blk) {
-    const int n = end - (prefix + 16 * i);                // (nothing past the last key is looked at)
-    const __nv_bfloat16* p = tile(a.kc, i, blk);
-#pragma unroll
-    for (int d = 0; d < HDG * 2; ++d)
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        kr[d][x] = 8 * x + r < n && 32 * d + 8 * c < hd
-            ? __ldg(reinterpret_cast<const uint4*>(p + (8 * x + r) * hd + 32 * d + 8 * c)) : zero;
-  };
-  auto load_v = [&](int i, int blk) {
-    const int n = end - (prefix + 16 * i);
-    const __nv_bfloat16* p = tile(a.vc, i, blk);
-#pragma unroll
-    for (int v = 0; v < HDG; ++v)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int key = 2 * c + (x & 1) + 8 * (x >> 1);
-        vr[v][x] = key < n && 64 * v + 8 * r < hd
-            ? __ldg(reinterpret_cast<const uint4*>(p + key * hd + 64 * v + 8 * r)) : zero;
-      }
-  };
-  int blk = block(first), ahead = block(first + stride);
-  if (has(first)) { load_k(first, blk); load_v(first, blk); }
-  for (int i = first; has(i); i += stride) {
-    const int key0 = prefix + 16 * i;
-    const bool more = has(i + stride);
-    blk = ahead;
-    ahead = block(i + 2 * stride);
-    float s[2][4];
+  const int mat = lane >> 3, rin = lane & 7;
+  bool ok = true;
+  for (int k = 0, s = 0, turn = 0; k < steps; ++k) {
+    if (!tc::mbar_wait(&full[s], (uint32_t)(turn & 1), abort)) { ok = false; break; }
+    const int key0 = prefix + (first + k * stride) * kSoKeys, n = end - key0;
+    const uint32_t kbase = tc::smem_u32(ring + s * kSoStage<HDG>), vbase = kbase + HDG * kSoKeys * 128;
+    float sc[2][4];
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[x][e] = 0.f;
+      for (int e = 0; e < 4; ++e) sc[x][e] = 0.f;
 #pragma unroll
-    for (int d = 0; d < HDG * 2; ++d)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        mma_16816_f32(s[x], qa[d][0][0], NR == 2 ? qa[d][NR - 1][0] : 0u, qa[d][0][1], NR == 2 ? qa[d][NR - 1][1] : 0u,
-                      kr[d][x].x, kr[d][x].y);
-        mma_16816_f32(s[x], qa[d][0][2], NR == 2 ? qa[d][NR - 1][2] : 0u, qa[d][0][3], NR == 2 ? qa[d][NR - 1][3] : 0u,
-                      kr[d][x].z, kr[d][x].w);
+    for (int d = 0; d < HDG * 4; ++d) {
+      if (16 * d < hd) {
+        const int key = (mat >> 1) * 8 + rin, chunk = 2 * d + (mat & 1);
+        uint32_t kb[4];
+        ldmatrix_x4(kb, kbase + (chunk >> 3) * (kSoKeys * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+        mma_16816_f32(sc[0], qa[d][0][0], NR == 2 ? qa[d][NR - 1][0] : 0u, qa[d][0][1], NR == 2 ? qa[d][NR - 1][1] : 0u,
+                      kb[0], kb[1]);
+        mma_16816_f32(sc[1], qa[d][0][0], NR == 2 ? qa[d][NR - 1][0] : 0u, qa[d][0][1], NR == 2 ? qa[d][NR - 1][1] : 0u,
+                      kb[2], kb[3]);
       }
-    if (more) load_k(i + stride, blk);
+    }
     uint32_t pa[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int w = 0; w < NR; ++w) {                        // rows r, r + 8
@@ -538,7 +543,7 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = key0 + 8 * (e >> 1) + 2 * c + (e & 1);
-        t4[e] = key <= pos[w] ? s[e >> 1][2 * w + (e & 1)] * a.scale_log2 : -INFINITY;
+        t4[e] = key <= pos[w] ? sc[e >> 1][2 * w + (e & 1)] * a.scale_log2 : -INFINITY;
         mx = fmaxf(mx, t4[e]);
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -556,50 +561,54 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
       pa[w] = pack_bf16(p[0], p[1]);
       pa[2 + w] = pack_bf16(p[2], p[3]);
 #pragma unroll
-      for (int v = 0; v < HDG; ++v)
-#pragma unroll
-        for (int t = 0; t < 8; ++t) { o[v][t][2 * w] *= alpha; o[v][t][2 * w + 1] *= alpha; }
+      for (int t = 0; t < HDG * 8; ++t) { o[t][2 * w] *= alpha; o[t][2 * w + 1] *= alpha; }
     }
+    // values past the last key count for nothing, whatever they are
+    const bool whole = n >= kSoKeys;
+    const uint32_t keep0 = (2 * c < n ? 0xffffu : 0u) | (2 * c + 1 < n ? 0xffff0000u : 0u);
+    const uint32_t keep1 = (2 * c + 8 < n ? 0xffffu : 0u) | (2 * c + 9 < n ? 0xffff0000u : 0u);
 #pragma unroll
-    for (int v = 0; v < HDG; ++v) {
-      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[v][0]);
-      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[v][1]);
-      const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[v][2]);
-      const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vr[v][3]);
+    for (int d = 0; d < HDG * 4; ++d) {
+      if (16 * d < hd) {
+        const int key = (mat & 1) * 8 + rin, chunk = 2 * d + (mat >> 1);
+        uint32_t vb[4];
+        ldmatrix_x4_trans(vb, vbase + (chunk >> 3) * (kSoKeys * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+        if (!whole) { vb[0] &= keep0; vb[1] &= keep1; vb[2] &= keep0; vb[3] &= keep1; }
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const unsigned sel = t & 1 ? 0x7632u : 0x5410u;
-        float acc[4] = {o[v][t][0], o[v][t][1], NR == 2 ? o[v][t][2 * NR - 2] : 0.f, NR == 2 ? o[v][t][2 * NR - 1] : 0.f};
-        mma_16816_f32(acc, pa[0], pa[1], pa[2], pa[3], __byte_perm(w0[t >> 1], w1[t >> 1], sel),
-                      __byte_perm(w2[t >> 1], w3[t >> 1], sel));
+        for (int x = 0; x < 2; ++x) {
+          float* to = o[2 * d + x];
+          float acc[4] = {to[0], to[1], NR == 2 ? to[2 * NR - 2] : 0.f, NR == 2 ? to[2 * NR - 1] : 0.f};
+          mma_16816_f32(acc, pa[0], pa[1], pa[2], pa[3], vb[2 * x], vb[2 * x + 1]);
 #pragma unroll
-        for (int e = 0; e < 2 * NR; ++e) o[v][t][e] = acc[e];
+          for (int e = 0; e < 2 * NR; ++e) to[e] = acc[e];
+        }
       }
     }
-    if (more) load_v(i + stride, blk);
+    if (k + kSoStages < steps) {                          // the stage has been read: its next turn
+      tc::fence_proxy_async();
+      __syncwarp();
+      fetch(k + kSoStages);
+    }
+    if (++s == kSoStages) { s = 0; ++turn; }
   }
-  // ---- the warps' parts meet in shared memory: a lane has channels 16c .. 16c + 15 of its rows
+  if (!ok && lane == 0) atomicOr(a.fault, (unsigned)kFaultWaitExpired);
+  __syncwarp();
+  // ---- the warps' parts meet in shared memory, in the rings' place
   const int ld = hd + 4;
-  float* so = so_smem + of_cta * WPI * 8 * NR * ld;       // [warp][8 NR][hd + 4]
-  float2* sml = reinterpret_cast<float2*>(so_smem + kSoWarps * 8 * NR * ld) + of_cta * WPI * 8 * NR;   // [warp][8 NR]
+  float2* sml = reinterpret_cast<float2*>(smem + (size_t)(cta_warp - warp) * kRing);      // of the item's warp 0
+  constexpr int kPart = kRing / 4;                        // a warp's part: [8 NR] (m, l), then [8 NR][hd + 4]
+  auto part_ml_of = [&](int w) { return sml + w * (kPart / 2); };
+  auto part_o_of = [&](int w) { return reinterpret_cast<float*>(sml) + w * kPart + 16 * NR; };
 #pragma unroll
   for (int w = 0; w < NR; ++w) {
     l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
     l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
-    if (c == 0) sml[warp * 8 * NR + r + 8 * w] = make_float2(m[w], l[w]);
+    if (c == 0) part_ml_of(warp)[r + 8 * w] = make_float2(m[w], l[w]);
     if (r + 8 * w < it.n_rows) {
+      float* dst = part_o_of(warp) + (r + 8 * w) * ld + 2 * c;
 #pragma unroll
-      for (int v = 0; v < HDG; ++v) {
-        float* dst = so + (warp * 8 * NR + r + 8 * w) * ld + 64 * v + 16 * c;
-        if (64 * v + 16 * c < hd) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int t = 0; t < 8; t += 4)
-              *reinterpret_cast<float4*>(dst + 8 * h + t) =
-                  make_float4(o[v][t][2 * w + h], o[v][t + 1][2 * w + h], o[v][t + 2][2 * w + h], o[v][t + 3][2 * w + h]);
-        }
-      }
+      for (int t = 0; t < HDG * 8; ++t)
+        if (8 * t < hd) *reinterpret_cast<float2*>(dst + 8 * t) = make_float2(o[t][2 * w], o[t][2 * w + 1]);
     }
   }
   // The prefix pieces are there; and this kernel ends behind the prefix kernel, so that what waits
@@ -652,8 +661,8 @@ shared_own_mma_kernel(const __grid_constant__ SharedArgs a, int after_prefix) {
     float4 x[WPI];
 #pragma unroll
     for (int w = 0; w < WPI; ++w) {
-      ml[w] = sml[w * 8 * NR + row];
-      x[w] = *reinterpret_cast<const float4*>(so + (w * 8 * NR + row) * ld + ch);
+      ml[w] = part_ml_of(w)[row];
+      x[w] = *reinterpret_cast<const float4*>(part_o_of(w) + row * ld + ch);
     }
     add(ml, x);
     if (JOIN) {
@@ -693,25 +702,25 @@ static int sp_launch(void (*kernel)(Params...), dim3 grid, int threads, size_t s
 }
 
 template <int HDG, int NR>
-static int launch_own(const SharedArgs& a, cudaStream_t st) {
-  const size_t smem = (size_t)(kSoWarps * 8 * NR * (a.hd + 4) + kSoWarps * 8 * NR * 2) * 4;
+static int launch_own(const CUtensorMap& mk, const CUtensorMap& mv, const SharedArgs& a, cudaStream_t st) {
+  constexpr size_t smem = (size_t)kSoWarps * kSoStages * (kSoStage<HDG> + 8) + kSoWarps * 4 + 1024;
   const int after = a.n_pre > 0;
   if (a.own_splits > 1)
     return sp_launch(shared_own_mma_kernel<HDG, NR, 4, false>, dim3(a.n_own * a.own_splits, a.nkv), kSoThreads, smem, st,
-                     a, after);
-  if ((long long)a.n_own * a.nkv * kSoWarps > 32LL * kSmCount)
-    return sp_launch(shared_own_mma_kernel<HDG, NR, 1, true>, dim3((a.n_own + 3) / 4, a.nkv), kSoThreads, smem, st, a,
-                     after);
-  return sp_launch(shared_own_mma_kernel<HDG, NR, 4, true>, dim3(a.n_own, a.nkv), kSoThreads, smem, st, a, after);
+                     mk, mv, a, after);
+  if ((long long)a.n_own * a.nkv > 8 * kSmCount)
+    return sp_launch(shared_own_mma_kernel<HDG, NR, 1, true>, dim3((a.n_own + 3) / 4, a.nkv), kSoThreads, smem, st, mk,
+                     mv, a, after);
+  return sp_launch(shared_own_mma_kernel<HDG, NR, 4, true>, dim3(a.n_own, a.nkv), kSoThreads, smem, st, mk, mv, a, after);
 }
 
 // The prefix pieces and the own keys; joins the rows where the own keys are in one piece.
 int launch_shared_bf16(const SharedArgs& a, cudaStream_t st) {
   if (((uintptr_t)a.q & 15) || a.ldq % 8 || ((uintptr_t)a.out & 7) || a.ldo % 4) return kMisaligned;
+  const long long cache_rows = a.n_blocks * a.nkv * kShBlk;
+  if (cache_rows > 0x7fffffffLL) return kBadArgument;
+  CUtensorMap mk, mv;
   if (a.n_pre > 0) {
-    const long long cache_rows = a.n_blocks * a.nkv * kShBlk;
-    if (cache_rows > 0x7fffffffLL) return kBadArgument;
-    CUtensorMap mk, mv;
     if (make_tile_map_bf16(&mk, a.kc, (int)cache_rows, a.hd, a.hd, kShBlk) ||
         make_tile_map_bf16(&mv, a.vc, (int)cache_rows, a.hd, a.hd, kShBlk))
       return kBadArgument;
@@ -719,8 +728,11 @@ int launch_shared_bf16(const SharedArgs& a, cudaStream_t st) {
     const int e = sp_launch(shared_prefix_tc_kernel, dim3(a.n_pre, a.nkv), kSpThreads, L.total, st, mk, mv, a);
     if (e) return e;
   }
-  if (a.own_rows <= 8) return a.hd <= 64 ? launch_own<1, 1>(a, st) : launch_own<2, 1>(a, st);
-  return a.hd <= 64 ? launch_own<1, 2>(a, st) : launch_own<2, 2>(a, st);
+  if (make_tile_map_bf16(&mk, a.kc, (int)cache_rows, a.hd, a.hd, kSoKeys) ||
+      make_tile_map_bf16(&mv, a.vc, (int)cache_rows, a.hd, a.hd, kSoKeys))
+    return kBadArgument;
+  if (a.own_rows <= 8) return a.hd <= 64 ? launch_own<1, 1>(mk, mv, a, st) : launch_own<2, 1>(mk, mv, a, st);
+  return a.hd <= 64 ? launch_own<1, 2>(mk, mv, a, st) : launch_own<2, 2>(mk, mv, a, st);
 }
 
 }  // namespace cretif
