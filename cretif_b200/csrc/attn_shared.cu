@@ -3,8 +3,7 @@
 // (attn_shared.h has the formula).  The reference decodes one sequence at a time and has nothing of
 // the kind (its attention walks one cache, src/attention.cu:410-494).
 //
-// shared_pieces: a block of 256 threads per (item, key/value head), 32 rows and 64 keys a step in
-// 32-bit FMA; every element type.  shared_join: a warp per row joins its pieces.
+// Here the 32-bit kernel and the joining of pieces; the bfloat16 kernels are in attn_shared_tc.cu.
 #include "api.h"
 #include "attn_shared.h"
 
@@ -12,15 +11,20 @@ namespace cretif {
 
 constexpr int kShRows = 32, kShThreads = 256;
 
-template <typename T>
+// 32-bit pieces: a block of 256 threads per (item, key/value head), 32 rows and 64 keys a step.  A
+// thread has two rows and four keys of the scores, and eight channels of two rows of the output; the
+// next step's keys and values are on their way in registers.  What bounds it at a decode step's sizes is
+// the chain of loads in front of the first product, so a block takes one block of keys where there
+// are few (eight answers at 1,984 tokens: F32_NOW us, F32_BEFORE with loads of one number at a time).
 __global__ void __launch_bounds__(kShThreads)
 shared_pieces_kernel(const SharedArgs a) {
   extern __shared__ __align__(16) float sh_smem[];
-  const int hd = a.hd, ldk = hd + 4;
+  const int hd = a.hd, ldk = hd + 4, quads = hd >> 2;
   float* qs = sh_smem;                        // [32][hd + 4]
   float* ks = qs + kShRows * ldk;             // [64][hd + 4]
   float* vs = ks + kShBlk * ldk;              // [64][hd]
   float* ps = vs + kShBlk * hd;               // [32][65]
+  __shared__ int toks[kShRows];
   const int kvh = blockIdx.y, g = a.nh / a.nkv, tid = threadIdx.x;
   const int tx = tid & 15, ty = tid >> 4;
   dependent_begin();
@@ -36,40 +40,67 @@ shared_pieces_kernel(const SharedArgs a) {
     const SharedOwnItem it = a.own[x / a.own_splits];
     seq = it.seq; row0 = it.row0; n_rows = it.n_rows; tok0 = it.tok0;
     const int prefix = it.prefix;
-    const int end = shared_own_end(a, prefix, a.tok_pos[tok0 + (row0 + n_rows - 1) / g]);
+    const int end = shared_own_end(a, it, a.tok_pos[tok0 + (row0 + n_rows - 1) / g]);
     const int blocks = (end - prefix + kShBlk - 1) / kShBlk;
     key0 = prefix + (int)((long long)blocks * split / a.own_splits) * kShBlk;
     key_end = min(end, prefix + (int)((long long)blocks * (split + 1) / a.own_splits) * kShBlk);
     piece = a.max_pieces - a.own_splits + split;
   }
-  auto token = [&](int r) {
-    return row_base >= 0 ? a.rows[row_base + r / g] : tok0 + r / g;
+  // a thread's share of a step's tile: keys tid / quads, + step, ...; at most 8 of four channels
+  const int slot = a.seq_slot[seq];
+  const int k_of = tid / quads, ch = (tid - k_of * quads) * 4, k_step = kShThreads / quads;
+  const bool loads = k_of < k_step;           // (quads need not divide the threads)
+  float4 kr[8], vr[8];
+  auto fetch = [&](int k0) {
+    const size_t at = ((size_t)shared_block_of(a, slot, k0 / kShBlk) * a.nkv + kvh) * kShBlk * hd;
+    const int n = min(kShBlk, key_end - k0);  // (nothing past the last key is looked at)
+    const float *kp = static_cast<const float*>(a.kc) + at + ch, *vp = static_cast<const float*>(a.vc) + at + ch;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = k_of + i * k_step;
+      kr[i] = vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (loads && k < n) {
+        kr[i] = *reinterpret_cast<const float4*>(kp + (size_t)k * hd);
+        vr[i] = *reinterpret_cast<const float4*>(vp + (size_t)k * hd);
+      }
+    }
   };
-  for (int i = tid; i < kShRows * hd; i += kShThreads) {
-    const int r = i / hd, d = i - r * hd;
-    qs[r * ldk + d] = r < n_rows
-        ? to_float(static_cast<const T*>(a.q)[(size_t)token(row0 + r) * a.ldq +
-                                              (size_t)(kvh * g + (row0 + r) % g) * hd + d])
-        : 0.f;
+  if (key0 < key_end) fetch(key0);
+  if (tid < kShRows) {
+    const int r = row0 + tid;
+    toks[tid] = tid >= n_rows ? -1 : row_base >= 0 ? a.rows[row_base + r / g] : tok0 + r / g;
+  }
+  __syncthreads();
+  for (int i = tid; i < kShRows * quads; i += kShThreads) {
+    const int r = i / quads, d = (i - r * quads) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < n_rows) {
+      const float* src = static_cast<const float*>(a.q) + (size_t)toks[r] * a.ldq + (size_t)(kvh * g + (row0 + r) % g) * hd + d;
+      v = make_float4(src[0], src[1], src[2], src[3]);     // (queries may begin anywhere)
+    }
+    *reinterpret_cast<float4*>(qs + r * ldk + d) = v;
   }
   int pos[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = ty + 16 * i;
-    pos[i] = r < n_rows ? (row_base >= 0 ? key_end - 1 : a.tok_pos[token(row0 + r)]) : -1;
+    pos[i] = r < n_rows ? (row_base >= 0 ? key_end - 1 : a.tok_pos[toks[r]]) : -1;
   }
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   float o[2][2][4] = {};
   for (int k0 = key0; k0 < key_end; k0 += kShBlk) {
     __syncthreads();                          // the last step's readers are done (and Q is there)
-    const size_t at = ((size_t)shared_block(a, seq, k0 / kShBlk) * a.nkv + kvh) * kShBlk * hd;
     const int n = min(kShBlk, key_end - k0);
-    for (int i = tid; i < kShBlk * hd; i += kShThreads) {
-      const int r = i / hd, d = i - r * hd;   // (nothing past the last key is looked at)
-      ks[r * ldk + d] = r < n ? to_float(static_cast<const T*>(a.kc)[at + i]) : 0.f;
-      vs[i] = r < n ? to_float(static_cast<const T*>(a.vc)[at + i]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = k_of + i * k_step;
+      if (loads && k < kShBlk) {
+        *reinterpret_cast<float4*>(ks + k * ldk + ch) = kr[i];
+        *reinterpret_cast<float4*>(vs + k * hd + ch) = vr[i];
+      }
     }
     __syncthreads();
+    if (k0 + kShBlk < key_end) fetch(k0 + kShBlk);
     float s[2][4] = {};
     for (int d = 0; d < hd; d += 4) {
       float4 kk[4];
@@ -113,6 +144,7 @@ shared_pieces_kernel(const SharedArgs a) {
         for (int e = 0; e < 4; ++e) o[i][c][e] *= alpha;
     }
     __syncwarp();                             // a row's probabilities are its own half warp's
+#pragma unroll 4
     for (int k = 0; k < n; ++k) {
       const float p0 = ps[ty * 65 + k], p1 = ps[(ty + 16) * 65 + k];
 #pragma unroll
@@ -132,7 +164,7 @@ shared_pieces_kernel(const SharedArgs a) {
   for (int i = 0; i < 2; ++i) {
     const int r = ty + 16 * i;
     if (r >= n_rows) continue;
-    const size_t row = (size_t)piece * a.T * a.nh + (size_t)token(row0 + r) * a.nh + kvh * g + (row0 + r) % g;
+    const size_t row = ((size_t)piece * a.T + toks[r]) * a.nh + kvh * g + (row0 + r) % g;
     if (tx == 0) a.part_ml[row] = make_float2(m[i], l[i]);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -144,6 +176,8 @@ shared_pieces_kernel(const SharedArgs a) {
   }
 }
 
+// A warp joins the pieces of a row: four lanes' channels of a piece at once, so that 32 / (hd / 4) pieces
+// are read side by side, and eight of those at a time; the parts meet by shuffles.
 template <typename T>
 __global__ void __launch_bounds__(kShThreads) shared_join_kernel(const SharedArgs a) {
   dependent_begin();
@@ -153,27 +187,57 @@ __global__ void __launch_bounds__(kShThreads) shared_join_kernel(const SharedArg
   const size_t stride = (size_t)a.T * a.nh;
   const int own0 = a.max_pieces - a.own_splits, n = pre + a.own_splits;
   auto at = [&](int i) { return (i < pre ? i : own0 + i - pre) * stride + row; };
-  float mx = a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
-  for (int i = lane; i < n; i += 32) mx = fmaxf(mx, a.part_ml[at(i)].x);
-  mx = warp_max(mx);
-  if (mx == -INFINITY) mx = 0.f;              // (a row that sees nothing gives zeros)
-  float den = 0.f;
-  float acc[4] = {};
-  for (int i = 0; i < n; ++i) {
-    const float2 ml = a.part_ml[at(i)];
-    if (ml.x == -INFINITY) continue;          // a piece without keys
-    const float w = exp2f(ml.x - mx);
-    den = fmaf(w, ml.y, den);
+  // `side` groups of `wide` lanes (a power of two, at least hd / 4) take the pieces in turns
+  int wide = 4;
+  while (wide < a.hd >> 2) wide <<= 1;
+  const int side = 32 / wide, mine = lane / wide, ch = (lane & (wide - 1)) * 4;
+  const bool live = ch < a.hd;
+  const float sink = a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
+  float ref = -INFINITY, den = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int kAtOnce = 8;
+  for (int i0 = mine; i0 < n; i0 += side * kAtOnce) {
+    float2 ml[kAtOnce];
+    float4 x[kAtOnce];
+    float top = ref;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (lane + 32 * c < a.hd) acc[c] = fmaf(w, a.part_o[at(i) * a.hd + lane + 32 * c], acc[c]);
+    for (int e = 0; e < kAtOnce; ++e) {
+      const int i = i0 + e * side;
+      ml[e] = i < n ? a.part_ml[at(i)] : make_float2(-INFINITY, 0.f);
+      x[e] = i < n && live ? *reinterpret_cast<const float4*>(a.part_o + at(i) * a.hd + ch) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) top = fmaxf(top, ml[e].x);
+    if (top == -INFINITY) continue;           // pieces without keys
+    const float keep = ref == -INFINITY ? 0.f : exp2f(ref - top);
+    den *= keep; acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) {
+      const float w = ml[e].x == -INFINITY ? 0.f : exp2f(ml[e].x - top);
+      den = fmaf(w, ml[e].y, den);
+      acc.x = fmaf(w, x[e].x, acc.x); acc.y = fmaf(w, x[e].y, acc.y);
+      acc.z = fmaf(w, x[e].z, acc.z); acc.w = fmaf(w, x[e].w, acc.w);
+    }
+    ref = top;
   }
-  if (a.sink) den += exp2f(a.sink[h] * 1.4426950408889634f - mx);
-  const float inv = den > 0.f ? 1.0f / den : 0.f;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + 32 * c < a.hd)
-      static_cast<T*>(a.out)[(size_t)t * a.ldo + (size_t)h * a.hd + lane + 32 * c] = from_float<T>(acc[c] * inv);
+  float top = fmaxf(ref, sink);
+  for (int o = wide; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float w = ref == -INFINITY ? 0.f : exp2f(ref - top);
+  den *= w; acc.x *= w; acc.y *= w; acc.z *= w; acc.w *= w;
+  for (int o = wide; o < 32; o <<= 1) {
+    den += __shfl_xor_sync(0xffffffffu, den, o);
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o);
+    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o);
+    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+  }
+  if (a.sink) den += sink == top ? 1.0f : exp2f(sink - top);
+  if (mine == 0 && live) {
+    const float inv = den > 0.f ? 1.0f / den : 0.f;       // (a row that sees nothing gives zeros)
+    T* dst = static_cast<T*>(a.out) + (size_t)t * a.ldo + (size_t)h * a.hd + ch;
+    dst[0] = from_float<T>(acc.x * inv); dst[1] = from_float<T>(acc.y * inv);
+    dst[2] = from_float<T>(acc.z * inv); dst[3] = from_float<T>(acc.w * inv);
+  }
 }
 
 int launch_shared_bf16(const SharedArgs& a, cudaStream_t st);        // attn_shared_tc.cu
@@ -186,10 +250,10 @@ static int launch_join(const SharedArgs& a, cudaStream_t st) {
 
 static int launch_shared_f32(const SharedArgs& a, cudaStream_t st) {
   const size_t smem = ((size_t)(kShRows + kShBlk) * (a.hd + 4) + (size_t)kShBlk * a.hd + kShRows * 65) * 4;
-  cudaError_t e = cudaFuncSetAttribute(shared_pieces_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(shared_pieces_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)smem);
   if (e != cudaSuccess) return (int)e;
-  launch_dependent(shared_pieces_kernel<float>, dim3(a.n_pre + a.n_own * a.own_splits, a.nkv), dim3(kShThreads),
+  launch_dependent(shared_pieces_kernel, dim3(a.n_pre + a.n_own * a.own_splits, a.nkv), dim3(kShThreads),
                    smem, st, a);
   return launch_join<float>(a, st);
 }
@@ -214,6 +278,7 @@ extern "C" int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int
   if (dt != kF32 && dt != kBF16) return kBadDType;
   if ((((uintptr_t)kc | (uintptr_t)vc | (uintptr_t)plan | (uintptr_t)part_o) & 15) || ((uintptr_t)part_ml & 7))
     return kMisaligned;
+  if (!part_o && (dt == kF32 || n_pre > 0 || own_splits > 1)) return kBadArgument;
   SharedArgs a{};
   a.q = q; a.kc = kc; a.vc = vc; a.out = out; a.ldq = ldq; a.ldo = ldo; a.n_blocks = n_blocks;
   a.table = table; a.table_stride = table_stride; a.n_slots = n_slots;

@@ -27,8 +27,9 @@ struct SharedPrefixItem {
 // Some rows of one sequence over its own keys: row r is head kvh * g + r % g of token tok0 + r / g.
 struct SharedOwnItem {
   int seq, tok0, row0, n_rows;
-  int prefix, pieces;                      // tokens shared, and pieces they are in
-  int pad[2];
+  int prefix, pieces;                      // tokens that are other items' work, and pieces they are in
+  int least;                               // the least position of the sequence: the tokens it shares
+  int pad;
 };
 
 // What every kernel of a call reads.
@@ -69,12 +70,12 @@ __device__ __forceinline__ int shared_block(const SharedArgs& a, int seq, int at
   return shared_block_of(a, a.seq_slot[seq], at);
 }
 
-// One past the last own key that a row at position `last` sees.  A position inside the prefix is a
-// caller's mistake: the fault bit is set and there are none.
-__device__ __forceinline__ int shared_own_end(const SharedArgs& a, int prefix, int last) {
-  if (last >= prefix && last < 0x7fffff00) return last + 1;
+// One past the last own key that an item's row at position `last` sees.  A position inside the shared
+// tokens is a caller's mistake: the fault bit is set and there are none.
+__device__ __forceinline__ int shared_own_end(const SharedArgs& a, const SharedOwnItem& it, int last) {
+  if (last >= it.least && last < 0x7fffff00) return last + 1;
   atomicOr(a.fault, (unsigned)kFaultBlockTable);
-  return prefix;
+  return it.prefix;
 }
 
 }  // namespace cretif

@@ -44,7 +44,7 @@ struct SpSmem {
     ring = n_sub == 1 ? 0 : n_sub * kSpRows * 128;
     bars = ring + pairs * 2 * n_sub * kSpTile;
     xch = bars + (kSpDone + 6 + 4) * 8 + 16;
-    total = xch + kSpRows * 8 + 1024;
+    total = xch + kSpRows * 16 + 1024;
   }
 };
 
@@ -184,7 +184,8 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   uint64_t* q_full = p_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float2* xch = reinterpret_cast<float2*>(smem + L.xch);
+  float2* xch = reinterpret_cast<float2*>(smem + L.xch);  // [128] references and sums, then the rows' places
+  long long* place = reinterpret_cast<long long*>(xch + kSpRows);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const SharedPrefixItem it = a.pre[blockIdx.x];
@@ -301,13 +302,16 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   } else {
     // ---- the queries into tensor memory, or into shared memory
     const int row = threadIdx.x, copy = row / span, r = row - copy * span;
+    size_t at = 0;                                        // the row's place among the pieces
     {
       const bool there = r < it.n_rows;
-      const int rr = it.row0 + r;
+      const int rr = it.row0 + r, of = rr / g, head = kvh * g + rr - of * g;
       const __nv_bfloat16* src = nullptr;
-      if (there)
-        src = static_cast<const __nv_bfloat16*>(a.q) + (size_t)a.rows[it.row_base + rr / g] * a.ldq +
-              (size_t)(kvh * g + rr % g) * hd;
+      if (there) {
+        const int token = a.rows[it.row_base + of];
+        src = static_cast<const __nv_bfloat16*>(a.q) + (size_t)token * a.ldq + (size_t)head * hd;
+        at = ((size_t)it.piece * a.T + token) * a.nh + head;
+      }
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
       if (n_sub == 1) {                                   // two channels a column
         uint32_t all[32];
@@ -338,12 +342,8 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       tc::mbar_wait(&done[(n + 1) % kSpDone], (uint32_t)(((n + 1) / kSpDone) & 1), abort);
       tc::tc_fence_after();
     }
-    auto part_row = [&](int rr) {
-      return (size_t)it.piece * a.T * a.nh + (size_t)a.rows[it.row_base + rr / g] * a.nh + kvh * g + rr % g;
-    };
     if (fold == 1) {
       const bool there = r < it.n_rows;
-      const size_t at = there ? part_row(it.row0 + r) : 0;
       if (there) a.part_ml[at] = make_float2(m, l);
       if (active)
         for (int c0 = 0; c0 < hd; c0 += 32) {
@@ -364,6 +364,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       float* buf = reinterpret_cast<float*>(smem);
       const int ld = hd + 4;
       asm volatile("bar.sync 1, 128;" ::: "memory");      // all rows' products are done
+      if (copy == 0) place[r] = (long long)at;
       if (active) {
         xch[row] = make_float2(m, l);
         for (int c0 = 0; c0 < hd; c0 += 32) {
@@ -379,24 +380,24 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         }
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      const int quads = hd >> 2;
-      for (int i = threadIdx.x; i < it.n_rows * quads; i += kSpRows) {
-        const int rr = i / quads, c = (i - rr * quads) * 4;
-        float mm = -INFINITY;
+      // four channels a thread, `step` rows at once
+      const int quads = hd >> 2, step = kSpRows / quads, mine = threadIdx.x / quads;
+      const int ch = (threadIdx.x - mine * quads) * 4;
+      for (int rr = mine; mine < step && rr < it.n_rows; rr += step) {
+        float mm = -INFINITY, den = 0.f;
         for (int f = 0; f < fold; ++f) mm = fmaxf(mm, xch[f * span + rr].x);
-        float den = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int f = 0; f < fold; ++f) {
           const float2 ml = xch[f * span + rr];
           const float w = ml.x == -INFINITY ? 0.f : sp_exp2(ml.x - mm);
-          const float4 o = *reinterpret_cast<const float4*>(buf + (f * span + rr) * ld + c);
+          const float4 o = *reinterpret_cast<const float4*>(buf + (f * span + rr) * ld + ch);
           den = fmaf(w, ml.y, den);
           acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y);
           acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
         }
-        const size_t at = part_row(it.row0 + rr);
-        if (c == 0) a.part_ml[at] = make_float2(mm, den);
-        *reinterpret_cast<float4*>(a.part_o + at * hd + c) = acc;
+        const size_t to = (size_t)place[rr];
+        if (ch == 0) a.part_ml[to] = make_float2(mm, den);
+        *reinterpret_cast<float4*>(a.part_o + to * hd + ch) = acc;
       }
     }
   }
@@ -420,11 +421,11 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 // enough to fill the chip with warps.
 // With JOIN the item's warps hold all of the rows' own keys and join the rows' prefix pieces (the kernel is
 // launched while the prefix kernel runs and waits for it only then); else they leave pieces.
-constexpr int kSoWarps = 4, kSoThreads = kSoWarps * 32, kSoKeys = 16, kSoStages = 3;
-template <int HDG>
-constexpr int kSoStage = 2 * HDG * kSoKeys * 128;         // bytes: keys, then values
+constexpr int kSoWarps = 4, kSoThreads = kSoWarps * 32, kSoStages = 3;
+template <int HDG, int KEYS>
+constexpr int kSoStage = 2 * HDG * KEYS * 128;            // bytes: keys, then values
 
-template <int HDG, int NR, int WPI, bool JOIN>
+template <int HDG, int NR, int KEYS, int WPI, bool JOIN>
 __global__ void __launch_bounds__(kSoThreads)
 shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ SharedArgs a, int after_prefix) {
@@ -439,7 +440,7 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   const bool none = which >= a.n_own;                     // (a warp of its own: WPI is 1)
   // (the plan is never written by a kernel)
   const SharedOwnItem it = a.own[none ? 0 : which];
-  constexpr int kRing = kSoStages * kSoStage<HDG>;
+  constexpr int kRing = kSoStages * kSoStage<HDG, KEYS>;
   unsigned char* ring = smem + cta_warp * kRing;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kSoWarps * kRing) + cta_warp * kSoStages;
   int* abort_word = reinterpret_cast<int*>(smem + kSoWarps * kRing + kSoWarps * kSoStages * 8) + cta_warp;
@@ -461,14 +462,14 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   const int prefix = it.prefix, blk0 = prefix / kShBlk;
   const int slot = a.seq_slot[it.seq];
   const int last = a.tok_pos[it.tok0 + (it.row0 + it.n_rows - 1) / g];
-  const int end = shared_own_end(a, prefix, last);
-  // 16 keys a warp and step: keys 16 i .. of the own ones, i = first, first + stride, ...
+  const int end = shared_own_end(a, it, last);
+  // KEYS keys a warp and step: keys KEYS i .. of the own ones, i = first, first + stride, ...
   const int first = split * WPI + warp, stride = splits * WPI;
-  const int chunks = (end - prefix + kSoKeys - 1) / kSoKeys;
+  const int chunks = (end - prefix + KEYS - 1) / KEYS;
   const int steps = chunks > first ? (chunks - first + stride - 1) / stride : 0;
   // the physical blocks of 32 steps, a lane each
   auto window = [&](int k0) {
-    return k0 + lane < steps ? shared_block_of(a, slot, blk0 + ((first + (k0 + lane) * stride) >> 2)) : 0;
+    return k0 + lane < steps ? shared_block_of(a, slot, blk0 + (first + (k0 + lane) * stride) / (kShBlk / KEYS)) : 0;
   };
   int blocks = window(0);
   auto fetch = [&](int k) {                               // step k into the ring
@@ -476,13 +477,13 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int blk = __shfl_sync(0xffffffffu, blocks, k & 31);
     if (lane == 0) {
       const int s = k % kSoStages, i = first + k * stride;
-      const int row = (blk * a.nkv + kvh) * kShBlk + (i & 3) * kSoKeys;
-      unsigned char* at = ring + s * kSoStage<HDG>;
-      tc::mbar_expect_tx(&full[s], (uint32_t)kSoStage<HDG>);
+      const int row = (blk * a.nkv + kvh) * kShBlk + i % (kShBlk / KEYS) * KEYS;
+      unsigned char* at = ring + s * kSoStage<HDG, KEYS>;
+      tc::mbar_expect_tx(&full[s], (uint32_t)kSoStage<HDG, KEYS>);
 #pragma unroll
       for (int sub = 0; sub < HDG; ++sub) {
-        tc::tma_load_2d(at + sub * kSoKeys * 128, &map_k, 64 * sub, row, &full[s]);
-        tc::tma_load_2d(at + (HDG + sub) * kSoKeys * 128, &map_v, 64 * sub, row, &full[s]);
+        tc::tma_load_2d(at + sub * KEYS * 128, &map_k, 64 * sub, row, &full[s]);
+        tc::tma_load_2d(at + (HDG + sub) * KEYS * 128, &map_v, 64 * sub, row, &full[s]);
       }
     }
   };
@@ -517,31 +518,35 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   bool ok = true;
   for (int k = 0, s = 0, turn = 0; k < steps; ++k) {
     if (!tc::mbar_wait(&full[s], (uint32_t)(turn & 1), abort)) { ok = false; break; }
-    const int key0 = prefix + (first + k * stride) * kSoKeys, n = end - key0;
-    const uint32_t kbase = tc::smem_u32(ring + s * kSoStage<HDG>), vbase = kbase + HDG * kSoKeys * 128;
-    float sc[2][4];
+    const int key0 = prefix + (first + k * stride) * KEYS, n = end - key0;
+    const uint32_t kbase = tc::smem_u32(ring + s * kSoStage<HDG, KEYS>), vbase = kbase + HDG * KEYS * 128;
+    constexpr int X = KEYS / 16;
+    float sc[2 * X][4];
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < 2 * X; ++x)
 #pragma unroll
       for (int e = 0; e < 4; ++e) sc[x][e] = 0.f;
 #pragma unroll
     for (int d = 0; d < HDG * 4; ++d) {
       if (16 * d < hd) {
-        const int key = (mat >> 1) * 8 + rin, chunk = 2 * d + (mat & 1);
-        uint32_t kb[4];
-        ldmatrix_x4(kb, kbase + (chunk >> 3) * (kSoKeys * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
-        mma_16816_f32(sc[0], qa[d][0][0], NR == 2 ? qa[d][NR - 1][0] : 0u, qa[d][0][1], NR == 2 ? qa[d][NR - 1][1] : 0u,
-                      kb[0], kb[1]);
-        mma_16816_f32(sc[1], qa[d][0][0], NR == 2 ? qa[d][NR - 1][0] : 0u, qa[d][0][1], NR == 2 ? qa[d][NR - 1][1] : 0u,
-                      kb[2], kb[3]);
+#pragma unroll
+        for (int x = 0; x < X; ++x) {
+          const int key = 16 * x + (mat >> 1) * 8 + rin, chunk = 2 * d + (mat & 1);
+          uint32_t kb[4];
+          ldmatrix_x4(kb, kbase + (chunk >> 3) * (KEYS * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            mma_16816_f32(sc[2 * x + y], qa[d][0][0], NR == 2 ? qa[d][NR - 1][0] : 0u, qa[d][0][1],
+                          NR == 2 ? qa[d][NR - 1][1] : 0u, kb[2 * y], kb[2 * y + 1]);
+        }
       }
     }
-    uint32_t pa[4] = {0u, 0u, 0u, 0u};
+    uint32_t pa[X][4];
 #pragma unroll
     for (int w = 0; w < NR; ++w) {                        // rows r, r + 8
-      float t4[4], mx = -INFINITY;
+      float t4[4 * X], mx = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 4 * X; ++e) {
         const int key = key0 + 8 * (e >> 1) + 2 * c + (e & 1);
         t4[e] = key <= pos[w] ? sc[e >> 1][2 * w + (e & 1)] * a.scale_log2 : -INFINITY;
         mx = fmaxf(mx, t4[e]);
@@ -550,37 +555,45 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float m_new = fmaxf(m[w], mx);
       const float alpha = m[w] == -INFINITY ? 0.f : sp_exp2(m[w] - m_new);
-      float p[4], sum = 0.f;
+      float p[4 * X], sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 4 * X; ++e) {
         p[e] = t4[e] == -INFINITY ? 0.f : sp_exp2(t4[e] - m_new);
         sum += p[e];
       }
       l[w] = l[w] * alpha + sum;
       m[w] = m_new;
-      pa[w] = pack_bf16(p[0], p[1]);
-      pa[2 + w] = pack_bf16(p[2], p[3]);
+#pragma unroll
+      for (int x = 0; x < X; ++x) {
+        pa[x][w] = pack_bf16(p[4 * x], p[4 * x + 1]);
+        pa[x][2 + w] = pack_bf16(p[4 * x + 2], p[4 * x + 3]);
+        if (NR == 1) pa[x][1] = pa[x][3] = 0u;
+      }
 #pragma unroll
       for (int t = 0; t < HDG * 8; ++t) { o[t][2 * w] *= alpha; o[t][2 * w + 1] *= alpha; }
     }
     // values past the last key count for nothing, whatever they are
-    const bool whole = n >= kSoKeys;
-    const uint32_t keep0 = (2 * c < n ? 0xffffu : 0u) | (2 * c + 1 < n ? 0xffff0000u : 0u);
-    const uint32_t keep1 = (2 * c + 8 < n ? 0xffffu : 0u) | (2 * c + 9 < n ? 0xffff0000u : 0u);
+    const bool whole = n >= KEYS;
 #pragma unroll
-    for (int d = 0; d < HDG * 4; ++d) {
-      if (16 * d < hd) {
-        const int key = (mat & 1) * 8 + rin, chunk = 2 * d + (mat >> 1);
-        uint32_t vb[4];
-        ldmatrix_x4_trans(vb, vbase + (chunk >> 3) * (kSoKeys * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
-        if (!whole) { vb[0] &= keep0; vb[1] &= keep1; vb[2] &= keep0; vb[3] &= keep1; }
+    for (int x = 0; x < X; ++x) {
+      const int at = 16 * x + 2 * c;
+      const uint32_t keep0 = (at < n ? 0xffffu : 0u) | (at + 1 < n ? 0xffff0000u : 0u);
+      const uint32_t keep1 = (at + 8 < n ? 0xffffu : 0u) | (at + 9 < n ? 0xffff0000u : 0u);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float* to = o[2 * d + x];
-          float acc[4] = {to[0], to[1], NR == 2 ? to[2 * NR - 2] : 0.f, NR == 2 ? to[2 * NR - 1] : 0.f};
-          mma_16816_f32(acc, pa[0], pa[1], pa[2], pa[3], vb[2 * x], vb[2 * x + 1]);
+      for (int d = 0; d < HDG * 4; ++d) {
+        if (16 * d < hd) {
+          const int key = 16 * x + (mat & 1) * 8 + rin, chunk = 2 * d + (mat >> 1);
+          uint32_t vb[4];
+          ldmatrix_x4_trans(vb, vbase + (chunk >> 3) * (KEYS * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+          if (!whole) { vb[0] &= keep0; vb[1] &= keep1; vb[2] &= keep0; vb[3] &= keep1; }
 #pragma unroll
-          for (int e = 0; e < 2 * NR; ++e) to[e] = acc[e];
+          for (int y = 0; y < 2; ++y) {
+            float* to = o[2 * d + y];
+            float acc[4] = {to[0], to[1], NR == 2 ? to[2 * NR - 2] : 0.f, NR == 2 ? to[2 * NR - 1] : 0.f};
+            mma_16816_f32(acc, pa[x][0], pa[x][1], pa[x][2], pa[x][3], vb[2 * y], vb[2 * y + 1]);
+#pragma unroll
+            for (int e = 0; e < 2 * NR; ++e) to[e] = acc[e];
+          }
         }
       }
     }
@@ -683,10 +696,19 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   }
 }
 
+constexpr int kShDevices = 64;
+
 template <typename... Params, typename... Args>
-static int sp_launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args&&... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+static int sp_launch(unsigned* limit, void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args&&... args) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
+  // (the limit is asked for once a device and kernel: `limit` says up to what)
+  if (dev >= kShDevices || smem > limit[dev < kShDevices ? dev : 0]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < kShDevices) limit[dev] = (unsigned)smem;
+  }
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = dependent_launch_enabled();
@@ -701,17 +723,30 @@ static int sp_launch(void (*kernel)(Params...), dim3 grid, int threads, size_t s
   return e == cudaSuccess ? launch_status() : (int)e;
 }
 
+// How an item's keys are cut, by how many warps the launch keeps busy.
+enum SoCut { kSoWide, kSoNarrow, kSoWarp };               // 32 keys, 16 keys, a warp an item
+
+template <int HDG, int NR, int KEYS, int WPI, bool JOIN>
+static int launch_own_as(const SharedArgs& a, cudaStream_t st) {
+  constexpr size_t smem = (size_t)kSoWarps * kSoStages * (kSoStage<HDG, KEYS> + 8) + kSoWarps * 4 + 1024;
+  static unsigned limit[kShDevices];
+  CUtensorMap mk, mv;
+  const int rows = (int)(a.n_blocks * a.nkv * kShBlk);
+  if (make_tile_map_bf16(&mk, a.kc, rows, a.hd, a.hd, KEYS) || make_tile_map_bf16(&mv, a.vc, rows, a.hd, a.hd, KEYS))
+    return kBadArgument;
+  const int ctas = JOIN ? (a.n_own * WPI + kSoWarps - 1) / kSoWarps : a.n_own * a.own_splits;
+  return sp_launch(limit, shared_own_mma_kernel<HDG, NR, KEYS, WPI, JOIN>, dim3(ctas, a.nkv), kSoThreads, smem, st, mk,
+                   mv, a, (int)(a.n_pre > 0));
+}
+
 template <int HDG, int NR>
-static int launch_own(const CUtensorMap& mk, const CUtensorMap& mv, const SharedArgs& a, cudaStream_t st) {
-  constexpr size_t smem = (size_t)kSoWarps * kSoStages * (kSoStage<HDG> + 8) + kSoWarps * 4 + 1024;
-  const int after = a.n_pre > 0;
-  if (a.own_splits > 1)
-    return sp_launch(shared_own_mma_kernel<HDG, NR, 4, false>, dim3(a.n_own * a.own_splits, a.nkv), kSoThreads, smem, st,
-                     mk, mv, a, after);
-  if ((long long)a.n_own * a.nkv > 8 * kSmCount)
-    return sp_launch(shared_own_mma_kernel<HDG, NR, 1, true>, dim3((a.n_own + 3) / 4, a.nkv), kSoThreads, smem, st, mk,
-                     mv, a, after);
-  return sp_launch(shared_own_mma_kernel<HDG, NR, 4, true>, dim3(a.n_own, a.nkv), kSoThreads, smem, st, mk, mv, a, after);
+static int launch_own(const SharedArgs& a, cudaStream_t st) {
+  const long long items = (long long)a.n_own * a.nkv;
+  if (a.own_splits > 1) return launch_own_as<HDG, NR, 32, 4, false>(a, st);
+  const SoCut cut = items > 8 * kSmCount ? kSoWarp : items > (HDG == 1 ? 2 : 1) * kSmCount ? kSoNarrow : kSoWide;
+  if (cut == kSoWarp) return launch_own_as<HDG, NR, 16, 1, true>(a, st);
+  if (cut == kSoNarrow) return launch_own_as<HDG, NR, 16, 4, true>(a, st);
+  return launch_own_as<HDG, NR, 32, 4, true>(a, st);
 }
 
 // The prefix pieces and the own keys; joins the rows where the own keys are in one piece.
@@ -719,20 +754,18 @@ int launch_shared_bf16(const SharedArgs& a, cudaStream_t st) {
   if (((uintptr_t)a.q & 15) || a.ldq % 8 || ((uintptr_t)a.out & 7) || a.ldo % 4) return kMisaligned;
   const long long cache_rows = a.n_blocks * a.nkv * kShBlk;
   if (cache_rows > 0x7fffffffLL) return kBadArgument;
-  CUtensorMap mk, mv;
   if (a.n_pre > 0) {
+    CUtensorMap mk, mv;
     if (make_tile_map_bf16(&mk, a.kc, (int)cache_rows, a.hd, a.hd, kShBlk) ||
         make_tile_map_bf16(&mv, a.vc, (int)cache_rows, a.hd, a.hd, kShBlk))
       return kBadArgument;
     const SpSmem L((a.hd + 63) / 64);
-    const int e = sp_launch(shared_prefix_tc_kernel, dim3(a.n_pre, a.nkv), kSpThreads, L.total, st, mk, mv, a);
+    static unsigned limit[kShDevices];
+    const int e = sp_launch(limit, shared_prefix_tc_kernel, dim3(a.n_pre, a.nkv), kSpThreads, L.total, st, mk, mv, a);
     if (e) return e;
   }
-  if (make_tile_map_bf16(&mk, a.kc, (int)cache_rows, a.hd, a.hd, kSoKeys) ||
-      make_tile_map_bf16(&mv, a.vc, (int)cache_rows, a.hd, a.hd, kSoKeys))
-    return kBadArgument;
-  if (a.own_rows <= 8) return a.hd <= 64 ? launch_own<1, 1>(mk, mv, a, st) : launch_own<2, 1>(mk, mv, a, st);
-  return a.hd <= 64 ? launch_own<1, 2>(mk, mv, a, st) : launch_own<2, 2>(mk, mv, a, st);
+  if (a.own_rows <= 8) return a.hd <= 64 ? launch_own<1, 1>(a, st) : launch_own<2, 1>(a, st);
+  return a.hd <= 64 ? launch_own<1, 2>(a, st) : launch_own<2, 2>(a, st);
 }
 
 }  // namespace cretif

@@ -8,6 +8,7 @@ library, or with a tensor that is not on a CUDA device, the call fails.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -36,6 +37,10 @@ def lib():
         L.cretif_uniform01.restype = ctypes.c_float
         L.cretif_delta_chunk_row.restype = ctypes.c_longlong
         L.cretif_verify_scratch.restype = ctypes.c_longlong
+        # (with the types named, plain integers go through: half the time of wrapping each)
+        p, i, ll, f, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_double
+        L.cretif_attn_shared.argtypes = [p, i, i, p, i, p, p, ll, p, i, i, p, p, p] + [i] * 11 + [f, p, p, p, p, p]
+        L.cretif_verify_drafts.argtypes = [p, i, i, p, p, i, i, p, ll, ll, p, i, p, i, i, d, i, p, p, i, p, p, p]
         L.cretif_uniform01.argtypes = [ctypes.c_ulonglong, ctypes.c_longlong, ctypes.c_int]
         _lib = L
     return _lib
@@ -94,6 +99,16 @@ def _stream():
     if _raw_stream is not None:
         return ctypes.c_void_p(_raw_stream(torch.cuda.current_device()))
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _stream_of(device: int) -> int:
+    """The current stream of a device, by its index, as an address."""
+    if _raw_stream is not None:
+        return _raw_stream(device)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, dim=None) -> None:
@@ -1540,53 +1555,84 @@ def verify_drafts(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens, t
     entries are infinite is uniform over them.  A draft outside the vocabulary does not stand, a
     sequence without rows or with more than K drafts gives no token (-1); both set the token bit of
     ``fault``."""
+    if fault is None:
+        fault = fault_word(logits.device)
+    f32, i32 = torch.float32, torch.int32
+    dev = logits.get_device()
+    # one look at everything that has to hold; what does not is named by the slow way
+    if not (logits.dtype == accept_u.dtype == next_u.dtype == f32
+            and cu_rows.dtype == drafts.dtype == accepted.dtype == tokens.dtype == fault.dtype == i32
+            and dev >= 0 and cu_rows.get_device() == drafts.get_device() == accept_u.get_device()
+            == next_u.get_device() == accepted.get_device() == tokens.get_device() == fault.get_device() == dev
+            == _current_device()
+            and logits.dim() == drafts.dim() == accept_u.dim() == tokens.dim() == 2
+            and cu_rows.dim() == next_u.dim() == accepted.dim() == 1):
+        _verify_refused(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens, temperature, top_k, draft_logits,
+                        fault)
+    (R, V), (B, K), ll, dl, ul, tl = (logits.shape, drafts.shape, logits.stride(), drafts.stride(), accept_u.stride(),
+                                      tokens.stride())
+    ql = (0, 0, 1) if draft_logits is None else draft_logits.stride()
+    if not (cu_rows.numel() == B + 1 and accept_u.shape == (B, K) and next_u.numel() == accepted.numel() == B
+            and tokens.shape == (B, K + 1) and V >= 1 and ll[1] == 1
+            and cu_rows.is_contiguous() and next_u.is_contiguous() and accepted.is_contiguous()
+            and (K == 0 or (dl[1] == ul[1] == tl[1] == 1)) and (B < 2 or tl[0] > K)
+            and temperature == temperature and top_k >= 0
+            and (temperature <= 0 or top_k <= 1024 or top_k >= V) and (R or not B)
+            and (draft_logits is None or (
+                draft_logits.dtype == f32 and draft_logits.get_device() == dev and draft_logits.shape == (B, K, V)
+                and (V == 1 or ql[2] == 1)))):
+        _verify_refused(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens, temperature, top_k, draft_logits,
+                        fault)
+    if not B:
+        return
+    q = ld_seq = ld_place = 0
+    if draft_logits is not None and temperature > 0 and K:   # (a greedy draft is judged by the arg max alone)
+        q, ld_seq, ld_place = draft_logits.data_ptr(), ql[0], ql[1]
+    scratch = torch.empty(_verify_scratch(R, B, K, V, top_k if temperature > 0 else 0, q != 0), dtype=torch.float64,
+                          device=logits.device)
+    _check((_lib or lib()).cretif_verify_drafts(
+        logits.data_ptr(), ll[0], R, cu_rows.data_ptr(), drafts.data_ptr(), dl[0], K, q, ld_seq, ld_place,
+        accept_u.data_ptr(), ul[0], next_u.data_ptr(), B, V, temperature, top_k, accepted.data_ptr(), tokens.data_ptr(),
+        tl[0], scratch.data_ptr(), fault.data_ptr(), _stream_of(dev)), "verify_drafts", 2)
+
+
+@functools.lru_cache(maxsize=256)
+def _verify_scratch(R: int, B: int, K: int, V: int, top_k: int, proposed: bool) -> int:
+    """The scratch of a verification, in numbers of eight bytes."""
+    L = lib()
+    size = L.cretif_verify_scratch(R, B, K, V, top_k, int(proposed))
+    return -(-int(size) // 8)
+
+
+def _verify_refused(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens, temperature, top_k, draft_logits,
+                    fault) -> None:
+    """What :func:`verify_drafts` does not take in these arguments."""
     _need(logits, "logits", torch.float32, 2); _need(cu_rows, "cu_rows", torch.int32, 1)
     _need(drafts, "drafts", torch.int32, 2); _need(accept_u, "accept_u", torch.float32, 2)
     _need(next_u, "next_u", torch.float32, 1); _need(accepted, "accepted", torch.int32, 1)
-    _need(tokens, "tokens", torch.int32, 2)
+    _need(tokens, "tokens", torch.int32, 2); _need(fault, "fault", torch.int32)
+    if draft_logits is not None:
+        _need(draft_logits, "draft_logits", torch.float32, 3)
     R, V = logits.shape
     B, K = drafts.shape
-    dev = logits.device
-    if fault is None:
-        fault = fault_word(dev)
-    _need(fault, "fault", torch.int32)
-    if any(t.device != dev for t in (cu_rows, drafts, accept_u, next_u, accepted, tokens, fault)) \
-            or dev.index != torch.cuda.current_device():
+    dev = logits.get_device()
+    if any(t.get_device() != dev for t in (cu_rows, drafts, accept_u, next_u, accepted, tokens, fault)
+           + (() if draft_logits is None else (draft_logits,))) or dev != _current_device():
         raise KernelError("verify_drafts: all tensors must be on the current device")
     if cu_rows.shape[0] != B + 1 or tuple(accept_u.shape) != (B, K) or next_u.shape[0] != B \
             or accepted.shape[0] != B or tuple(tokens.shape) != (B, K + 1) or V < 1:
         raise KernelError(f"verify_drafts: for {B} sequences of up to {K} drafts cu_rows is [{B + 1}], "
                           f"accept_u [{B}, {K}], next_u and accepted [{B}], tokens [{B}, {K + 1}]")
-    if not (cu_rows.is_contiguous() and next_u.is_contiguous() and accepted.is_contiguous()) \
-            or (K > 0 and (drafts.stride(1) != 1 or accept_u.stride(1) != 1)) \
-            or (K > 0 and tokens.stride(1) != 1):
-        raise KernelError("verify_drafts: rows must be dense")
     if not temperature == temperature:
         raise KernelError("verify_drafts: the temperature is NaN")
-    if top_k < 0 or (temperature > 0 and 0 < top_k < V and top_k > lib().cretif_max_top_k()):
-        raise KernelError(f"verify_drafts: top_k {top_k} is below zero or exceeds the kernel's limit "
-                          f"{lib().cretif_max_top_k()}")
-    ld_seq = ld_place = V
-    if draft_logits is not None:
-        _need(draft_logits, "draft_logits", torch.float32, 3)
-        if tuple(draft_logits.shape) != (B, K, V) or (V > 1 and draft_logits.stride(2) != 1) \
-                or draft_logits.device != dev:
-            raise KernelError(f"verify_drafts: draft_logits must be [{B}, {K}, {V}] with dense rows")
-        ld_seq, ld_place = draft_logits.stride(0), draft_logits.stride(1)
-        if temperature <= 0 or K == 0:
-            draft_logits = None                # (a greedy draft is judged by the arg max alone)
-    if not B:
-        return
-    if not R:
+    if top_k < 0 or (temperature > 0 and 1024 < top_k < V):
+        raise KernelError(f"verify_drafts: top_k {top_k} is below zero or exceeds the kernel's limit 1024")
+    if draft_logits is not None and (tuple(draft_logits.shape) != (B, K, V)
+                                     or (V > 1 and draft_logits.stride(2) != 1)):
+        raise KernelError(f"verify_drafts: draft_logits must be [{B}, {K}, {V}] with dense rows")
+    if B and not R:
         raise KernelError("verify_drafts: every sequence has one row of logits at least")
-    scratch = torch.empty(lib().cretif_verify_scratch(R, B, K, V, int(top_k) if temperature > 0 else 0,
-                                                      int(draft_logits is not None)),
-                          dtype=torch.uint8, device=dev)
-    _check(lib().cretif_verify_drafts(
-        _p(logits), _rows(logits, "logits"), R, _p(cu_rows), _p(drafts), max(K, drafts.stride(0)), K,
-        _p(draft_logits), ctypes.c_longlong(ld_seq), ctypes.c_longlong(max(V, ld_place)), _p(accept_u),
-        accept_u.stride(0), _p(next_u), B, V, ctypes.c_double(temperature), int(top_k), _p(accepted),
-        _p(tokens), max(K + 1, tokens.stride(0)), _p(scratch), _p(fault), _stream()), "verify_drafts", 2)
+    raise KernelError("verify_drafts: rows must be dense")
 
 
 def uniform01(seed: int, request: int, draw: int) -> float:
@@ -1822,8 +1868,7 @@ class SharedPrefixPlan:
     share, not on slots, positions or values.  One plan serves every layer, and every later step of
     the same make-up."""
 
-    __slots__ = ("data", "n_pre", "n_own", "own_rows", "own_splits", "max_pieces", "n_rows", "B", "T", "nh", "nkv",
-                 "hd", "dtype", "prefix_blocks", "device")
+    __slots__ = ("data", "device", "sizes", "launch", "pieces", "kernels", "prefix_blocks", "T", "B")
 
 
 def _blocks_an_item(tiles, ctas: int, begin: int = 4) -> int:
@@ -1841,9 +1886,11 @@ def _blocks_an_item(tiles, ctas: int, begin: int = 4) -> int:
     return best[1]
 
 
-def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_rows: int, ctas: int):
+def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_rows: int, ctas: int,
+                  walk: bool = False):
     """The host side of a plan: (prefix items, own items, splits of the own keys, most pieces, tokens
-    of the groups, pieces of a token, prefix of a sequence), lists of integers."""
+    of the groups, pieces of a token, prefix of a sequence), lists of integers.  ``walk``: the shared
+    tokens are read by every sequence beside its own."""
     if nh <= 0 or nkv <= 0 or nh % nkv:
         raise KernelError(f"shared prefix: {nh} heads cannot share {nkv} key/value heads")
     news, starts = [int(n) for n in news], [int(n) for n in starts]
@@ -1870,7 +1917,7 @@ def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_r
                                   f"group shares {prefix}")
             seen.add(b)
             prefix_of[b] = prefix
-        if prefix and members:
+        if prefix and members and not walk:
             toks = [t for b in members for t in range(cu[b], cu[b + 1])]
             grouped.append((prefix // 64, len(rows), toks, members[0]))
             rows += toks
@@ -1887,12 +1934,23 @@ def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_r
             for row0 in range(0, n_rows, tile_rows):
                 pre += [base, row0, min(tile_rows, n_rows - row0), member, blk0, blk1, piece, 0]
     own = []
-    for b in range(B):
+    # (the longest first: what starts last is then short)
+    apart = [0] * B if walk else prefix_of
+    for b in sorted(range(B), key=lambda b: apart[b] - starts[b] - news[b]):
         for row0 in range(0, news[b] * g, own_rows):
-            own += [b, cu[b], row0, min(own_rows, news[b] * g - row0), prefix_of[b], tok_pieces[cu[b]], 0, 0]
-    own_blocks = max(-(-(starts[b] + news[b] - prefix_of[b]) // 64) for b in range(B))
+            own += [b, cu[b], row0, min(own_rows, news[b] * g - row0), apart[b], tok_pieces[cu[b]],
+                    prefix_of[b], 0]
+    own_blocks = max(-(-(starts[b] + news[b] - apart[b]) // 64) for b in range(B))
     splits = max(1, min(own_blocks // 8, ctas // max(1, len(own) // 8 * nkv), 8))
     return pre, own, splits, max(tok_pieces) + splits, rows, tok_pieces, prefix_of
+
+
+# A short prefix is walked by every sequence beside its own keys, in one launch instead of two (bfloat16).
+# Shared against walked, us: 9 heads on 3, 8 sequences, 128 tokens 7.1 / 4.4, 256 7.2 / 5.5, 512 7.2 / 7.8;
+# 32 heads on 32, 8 sequences, 256 tokens (17 MB read) 9.0 / 6.3, 512 (34 MB) 9.2 / 8.8, 32 sequences, 128 tokens
+# (34 MB) 13.7 / 12.4, 256 (67 MB) 15.1 / 16.5; heads of 128, 16 on 2, 128 sequences, 256 tokens (34 MB) 17.2 / 12.4.
+WALKED_TOKENS = 256
+WALKED_BYTES = 40 << 20
 
 
 def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, device) -> SharedPrefixPlan:
@@ -1907,18 +1965,25 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
         raise KernelError(f"shared prefix: head_dim {hd} is not a multiple of 16 up to 128")
     dev = torch.device(device)
     ctas = 2 * (sm_count(dev) if dev.type == "cuda" else 148)
+    groups, walk = [(list(m), int(p)) for m, p in groups], False
+    if dtype == torch.bfloat16 and all(p <= WALKED_TOKENS for _, p in groups) and sum(
+            p * len(m) for m, p in groups) * nkv * hd * 4 <= WALKED_BYTES:
+        walk = True
     tile_rows, own_rows = (128, 16) if dtype == torch.bfloat16 else (32, 32)
     if dtype == torch.bfloat16 and nkv > 0 and max(news, default=1) * nh // nkv <= 8:
         own_rows = 8
     pre, own, splits, pieces, rows, tok_pieces, prefix_of = _shared_items(groups, news, starts, nh, nkv, tile_rows,
-                                                                          own_rows, ctas)
+                                                                          own_rows, ctas, walk)
     plan = SharedPrefixPlan()
     packed = torch.tensor(pre + own + rows + tok_pieces, dtype=torch.int32)
     plan.data = packed.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else packed
-    plan.n_pre, plan.n_own, plan.own_rows = len(pre) // 8, len(own) // 8, own_rows
-    plan.own_splits, plan.max_pieces = splits, pieces
-    plan.n_rows, plan.B, plan.T = len(rows), len(prefix_of), len(tok_pieces)
-    plan.nh, plan.nkv, plan.hd, plan.dtype, plan.device = nh, nkv, hd, dtype, plan.data.device
+    plan.device, plan.T, plan.B = plan.data.device, len(tok_pieces), len(prefix_of)
+    plan.sizes = (nh, nkv, hd, plan.T, plan.B, dtype, plan.data.get_device())
+    # as the C entry takes them: items, splits, pieces, tokens of the groups, T, heads, head size
+    plan.launch = (len(pre) // 8, len(own) // 8, own_rows, splits, pieces, len(rows), plan.T, nh, nkv, hd)
+    whole = dtype == torch.bfloat16 and splits == 1      # the own keys' kernel joins, and leaves no piece
+    plan.pieces = pieces - 1 if whole else pieces
+    plan.kernels = (1 if whole else 2) + (1 if pre and dtype == torch.bfloat16 else 0)
     plan.prefix_blocks = max(prefix_of) // 64
     return plan
 
@@ -1933,18 +1998,56 @@ def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: Shar
     joins head h's softmax denominator.  bfloat16 or float32, head sizes in multiples of 16 up to 128,
     any number of query heads on a key/value head.  A table entry that names no block, or a position
     inside the shared tokens, sets the block-table bit of ``fault``."""
-    nh, nkv, hd, T, B = plan.nh, plan.nkv, plan.hd, plan.T, plan.B
-    _need(q, "q", plan.dtype, 2); _need(out, "out", plan.dtype, 2)
-    _need(kc, "k cache", plan.dtype, 4); _need(vc, "v cache", plan.dtype, 4)
+    nh, nkv, hd, T, B, dt, dev = plan.sizes
+    i32 = torch.int32
+    # one look at everything that has to hold; what does not is named by the slow way
+    qs, os, ks, ts, ql, ol, tl = q.shape, out.shape, kc.shape, table.shape, q.stride(), out.stride(), table.stride()
+    if not (q.dtype == out.dtype == kc.dtype == vc.dtype == dt
+            and table.dtype == tok_pos.dtype == cu_seqlens.dtype == seq_slot.dtype == fault.dtype == i32
+            and dev >= 0 and q.get_device() == out.get_device() == kc.get_device() == vc.get_device() == dev
+            and table.get_device() == tok_pos.get_device() == cu_seqlens.get_device() == seq_slot.get_device()
+            == fault.get_device() == dev == _current_device()
+            and len(qs) == len(os) == len(ts) == 2 and tok_pos.dim() == cu_seqlens.dim() == seq_slot.dim() == 1
+            and qs[0] >= T and os[0] >= T and qs[1] >= nh * hd and os[1] >= nh * hd
+            and ql[1] == ol[1] == tl[1] == 1 and (T < 2 or ol[0] >= nh * hd)
+            and tok_pos.numel() >= T and cu_seqlens.numel() > B and seq_slot.numel() >= B
+            and tok_pos.is_contiguous() and cu_seqlens.is_contiguous() and seq_slot.is_contiguous()
+            and ks == vc.shape and ks[1:] == (nkv, 64, hd) and block_tokens == 64
+            and kc.is_contiguous() and vc.is_contiguous() and ts[1] >= plan.prefix_blocks and scale > 0
+            and (sink is None or (sink.dtype == torch.float32 and tuple(sink.shape) == (nh,)
+                                  and sink.is_contiguous() and sink.get_device() == dev))):
+        _attn_shared_refused(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan, scale, block_tokens, fault,
+                             sink)
+    part_o = part_ml = 0
+    if plan.pieces:
+        n = plan.pieces * T * nh
+        scratch = torch.empty(n * (hd + 2), dtype=torch.float32, device=plan.device)
+        part_o = scratch.data_ptr()
+        part_ml = part_o + 4 * n * hd
+    _check((_lib or lib()).cretif_attn_shared(
+        q.data_ptr(), ql[0], _DT[dt], out.data_ptr(), ol[0], kc.data_ptr(), vc.data_ptr(), ks[0],
+        table.data_ptr(), tl[0], ts[0], tok_pos.data_ptr(), seq_slot.data_ptr(),
+        plan.data.data_ptr(), *plan.launch, block_tokens, scale, 0 if sink is None else sink.data_ptr(), part_o, part_ml,
+        fault.data_ptr(), _stream_of(dev)), "attn_shared", plan.kernels)
+
+
+def _attn_shared_refused(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan, scale, block_tokens, fault,
+                         sink) -> None:
+    """What :func:`attn_shared` does not take in these arguments."""
+    nh, nkv, hd, T, B, dt, dev = plan.sizes
+    _need(q, "q", dt, 2); _need(out, "out", dt, 2)
+    _need(kc, "k cache", dt, 4); _need(vc, "v cache", dt, 4)
     _need(table, "table", torch.int32, 2); _need(tok_pos, "tok_pos", torch.int32, 1)
     _need(cu_seqlens, "cu_seqlens", torch.int32, 1); _need(seq_slot, "seq_slot", torch.int32, 1)
     _need(fault, "fault", torch.int32)
-    dev = plan.device
-    if not (dev == q.device == out.device == kc.device == vc.device == table.device == tok_pos.device
-            == cu_seqlens.device == seq_slot.device == fault.device) or dev.index != torch.cuda.current_device():
+    if sink is not None:
+        _need(sink, "sink", torch.float32, 1)
+    if any(t.get_device() != dev for t in (q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, fault)
+           + (() if sink is None else (sink,))) or dev != _current_device():
         raise KernelError("attn_shared: the plan and all tensors must be on the current device")
     if q.shape[0] < T or out.shape[0] < T or q.shape[1] < nh * hd or out.shape[1] < nh * hd:
         raise KernelError(f"attn_shared: q and out must have at least {T} rows of {nh * hd}")
+    _rows(q, "q"); _rows(out, "out"); _rows(table, "table")
     if tok_pos.shape[0] < T or cu_seqlens.shape[0] < B + 1 or seq_slot.shape[0] < B \
             or not (tok_pos.is_contiguous() and cu_seqlens.is_contiguous() and seq_slot.is_contiguous()):
         raise KernelError("attn_shared: a position per token, a slot per sequence and their offsets")
@@ -1954,21 +2057,11 @@ def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: Shar
                           f"{tuple(kc.shape)} with blocks of {block_tokens}")
     if table.shape[1] < plan.prefix_blocks:
         raise KernelError("attn_shared: the table is shorter than the shared prefix")
-    if sink is not None:
-        _need(sink, "sink", torch.float32, 1)
-        if sink.shape[0] != nh or not sink.is_contiguous() or sink.device != dev:
-            raise KernelError("attn_shared: the sink has one number per query head")
+    if sink is not None and (sink.shape[0] != nh or not sink.is_contiguous()):
+        raise KernelError("attn_shared: the sink has one number per query head")
     if not scale > 0:
         raise KernelError("attn_shared: the scale must be above zero")
-    scratch = torch.empty(plan.max_pieces * T * nh * (hd + 2), dtype=torch.float32, device=dev)
-    part_o = scratch.data_ptr()
-    _check(lib().cretif_attn_shared(
-        _p(q), _rows(q, "q"), _DT[plan.dtype], _p(out), _rows(out, "out"), _p(kc), _p(vc),
-        ctypes.c_longlong(kc.shape[0]), _p(table), _rows(table, "table"), table.shape[0], _p(tok_pos),
-        _p(seq_slot), _p(plan.data), plan.n_pre, plan.n_own, plan.own_rows, plan.own_splits,
-        plan.max_pieces, plan.n_rows, T, nh, nkv, hd, block_tokens, ctypes.c_float(scale), _p(sink),
-        ctypes.c_void_p(part_o), ctypes.c_void_p(part_o + 4 * plan.max_pieces * T * nh * hd), _p(fault),
-        _stream()), "attn_shared", 2)
+    raise KernelError("attn_shared: the rows of out lie over each other")
 
 
 _COUNTERS = {}

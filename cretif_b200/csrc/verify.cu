@@ -889,9 +889,9 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
                                     int top_k, int* accepted, int* tokens, int ld_tokens,
                                     void* scratch, unsigned int* fault, void* stream) {
   if (B <= 0) return kOk;
-  if (V <= 0 || ld < V || K < 0 || n_rows <= 0 || ld_tokens < K + 1 || top_k < 0 || temperature != temperature ||
-      (temperature > 0 && top_k > kVfMaxTopK && top_k < V) || (K > 0 && ld_drafts < K) ||
-      (draft_logits && ld_place < V) || B > 65535 || !scratch)
+  if (V <= 0 || ld < 0 || K < 0 || n_rows <= 0 || (B > 1 && ld_tokens < K + 1) || top_k < 0 ||
+      temperature != temperature || (temperature > 0 && top_k > kVfMaxTopK && top_k < V) || ld_drafts < 0 || ld_u < 0 ||
+      ld_seq < 0 || ld_place < 0 || B > 65535 || !scratch)
     return kBadArgument;
   const bool greedy = temperature <= 0.0;
   if (greedy) draft_logits = nullptr;

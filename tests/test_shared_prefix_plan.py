@@ -5,9 +5,9 @@ import torch
 from cretif_b200.csrc import ops
 
 
-def walk(groups, news, starts, nh, nkv, tile_rows, own_rows, ctas):
+def walk(groups, news, starts, nh, nkv, tile_rows, own_rows, ctas, whole=False):
     pre, own, splits, pieces, rows, tok_pieces, prefix = ops._shared_items(
-        groups, news, starts, nh, nkv, tile_rows, own_rows, ctas)
+        groups, news, starts, nh, nkv, tile_rows, own_rows, ctas, whole)
     g = nh // nkv
     cu = [0]
     for n in news:
@@ -28,13 +28,13 @@ def walk(groups, news, starts, nh, nkv, tile_rows, own_rows, ctas):
     for t, b in enumerate(tok_seq):
         assert cu[b] <= t < cu[b + 1]
         for h in range(g):
-            for blk in range(prefix[b] // 64):
+            for blk in range(0 if whole else prefix[b] // 64):
                 assert (t, h, blk) in seen
-    assert len(seen) == g * sum(prefix[b] // 64 * news[b] for b in range(len(news)))
+    assert len(seen) == (0 if whole else g * sum(prefix[b] // 64 * news[b] for b in range(len(news))))
     mine = set()
     for i in range(0, len(own), 8):
-        b, tok0, row0, n, shared, mine_pieces = own[i:i + 6]
-        assert 0 < n <= own_rows and tok0 == cu[b] and shared == prefix[b]
+        b, tok0, row0, n, shared, mine_pieces, least, _ = own[i:i + 8]
+        assert 0 < n <= own_rows and tok0 == cu[b] and shared == (0 if whole else prefix[b]) and least == prefix[b]
         assert all(tok_pieces[t] == mine_pieces for t in range(cu[b], cu[b + 1]))
         for r in range(row0, row0 + n):
             assert (b, r) not in mine
@@ -51,6 +51,7 @@ def test_every_row_meets_every_key_once(tile_rows, own_rows, ctas):
     walk([(list(range(50)), 1024)], [1 + b % 3 for b in range(50)], [1024 + b for b in range(50)], 9, 3, tile_rows,
          own_rows, ctas)
     walk([], [1, 2], [0, 5], 4, 1, tile_rows, own_rows, ctas)
+    walk([([0, 2], 128), ([1], 64)], [1, 2, 1], [128, 70, 140], 4, 1, tile_rows, own_rows, ctas, whole=True)
     walk([([0], 0), ([1], 64)], [1, 2], [0, 64], 4, 1, tile_rows, own_rows, ctas)
 
 

@@ -204,6 +204,22 @@ def test_strides(ops):
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_rows_that_lie_over_each_other(ops):
+    """One row of logits for every place (expanded tensors) is read as such."""
+    s = make(4, 3, 777, [3, 3, 2, 0], seed=13, temperature=0.8, top_k=0)
+    row, q = s["logits"][:1], s["draft_logits"][:1, :1]
+    t = {**s, "logits": row.expand(s["logits"].shape), "draft_logits": q.expand(4, 3, 777)}
+    same = {**s, "logits": t["logits"].contiguous(), "draft_logits": t["draft_logits"].contiguous()}
+    for k in (0, 20):
+        want = verify(ops, same, 0.8, k, same["draft_logits"])
+        got = verify(ops, t, 0.8, k, t["draft_logits"])
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with pytest.raises(ops.KernelError):
+        ops.verify_drafts(s["logits"], s["cu"], s["drafts"], s["accept_u"], s["next_u"],
+                          torch.empty(4, dtype=torch.int32, device="cuda"),
+                          torch.empty((1, 4), dtype=torch.int32, device="cuda").expand(4, 4), 0.8)
+
+
 def test_broken_input_sets_the_fault_word(ops):
     s = make(3, 2, 500, [2, 2, 2], seed=8, temperature=0.8, top_k=0)
     fault = torch.zeros(1, dtype=torch.int32, device="cuda")
