@@ -1871,22 +1871,24 @@ class SharedPrefixPlan:
     __slots__ = ("data", "device", "sizes", "launch", "pieces", "kernels", "prefix_blocks", "T", "B")
 
 
-def _blocks_an_item(tiles, ctas: int, begin: int = 4) -> int:
+def _blocks_an_item(tiles, ctas: int, turns: int = 1, begin: float = 4.0, join: float = 0.8) -> int:
     """How many blocks of its prefix an item walks: ``tiles`` are (blocks of a prefix, items that walk
-    each of its ranges at once) pairs; the fewest turns of ``ctas`` items times what one takes, which
-    is its blocks and some ``begin`` more for setting up."""
+    each of its ranges at once) pairs.  The least of: the turns of ``ctas`` items times what one takes,
+    which is its blocks and some ``begin`` more for setting up, and the joining of the pieces, eight at a
+    time in ``turns`` turns of ``join`` each.  (16 heads of 128 on 2, 24 rows a sequence, 2,432 shared
+    tokens: 19 pieces PIECES19 us, 8 pieces PIECES8.)"""
     longest = max((blocks for blocks, _ in tiles), default=1)
     best = (None, longest)
     for pieces in range(1, min(longest, ctas) + 1):
         per = -(-longest // pieces)
         items = sum(-(-blocks // per) * n for blocks, n in tiles)
-        cost = -(-items // ctas) * (per + begin)
+        cost = -(-items // ctas) * (per + begin) + -(-pieces // 8) * turns * join
         if best[0] is None or cost < best[0]:
             best = (cost, per)
     return best[1]
 
 
-def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_rows: int, ctas: int,
+def _shared_items(groups, news, starts, nh: int, nkv: int, hd: int, tile_rows: int, own_rows: int, ctas: int,
                   walk: bool = False):
     """The host side of a plan: (prefix items, own items, splits of the own keys, most pieces, tokens
     of the groups, pieces of a token, prefix of a sequence), lists of integers.  ``walk``: the shared
@@ -1923,7 +1925,8 @@ def _shared_items(groups, news, starts, nh: int, nkv: int, tile_rows: int, own_r
             rows += toks
     tok_pieces = [0] * cu[-1]
     pre = []
-    per = _blocks_an_item([(blocks, -(-len(toks) * g // tile_rows) * nkv) for blocks, _, toks, _ in grouped], ctas)
+    per = _blocks_an_item([(blocks, -(-len(toks) * g // tile_rows) * nkv) for blocks, _, toks, _ in grouped], ctas,
+                          -(-min(own_rows, max(news) * g) * hd // 512))
     for blocks, base, toks, member in grouped:
         pieces = -(-blocks // per)
         for t in toks:
@@ -1972,7 +1975,7 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
     tile_rows, own_rows = (128, 16) if dtype == torch.bfloat16 else (32, 32)
     if dtype == torch.bfloat16 and nkv > 0 and max(news, default=1) * nh // nkv <= 8:
         own_rows = 8
-    pre, own, splits, pieces, rows, tok_pieces, prefix_of = _shared_items(groups, news, starts, nh, nkv, tile_rows,
+    pre, own, splits, pieces, rows, tok_pieces, prefix_of = _shared_items(groups, news, starts, nh, nkv, hd, tile_rows,
                                                                           own_rows, ctas, walk)
     plan = SharedPrefixPlan()
     packed = torch.tensor(pre + own + rows + tok_pieces, dtype=torch.int32)

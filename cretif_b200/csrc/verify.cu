@@ -41,6 +41,7 @@ struct VfArgs {
   int ld_u;
   const float* next_u;
   double log2_t;                // log2 e / T, within what float32 holds
+  float reach;                  // how far below the largest entry an entry counts: 1000 / log2_t
   int top_k;
   int* accepted;
   int* tokens;
@@ -253,6 +254,18 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const __grid_constan
 // ---- second launch, whole vocabulary: a cluster a sequence, its CTAs share the vocabulary
 constexpr int kVdThreads = 512, kVdSeg = 128;             // entries a warp takes at once
 
+// 2^(i / 32)
+__device__ const double kVfTable[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
+
 // A row's terms 2^((v - top) c) in 64 bits.  32 (v - top) c = n + f with |f| <= 1/2; 2^(n / 32) from a
 // table of 32 and a power of two, 2^(f / 32) by its series to the fifth power (the sixth term is below
 // 2.3e-15) (table-driven exponential, P. T. P. Tang, 1989).  Some 20 instructions, ten of them 64-bit.
@@ -260,13 +273,13 @@ struct VfTerm {
   double c32, top;              // 32 log2 e / T, the row's maximum
   float lo;                     // entries below it (2^-1000 of the largest) and NaN count 0
   bool infinite;                // the maximum is: entries equal to it count 1, all others 0
-  __device__ __forceinline__ void set(float top_, double c) {
+  __device__ __forceinline__ void set(float top_, double c, float reach) {       // reach: 1000 / c
     infinite = fabsf(top_) == INFINITY;
     top = top_;
     c32 = 32.0 * c;
     lo = top_;
     if (!infinite) {
-      lo = (float)((double)top_ - 1000.0 / c);
+      lo = top_ - reach;
       // (rounded down too far, an entry's n would not fit an exponent)
       while (lo < top_ && ((double)lo - (double)top_) * c < -1020.0) lo = nextafterf(lo, INFINITY);
     }
@@ -312,17 +325,18 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
   // sums of the CTA's segments; where they fit (cached) the terms of its share of both rows
   extern __shared__ __align__(16) double vd_smem[];
   __shared__ double table[32];
-  __shared__ double sums[kVdThreads / 32];
-  __shared__ double shared_tot[3];                        // this CTA's: p, q, what is drawn from
+  __shared__ double sums[2 * kVdThreads / 32];
+  __shared__ double shared_tot[4];                        // this CTA's: p and q, what is drawn from
+  __shared__ double weight_s;
+  __shared__ bool left_s;
   __shared__ int first_bad;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int kWarps = kVdThreads / 32;
-  if (tid < 32) table[tid] = exp2((double)tid / 32.0);
+  if (tid < 32) table[tid] = kVfTable[tid];
   if (tid == 0) first_bad = 0x7fffffff;
   dependent_begin();
-  __syncthreads();
   int row0, n;
   int* out = a.tokens + (size_t)b * a.ld_tokens;
   if (!vf_sequence(a, b, row0, n)) {                      // (all CTAs of the cluster alike)
@@ -332,12 +346,27 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
     }
     return;
   }
-  // ---- which drafts stand: a warp a draft
+  // ---- the rows' maxima and sums, a warp a row: the logits' n + 1 rows, then the drafts' n; meanwhile
+  // a thread a draft has its numbers on their way
   const float cf = (float)a.log2_t;
   const VfPart* stats = static_cast<const VfPart*>(a.stats);
-  auto whole = [&](int row) {                             // a row's maximum and sum
+  VfPart* rows = reinterpret_cast<VfPart*>(vd_smem);      // [2 K + 1]
+  const bool proposed = a.draft_logits != nullptr;
+  int d = -1;
+  float u = 0.f, xd = 0.f, yd = 0.f;
+  auto draft = [&](int j) {
+    d = a.drafts[(size_t)b * a.ld_drafts + j];
+    u = a.accept_u[(size_t)b * a.ld_u + j];
+    if (d >= 0 && d < a.V) {
+      xd = a.logits[(size_t)(row0 + j) * a.ld + d];
+      if (proposed) yd = a.draft_logits[b * a.ld_seq + j * a.ld_place + d];
+    }
+  };
+  if (tid < n) draft(tid);
+  for (int i = warp; i < (proposed ? 2 * n + 1 : n + 1); i += kWarps) {
+    const size_t row = i <= n ? row0 + i : a.n_rows + (size_t)b * a.K + (i - n - 1);
     VfPart p{-INFINITY, 0.f};
-    for (int i = lane; i < a.slices; i += 32) p = vf_merge(p, stats[(size_t)row * a.slices + i], cf);
+    for (int s = lane; s < a.slices; s += 32) p = vf_merge(p, stats[row * a.slices + s], cf);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       VfPart q;
@@ -345,53 +374,63 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
       q.z = __shfl_xor_sync(0xffffffffu, p.z, o);
       p = vf_merge(p, q, cf);
     }
-    return p;
-  };
-  for (int j = warp; j < n; j += kWarps) {
-    const int d = a.drafts[(size_t)b * a.ld_drafts + j];
-    const bool in = d >= 0 && d < a.V;
+    if (lane == 0) rows[i] = p;
+  }
+  __syncthreads();
+  // ---- which drafts stand
+  for (int j = tid; j < n; j += kVdThreads) {
+    if (j != tid) draft(j);
     bool stands = false;
-    if (in) {
+    if (d >= 0 && d < a.V) {
       VfTerm t;
-      const VfPart p = whole(row0 + j);
-      t.set(p.m, a.log2_t);
-      const double px = t(a.logits[(size_t)(row0 + j) * a.ld + d], table) / (double)p.z;
+      t.set(rows[j].m, a.log2_t, a.reach);
+      const double px = t(xd, table) / (double)rows[j].z;
       double qx = 1.0;
-      if (a.draft_logits) {
-        const VfPart q = whole(a.n_rows + b * a.K + j);
-        t.set(q.m, a.log2_t);
-        qx = t(a.draft_logits[b * a.ld_seq + j * a.ld_place + d], table) / (double)q.z;
+      if (proposed) {
+        t.set(rows[n + 1 + j].m, a.log2_t, a.reach);
+        qx = t(yd, table) / (double)rows[n + 1 + j].z;
       }
-      stands = (double)a.accept_u[(size_t)b * a.ld_u + j] * qx < px;
+      stands = (double)u * qx < px;
     }
-    if (!stands && lane == 0) atomicMin(&first_bad, j);
+    if (!stands) atomicMin(&first_bad, j);
   }
   __syncthreads();
   const int j = min(first_bad, n);
   const bool rest = j < n;
-  const int d = rest ? a.drafts[(size_t)b * a.ld_drafts + j] : -1;
+  d = rest ? a.drafts[(size_t)b * a.ld_drafts + j] : -1;
   if (rest && (d < 0 || d >= a.V) && rank == 0 && tid == 0) atomicOr(a.fault, (unsigned)kFaultTokenRange);
   // ---- the row (two rows) to draw from
-  const bool minus_q = rest && a.draft_logits != nullptr;
+  const bool minus_q = rest && proposed;
   const float* xp = a.logits + (size_t)(row0 + j) * a.ld;
   const float* xq = minus_q ? a.draft_logits + b * a.ld_seq + j * a.ld_place : xp;
   const bool ap = ((uintptr_t)xp & 15) == 0, aq = ((uintptr_t)xq & 15) == 0;
   VfTerm tp, tq;
-  tp.set(whole(row0 + j).m, a.log2_t);
+  tp.set(rows[j].m, a.log2_t, a.reach);
   tq = tp;
-  if (minus_q) tq.set(whole(a.n_rows + b * a.K + j).m, a.log2_t);
+  if (minus_q) tq.set(rows[n + 1 + j].m, a.log2_t, a.reach);
+  __syncthreads();                                        // (the rows' numbers give way to the segments')
   const int segs = (a.V + kVdSeg - 1) / kVdSeg;
   const int s0 = (int)((long long)segs * rank / C), s1 = (int)((long long)segs * (rank + 1) / C);
-  auto block_total = [&](double v, double* where) {       // into *where of this CTA
+  // Two sums of all the cluster's threads, for warp 0; each in this CTA's shared_tot[at] and [at + 1].
+  // Lane r < C of warp 0 has CTA r's afterwards.
+  auto gather = [&](double v, double w, int at, double& rv, double& rw) {
     v = vf_warp_sum(v);
-    if (lane == 0) sums[warp] = v;
+    w = vf_warp_sum(w);
+    if (lane == 0) { sums[warp] = v; sums[kWarps + warp] = w; }
     __syncthreads();
-    if (tid == 0) {
-      double t = 0.0;
-      for (int w = 0; w < kWarps; ++w) t += sums[w];
-      *where = t;
+    if (warp == 0) {                                      // 16 warps: lanes 0-15 the first sum, 16-31 the second
+      double t = sums[lane];
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      if ((lane & 15) == 0) shared_tot[at + (lane >> 4)] = t;
     }
-    __syncthreads();
+    cluster.sync();
+    rv = rw = 0.0;
+    if (warp == 0 && lane < C) {
+      const double* there = cluster.map_shared_rank(shared_tot, lane);
+      rv = there[at];
+      rw = there[at + 1];
+    }
   };
   double2* keep = reinterpret_cast<double2*>(vd_smem + seg_room);   // [segment][row][lane][2]
   // the four terms of a lane in a segment of a row (0 behind the vocabulary)
@@ -424,16 +463,17 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
         at[96] = make_double2(vq[2], vq[3]);
       }
     }
-    block_total(zp, &shared_tot[0]);
-    block_total(zq, &shared_tot[1]);
-    cluster.sync();
-    double all_p = 0.0, all_q = 0.0;
-    for (int r = 0; r < C; ++r) {
-      const double* there = cluster.map_shared_rank(shared_tot, r);
-      all_p += there[0];
-      all_q += there[1];
+    double rp, rq, all_p = 0.0, all_q = 0.0;
+    gather(zp, zq, 0, rp, rq);
+    if (warp == 0) {
+      for (int r = 0; r < C; ++r) {                       // (in the same order everywhere)
+        all_p += __shfl_sync(0xffffffffu, rp, r);
+        all_q += __shfl_sync(0xffffffffu, rq, r);
+      }
+      if (lane == 0) weight_s = all_p / all_q;
     }
-    weight = all_p / all_q;
+    __syncthreads();
+    weight = weight_s;
   }
   for (int turn = rest ? 0 : 1; turn < 2; ++turn) {       // (the second where p and q leave nothing)
     const bool minus = turn == 0;
@@ -475,23 +515,25 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
         mine += sum;
       }
     }
-    block_total(mine, &shared_tot[2]);
-    cluster.sync();
-    double total = 0.0, base = 0.0;
+    double rv, unused, total = 0.0, base = 0.0, own = 0.0;
+    gather(mine, 0.0, 2, rv, unused);
     int last_rank = -1;
-    for (int r = 0; r < C; ++r) {
-      const double t = cluster.map_shared_rank(shared_tot, r)[2];
-      if (r == rank) base = total;
+    for (int r = 0; r < C; ++r) {                         // (warp 0 has the numbers, and goes on alone)
+      const double t = __shfl_sync(0xffffffffu, rv, r);
+      if (r == rank) { base = total; own = t; }
       if (t > 0.0) last_rank = r;
       total += t;
     }
-    cluster.sync();                                       // nobody leaves, or writes again, before all have read
-    if (!(total > 0.0)) continue;
+    cluster.barrier_arrive();                             // its reads of the others' memory are done
+    if (tid == 0) left_s = total > 0.0;
+    __syncthreads();
+    const bool left = left_s;
+    if (!left && turn == 0) { cluster.barrier_wait(); continue; }
     // (a number that is not in [0, 1) counts as the nearest that is)
     double goal = (double)a.next_u[b] * total;
     if (!(goal >= 0.0)) goal = 0.0;
     const bool past = goal >= total;                      // the last id with any
-    const bool here = past ? rank == last_rank : base <= goal && goal < base + shared_tot[2];
+    const bool here = past ? rank == last_rank : base <= goal && goal < base + own;
     if (here && warp == 0) {
       // the segment, 32 at a time, and the place in it
       double run = base;
@@ -548,6 +590,7 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
         out[i] = i < j ? a.drafts[(size_t)b * a.ld_drafts + i] : i == j ? next : -1;
       if (lane == 0) a.accepted[b] = j;
     }
+    cluster.barrier_wait();                               // nobody leaves before all have read
     break;
   }
 }
@@ -557,14 +600,17 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
 // above it are few more than k.  They are listed in a second look at the row (from L2) and sorted by
 // (value, id).  Where they are too many for the list (equal logits in masses) the k-th largest is
 // found digit by digit over the whole row.
-constexpr int kVkThreads = 1024, kVkList = 4096;
+// (512 threads: three CTAs of them fit an SM, and one's sort runs under another's loads.  218 rows of 49,152:
+// KEPT_NOW us, with 1,024 threads, one CTA an SM, 35.)
+constexpr int kVkThreads = 512, kVkWarps = kVkThreads / 32, kVkList = 4096;
+constexpr int kVkMaxima = kVfMaxTopK / kVkThreads;        // maxima a thread keeps: together at least top_k
 
 struct VkShared {
   unsigned long long list[kVkList];
-  double sums[32];
+  double sums[kVkWarps];
   unsigned int hist[256];
   unsigned int digit, need, count;
-  unsigned int best[32];
+  unsigned int best[kVkWarps];
 };
 
 // The key of the need-th largest of what `each` hands to its argument, 8 bits at a time; `need` is
@@ -613,7 +659,7 @@ __device__ __forceinline__ unsigned int vk_select(VkShared& s, unsigned int need
   return prefix;
 }
 
-__global__ void __launch_bounds__(kVkThreads)
+__global__ void __launch_bounds__(kVkThreads, 3)
 verify_kept_kernel(const __grid_constant__ VfArgs a) {
   __shared__ VkShared s;
   dependent_begin();
@@ -623,7 +669,7 @@ verify_kept_kernel(const __grid_constant__ VfArgs a) {
   const int head = min(V, (int)((0u - (unsigned)((uintptr_t)x >> 2)) & 3u));
   const int n4 = (V - head) >> 2, tail = V - head - 4 * n4;
   const float4* x4 = reinterpret_cast<const float4*>(x + head);
-  // f(value, id) for every entry of the row, a thread's in ascending order of id but the odd ones
+  // f(value, id, turn) for every entry of the row
   auto each = [&](auto f) {
     constexpr int U = 4;
     for (int i0 = tid; i0 < n4; i0 += U * kVkThreads) {
@@ -635,28 +681,37 @@ verify_kept_kernel(const __grid_constant__ VfArgs a) {
       for (int u = 0; u < U; ++u) {
         const int i = i0 + u * kVkThreads;
         if (i < n4) {
-          f(v[u].x, head + 4 * i); f(v[u].y, head + 4 * i + 1); f(v[u].z, head + 4 * i + 2); f(v[u].w, head + 4 * i + 3);
+          f(v[u].x, head + 4 * i, u);
+          f(v[u].y, head + 4 * i + 1, u);
+          f(v[u].z, head + 4 * i + 2, u);
+          f(v[u].w, head + 4 * i + 3, u);
         }
       }
     }
     if (tid < head + tail) {
       const int id = tid < head ? tid : 4 * n4 + tid;
-      f(x[id], id);
+      f(x[id], id, 0);
     }
   };
-  unsigned int mine = 0u;
-  each([&](float v, int) { mine = max(mine, vf_key(v)); });
-  unsigned int best = __reduce_max_sync(0xffffffffu, mine);
+  unsigned int mine[kVkMaxima] = {};
+  each([&](float v, int, int u) { mine[u % kVkMaxima] = max(mine[u % kVkMaxima], vf_key(v)); });
+  unsigned int best = 0u;
+#pragma unroll
+  for (int i = 0; i < kVkMaxima; ++i) best = max(best, mine[i]);
+  best = __reduce_max_sync(0xffffffffu, best);
   if (lane == 0) s.best[warp] = best;
   if (tid == 0) s.count = 0u;
   __syncthreads();
-  best = __reduce_max_sync(0xffffffffu, s.best[lane]);
+  best = __reduce_max_sync(0xffffffffu, s.best[lane % kVkWarps]);
   const float top = vf_value(best);
-  // (threads without entries hold key 0, below every entry's; there are at least k entries, and where
-  // V < 1,024 some of the k largest maxima may be such: everything is listed then)
+  // (a maximum of no entries is key 0, below every entry's; where V < 4,096 one of the k largest maxima
+  // may be such, and everything is listed then)
   unsigned int equal;
-  const unsigned int floor_key = vk_select(s, (unsigned)k, equal, [&](auto f) { f(mine); });
-  each([&](float v, int id) {
+  const unsigned int floor_key = vk_select(s, (unsigned)k, equal, [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < kVkMaxima; ++i) f(mine[i]);
+  });
+  each([&](float v, int id, int) {
     if (vf_key(v) >= floor_key) {
       const unsigned int at = atomicAdd(&s.count, 1u);
       if (at < kVkList) s.list[at] = vf_rank(v, id);
@@ -666,10 +721,10 @@ verify_kept_kernel(const __grid_constant__ VfArgs a) {
   unsigned int n = s.count;
   if (n > kVkList) {
     // list the larger ones and the equals with the lowest ids: the equals' ids are taken in the row's order
-    const unsigned int kth = vk_select(s, (unsigned)k, equal, [&](auto f) { each([&](float v, int) { f(vf_key(v)); }); });
+    const unsigned int kth = vk_select(s, (unsigned)k, equal, [&](auto f) { each([&](float v, int, int) { f(vf_key(v)); }); });
     if (tid == 0) s.count = 0u;
     __syncthreads();
-    each([&](float v, int id) {
+    each([&](float v, int id, int) {
       if (vf_key(v) > kth) s.list[atomicAdd(&s.count, 1u)] = vf_rank(v, id);
     });
     __syncthreads();
@@ -681,7 +736,7 @@ verify_kept_kernel(const __grid_constant__ VfArgs a) {
       if (lane == 0) s.best[warp] = __popc(votes);
       __syncthreads();
       unsigned int before = __popc(votes & ((1u << lane) - 1u)), all = 0u;
-      for (int w = 0; w < 32; ++w) {
+      for (int w = 0; w < kVkWarps; ++w) {
         if (w < warp) before += s.best[w];
         all += s.best[w];
       }
@@ -711,20 +766,20 @@ verify_kept_kernel(const __grid_constant__ VfArgs a) {
   // the kept ones, their sum in 64 bits
   const double c = a.log2_t;
   double z = 0.0;
-  if (tid < k) {
-    const unsigned long long r = s.list[tid];
+  for (int i = tid; i < k; i += kVkThreads) {
+    const unsigned long long r = s.list[i];
     const float v = vf_value((unsigned int)(r >> 32));
-    const size_t at = (size_t)blockIdx.x * k + tid;
+    const size_t at = (size_t)blockIdx.x * k + i;
     a.list_v[at] = v;
     a.list_i[at] = (int)(0xffffffffu - (unsigned)r);
-    z = v == top ? 1.0 : fabsf(top) == INFINITY ? 0.0 : exp2(((double)v - (double)top) * c);
+    z += v == top ? 1.0 : fabsf(top) == INFINITY ? 0.0 : exp2(((double)v - (double)top) * c);
   }
   z = vf_warp_sum(z);
   if (lane == 0) s.sums[warp] = z;
   __syncthreads();
   if (tid == 0) {
     double t = 0.0;
-    for (int w = 0; w < 32; ++w) t += s.sums[w];
+    for (int w = 0; w < kVkWarps; ++w) t += s.sums[w];
     static_cast<VfKept*>(a.stats)[blockIdx.x] = VfKept{t, s.list[k - 1], top, 0};
   }
 }
@@ -736,6 +791,7 @@ __global__ void __launch_bounds__(kVlThreads)
 verify_kept_draw_kernel(const __grid_constant__ VfArgs a) {
   __shared__ unsigned long long order[kVfMaxTopK];         // (id, place in the list), by id
   __shared__ double term[kVfMaxTopK];
+  int* term_ids = reinterpret_cast<int*>(term);            // (before the terms are)
   __shared__ double sums[kVlThreads / 32];
   __shared__ int first_bad, chosen;
   dependent_begin();
@@ -782,22 +838,38 @@ verify_kept_draw_kernel(const __grid_constant__ VfArgs a) {
   const float* xq = minus_q ? a.draft_logits + b * a.ld_seq + j * a.ld_place : nullptr;
   const double weight = p.z / q.z;
   const size_t list = (size_t)(row0 + j) * k;
-  int np2 = 1;
-  while (np2 < k) np2 <<= 1;
-  for (int i = tid; i < np2; i += kVlThreads)
-    order[i] = i < k ? ((unsigned long long)(unsigned)a.list_i[list + i] << 32) | (unsigned)i : ~0ull;
-  __syncthreads();
-  for (int size = 2; size <= np2; size <<= 1)
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      for (int i = tid; i < np2; i += kVlThreads) {
-        const int o = i ^ stride;
-        if (o > i) {
-          const unsigned long long u = order[i], v = order[o];
-          if ((u < v) != ((i & size) == 0)) { order[i] = v; order[o] = u; }
-        }
-      }
-      __syncthreads();
+  // the kept ids in ascending order: an id's place is how many are smaller where a thread has one id,
+  // else they are sorted
+  if (k <= kVlThreads) {
+    unsigned long long mine = 0ull;
+    if (tid < k) term_ids[tid] = a.list_i[list + tid];
+    __syncthreads();
+    if (tid < k) {
+      const int id = term_ids[tid];
+      mine = ((unsigned long long)(unsigned)id << 32) | (unsigned)tid;
+      int at = 0;
+      for (int i = 0; i < k; ++i) at += term_ids[i] < id;
+      order[at] = mine;
     }
+    __syncthreads();
+  } else {
+    int np2 = 1;
+    while (np2 < k) np2 <<= 1;
+    for (int i = tid; i < np2; i += kVlThreads)
+      order[i] = i < k ? ((unsigned long long)(unsigned)a.list_i[list + i] << 32) | (unsigned)i : ~0ull;
+    __syncthreads();
+    for (int size = 2; size <= np2; size <<= 1)
+      for (int stride = size >> 1; stride > 0; stride >>= 1) {
+        for (int i = tid; i < np2; i += kVlThreads) {
+          const int o = i ^ stride;
+          if (o > i) {
+            const unsigned long long u = order[i], v = order[o];
+            if ((u < v) != ((i & size) == 0)) { order[i] = v; order[o] = u; }
+          }
+        }
+        __syncthreads();
+      }
+  }
   int next = 0;
   for (int turn = rest ? 0 : 1; turn < 2; ++turn) {
     // a thread's entries lie together: `per` of them
@@ -900,8 +972,9 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
   if (rows > 0x7fffffffLL) return kBadArgument;
   cudaStream_t st = (cudaStream_t)stream;
   VfArgs a{logits, ld, n_rows, cu, drafts, ld_drafts, K, B, V, draft_logits, ld_seq, ld_place, accept_u, ld_u, next_u,
-           greedy ? 1.0 : fmin(fmax(1.4426950408889634 / temperature, 1e-30), 3e38), top_k, accepted, tokens, ld_tokens, fault, scratch, 0, 0,
+           greedy ? 1.0 : fmin(fmax(1.4426950408889634 / temperature, 1e-30), 3e38), 0.f, top_k, accepted, tokens, ld_tokens, fault, scratch, 0, 0,
            nullptr, nullptr};
+  a.reach = (float)fmin(1000.0 / a.log2_t, 3e38);
   if (kept) {
     a.list_v = reinterpret_cast<float*>(static_cast<char*>(scratch) + rows * sizeof(VfKept));
     a.list_i = reinterpret_cast<int*>(a.list_v + rows * top_k);
@@ -922,7 +995,10 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
   int C = 8;
   while (C > 1 && (B * C > 4 * kSmCount || V < 1024 * C)) C >>= 1;
   const int segs = ((V + kVdSeg - 1) / kVdSeg + C - 1) / C + 1;
-  const int room = (segs + 1) & ~1;
+  // segments' sums, and before them the rows' numbers
+  const long long room_ll = segs > 2LL * K + 1 ? segs : 2LL * K + 1;
+  if (room_ll > 16 * 1024) return kBadArgument;
+  const int room = ((int)room_ll + 1) & ~1;
   // (two CTAs fit an SM with up to 100 KB of terms each)
   const int cached = a.draft_logits && (size_t)segs * kVdSeg * 16 <= 100 * 1024;
   const size_t smem = (size_t)room * 8 + (cached ? (size_t)segs * kVdSeg * 16 : 0);

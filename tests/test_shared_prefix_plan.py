@@ -7,7 +7,7 @@ from cretif_b200.csrc import ops
 
 def walk(groups, news, starts, nh, nkv, tile_rows, own_rows, ctas, whole=False):
     pre, own, splits, pieces, rows, tok_pieces, prefix = ops._shared_items(
-        groups, news, starts, nh, nkv, tile_rows, own_rows, ctas, whole)
+        groups, news, starts, nh, nkv, 64, tile_rows, own_rows, ctas, whole)
     g = nh // nkv
     cu = [0]
     for n in news:
