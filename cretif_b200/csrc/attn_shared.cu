@@ -11,11 +11,12 @@ namespace cretif {
 
 constexpr int kShRows = 32, kShThreads = 256;
 
-// 32-bit pieces: a block of 256 threads per (item, key/value head), 32 rows and 64 keys a step.  A
-// thread has two rows and four keys of the scores, and eight channels of two rows of the output; the
-// next step's keys and values are on their way in registers.  What bounds it at a decode step's sizes is
-// the chain of loads in front of the first product, so a block takes one block of keys where there
-// are few (eight answers at 1,984 tokens: F32_NOW us, F32_BEFORE with loads of one number at a time).
+// 32-bit pieces: a block of 256 threads per (item, key/value head), up to 32 rows and 64 keys a step.
+// A warp has rows w, w + 8, w + 16, w + 24, those that there are: a lane two keys of their scores and VD
+// channels of their outputs, so a softmax is the warp's own.  The next step's keys and values are on
+// their way in registers.  (Eight answers at 1,984 tokens: F32_NOW us; 16 x 16 threads on 32 rows whatever
+// there were took 25, most of it on the own keys' three rows.)
+template <int VD>
 __global__ void __launch_bounds__(kShThreads)
 shared_pieces_kernel(const SharedArgs a) {
   extern __shared__ __align__(16) float sh_smem[];
@@ -23,10 +24,11 @@ shared_pieces_kernel(const SharedArgs a) {
   float* qs = sh_smem;                        // [32][hd + 4]
   float* ks = qs + kShRows * ldk;             // [64][hd + 4]
   float* vs = ks + kShBlk * ldk;              // [64][hd]
-  float* ps = vs + kShBlk * hd;               // [32][65]
+  float* ps = vs + kShBlk * hd;               // [32][64]
   __shared__ int toks[kShRows];
   const int kvh = blockIdx.y, g = a.nh / a.nkv, tid = threadIdx.x;
-  const int tx = tid & 15, ty = tid >> 4;
+  const int warp = tid >> 5, lane = tid & 31;
+  constexpr int kRows = kShRows / 8;          // of a warp
   dependent_begin();
 
   // ---- this block's rows and keys
@@ -80,17 +82,21 @@ shared_pieces_kernel(const SharedArgs a) {
     }
     *reinterpret_cast<float4*>(qs + r * ldk + d) = v;
   }
-  int pos[2];
+  const int mine = warp < n_rows ? (n_rows - warp + 7) >> 3 : 0;      // rows of this warp
+  int pos[kRows];
+  float m[kRows], l[kRows], o[kRows][VD];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = ty + 16 * i;
-    pos[i] = r < n_rows ? (row_base >= 0 ? key_end - 1 : a.tok_pos[toks[r]]) : -1;
+  for (int i = 0; i < kRows; ++i) {
+    pos[i] = i < mine ? (row_base >= 0 ? key_end - 1 : a.tok_pos[toks[warp + 8 * i]]) : -1;
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < VD; ++e) o[i][e] = 0.f;
   }
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float o[2][2][4] = {};
+  const int d0 = lane * VD;                   // this lane's channels
+  const bool has_d = d0 < hd;
   for (int k0 = key0; k0 < key_end; k0 += kShBlk) {
     __syncthreads();                          // the last step's readers are done (and Q is there)
-    const int n = min(kShBlk, key_end - k0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int k = k_of + i * k_step;
@@ -101,79 +107,96 @@ shared_pieces_kernel(const SharedArgs a) {
     }
     __syncthreads();
     if (k0 + kShBlk < key_end) fetch(k0 + kShBlk);
-    float s[2][4] = {};
-    for (int d = 0; d < hd; d += 4) {
-      float4 kk[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) kk[c] = *reinterpret_cast<const float4*>(ks + (tx + 16 * c) * ldk + d);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float4 qq = *reinterpret_cast<const float4*>(qs + (ty + 16 * i) * ldk + d);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          s[i][c] = fmaf(qq.x, kk[c].x, fmaf(qq.y, kk[c].y, fmaf(qq.z, kk[c].z, fmaf(qq.w, kk[c].w, s[i][c]))));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int key = k0 + tx + 16 * c;
-        s[i][c] = key < key_end && key <= pos[i] ? s[i][c] * a.scale_log2 : -INFINITY;
-        mx = fmaxf(mx, s[i][c]);
-      }
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      const float m_new = fmaxf(m[i], mx);
-      const float alpha = m[i] == -INFINITY ? 0.f : exp2f(m[i] - m_new);
-      float sum = 0.f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float p = s[i][c] == -INFINITY ? 0.f : exp2f(s[i][c] - m_new);
-        sum += p;
-        ps[(ty + 16 * i) * 65 + tx + 16 * c] = p;
-      }
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      l[i] = l[i] * alpha + sum;
-      m[i] = m_new;
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][c][e] *= alpha;
-    }
-    __syncwarp();                             // a row's probabilities are its own half warp's
+    // (the number of rows is a constant inside: a branch a row kept the loads from overlapping)
+    auto step = [&](auto constant) {
+      constexpr int R = decltype(constant)::value;
+      float s[R][2][2] = {};
 #pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float p0 = ps[ty * 65 + k], p1 = ps[(ty + 16) * 65 + k];
+      for (int d = 0; d < hd; d += 4) {
+        const float4 ka = *reinterpret_cast<const float4*>(ks + lane * ldk + d);
+        const float4 kb = *reinterpret_cast<const float4*>(ks + (lane + 32) * ldk + d);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int d = tx * 4 + 64 * c;
-        if (d < hd) {
-          const float4 v = *reinterpret_cast<const float4*>(vs + k * hd + d);
-          o[0][c][0] = fmaf(p0, v.x, o[0][c][0]); o[0][c][1] = fmaf(p0, v.y, o[0][c][1]);
-          o[0][c][2] = fmaf(p0, v.z, o[0][c][2]); o[0][c][3] = fmaf(p0, v.w, o[0][c][3]);
-          o[1][c][0] = fmaf(p1, v.x, o[1][c][0]); o[1][c][1] = fmaf(p1, v.y, o[1][c][1]);
-          o[1][c][2] = fmaf(p1, v.z, o[1][c][2]); o[1][c][3] = fmaf(p1, v.w, o[1][c][3]);
+        for (int i = 0; i < R; ++i) {
+          const float4 qq = *reinterpret_cast<const float4*>(qs + (warp + 8 * i) * ldk + d);
+          s[i][0][0] = fmaf(qq.x, ka.x, fmaf(qq.y, ka.y, s[i][0][0]));
+          s[i][0][1] = fmaf(qq.z, ka.z, fmaf(qq.w, ka.w, s[i][0][1]));
+          s[i][1][0] = fmaf(qq.x, kb.x, fmaf(qq.y, kb.y, s[i][1][0]));
+          s[i][1][1] = fmaf(qq.z, kb.z, fmaf(qq.w, kb.w, s[i][1][1]));
         }
       }
-    }
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        float t2[2], mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int key = k0 + lane + 32 * c;
+          t2[c] = key < key_end && key <= pos[i] ? (s[i][c][0] + s[i][c][1]) * a.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, t2[c]);
+        }
+        mx = warp_max(mx);
+        const float m_new = fmaxf(m[i], mx);
+        const float alpha = m[i] == -INFINITY ? 0.f : exp2f(m[i] - m_new);
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float p = t2[c] == -INFINITY ? 0.f : exp2f(t2[c] - m_new);
+          sum += p;
+          ps[(warp + 8 * i) * kShBlk + lane + 32 * c] = p;
+        }
+        l[i] = l[i] * alpha + warp_sum(sum);
+        m[i] = m_new;
+#pragma unroll
+        for (int e = 0; e < VD; ++e) o[i][e] *= alpha;
+      }
+      __syncwarp();
+      if (has_d) {
+        float part[R][VD] = {};               // of the even pairs of keys
+#pragma unroll 4
+        for (int k = 0; k < kShBlk; k += 4) { // (keys past the last have probability and value zero)
+          float v[4][VD];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if constexpr (VD == 2) {
+              const float2 f = *reinterpret_cast<const float2*>(vs + (k + x) * hd + d0);
+              v[x][0] = f.x; v[x][1] = f.y;
+            } else {
+              const float4 f = *reinterpret_cast<const float4*>(vs + (k + x) * hd + d0);
+              v[x][0] = f.x; v[x][1] = f.y; v[x][2] = f.z; v[x][3] = f.w;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            const float4 p = *reinterpret_cast<const float4*>(ps + (warp + 8 * i) * kShBlk + k);
+#pragma unroll
+            for (int e = 0; e < VD; ++e) {
+              part[i][e] = fmaf(p.x, v[0][e], fmaf(p.y, v[1][e], part[i][e]));
+              o[i][e] = fmaf(p.z, v[2][e], fmaf(p.w, v[3][e], o[i][e]));
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+          for (int e = 0; e < VD; ++e) o[i][e] += part[i][e];
+      }
+    };
+    if (mine == 1) step(std::integral_constant<int, 1>{});
+    else if (mine == 2) step(std::integral_constant<int, 2>{});
+    else if (mine == 3) step(std::integral_constant<int, 3>{});
+    else if (mine == 4) step(std::integral_constant<int, 4>{});
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = ty + 16 * i;
-    if (r >= n_rows) continue;
-    const size_t row = ((size_t)piece * a.T + toks[r]) * a.nh + kvh * g + (row0 + r) % g;
-    if (tx == 0) a.part_ml[row] = make_float2(m[i], l[i]);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int d = tx * 4 + 64 * c;
-      if (d < hd)
-        *reinterpret_cast<float4*>(a.part_o + row * hd + d) =
-            make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
+  for (int i = 0; i < kRows; ++i)
+    if (i < mine) {
+      const int r = warp + 8 * i;
+      const size_t row = ((size_t)piece * a.T + toks[r]) * a.nh + kvh * g + (row0 + r) % g;
+      if (lane == 0) a.part_ml[row] = make_float2(m[i], l[i]);
+      if (has_d) {
+        float* to = a.part_o + row * hd + d0;
+        if constexpr (VD == 2) *reinterpret_cast<float2*>(to) = make_float2(o[i][0], o[i][1]);
+        else *reinterpret_cast<float4*>(to) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+      }
     }
-  }
 }
 
 // A warp joins the pieces of a row: four lanes' channels of a piece at once, so that 32 / (hd / 4) pieces
@@ -248,13 +271,14 @@ static int launch_join(const SharedArgs& a, cudaStream_t st) {
   return launch_status();
 }
 
+template <int VD>
 static int launch_shared_f32(const SharedArgs& a, cudaStream_t st) {
-  const size_t smem = ((size_t)(kShRows + kShBlk) * (a.hd + 4) + (size_t)kShBlk * a.hd + kShRows * 65) * 4;
-  cudaError_t e = cudaFuncSetAttribute(shared_pieces_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)smem);
+  const size_t smem = ((size_t)(kShRows + kShBlk) * (a.hd + 4) + (size_t)kShBlk * a.hd + kShRows * kShBlk) * 4;
+  const cudaError_t e = cudaFuncSetAttribute(shared_pieces_kernel<VD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)smem);
   if (e != cudaSuccess) return (int)e;
-  launch_dependent(shared_pieces_kernel, dim3(a.n_pre + a.n_own * a.own_splits, a.nkv), dim3(kShThreads),
-                   smem, st, a);
+  launch_dependent(shared_pieces_kernel<VD>, dim3(a.n_pre + a.n_own * a.own_splits, a.nkv), dim3(kShThreads), smem, st,
+                   a);
   return launch_join<float>(a, st);
 }
 
@@ -290,7 +314,8 @@ extern "C" int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int
   a.n_pre = n_pre; a.n_own = n_own; a.own_rows = own_rows; a.own_splits = own_splits; a.max_pieces = max_pieces; a.T = T;
   a.nh = nh; a.nkv = nkv; a.hd = hd; a.scale_log2 = scale * 1.4426950408889634f; a.sink = sink;
   a.part_o = part_o; a.part_ml = reinterpret_cast<float2*>(part_ml); a.fault = fault;
-  if (dt == kF32) return launch_shared_f32(a, (cudaStream_t)stream);
+  if (dt == kF32)
+    return hd <= 64 ? launch_shared_f32<2>(a, (cudaStream_t)stream) : launch_shared_f32<4>(a, (cudaStream_t)stream);
   const int e = launch_shared_bf16(a, (cudaStream_t)stream);
   return e || own_splits == 1 ? e : launch_join<__nv_bfloat16>(a, (cudaStream_t)stream);
 }

@@ -1889,7 +1889,7 @@ def _blocks_an_item(tiles, ctas: int, turns: int = 1, begin: float = 4.0, join: 
 
 
 def _shared_items(groups, news, starts, nh: int, nkv: int, hd: int, tile_rows: int, own_rows: int, ctas: int,
-                  walk: bool = False):
+                  walk: bool = False, own_depth: int = 8):
     """The host side of a plan: (prefix items, own items, splits of the own keys, most pieces, tokens
     of the groups, pieces of a token, prefix of a sequence), lists of integers.  ``walk``: the shared
     tokens are read by every sequence beside its own."""
@@ -1944,7 +1944,7 @@ def _shared_items(groups, news, starts, nh: int, nkv: int, hd: int, tile_rows: i
             own += [b, cu[b], row0, min(own_rows, news[b] * g - row0), apart[b], tok_pieces[cu[b]],
                     prefix_of[b], 0]
     own_blocks = max(-(-(starts[b] + news[b] - apart[b]) // 64) for b in range(B))
-    splits = max(1, min(own_blocks // 8, ctas // max(1, len(own) // 8 * nkv), 8))
+    splits = max(1, min(own_blocks // own_depth, ctas // max(1, len(own) // 8 * nkv), 8))
     return pre, own, splits, max(tok_pieces) + splits, rows, tok_pieces, prefix_of
 
 
@@ -1976,7 +1976,8 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
     if dtype == torch.bfloat16 and nkv > 0 and max(news, default=1) * nh // nkv <= 8:
         own_rows = 8
     pre, own, splits, pieces, rows, tok_pieces, prefix_of = _shared_items(groups, news, starts, nh, nkv, hd, tile_rows,
-                                                                          own_rows, ctas, walk)
+                                                                          own_rows, ctas, walk,
+                                                                          8 if dtype == torch.bfloat16 else 2)
     plan = SharedPrefixPlan()
     packed = torch.tensor(pre + own + rows + tok_pieces, dtype=torch.int32)
     plan.data = packed.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else packed

@@ -266,6 +266,12 @@ __device__ const double kVfTable[32] = {
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
 };
 
+// (ln2 / 32)^k / k! for k = 5 .. 1, 1, and 1.5 * 2^52, which rounds to an integer: in constant memory a
+// 64-bit product takes them as they are; written out, two moves bring each (64 sequences, 58.3 us
+// against CONST_NOW).
+__constant__ double kVfSeries[7] = {3.9737099845494154e-11, 9.172562701824643e-09, 1.6938509724371819e-06,
+                                    0.00023459619820224677, 0.02166084939249829, 1.0, 6755399441055744.0};
+
 // A row's terms 2^((v - top) c) in 64 bits.  32 (v - top) c = n + f with |f| <= 1/2; 2^(n / 32) from a
 // table of 32 and a power of two, 2^(f / 32) by its series to the fifth power (the sixth term is below
 // 2.3e-15) (table-driven exponential, P. T. P. Tang, 1989).  Some 20 instructions, ten of them 64-bit.
@@ -286,17 +292,16 @@ struct VfTerm {
   }
   __device__ __forceinline__ double operator()(float v, const double* table) const {
     if (infinite) return fmaxf(v, -INFINITY) == (float)top ? 1.0 : 0.0;
-    const double magic = 6755399441055744.0;              // 1.5 * 2^52: rounds to an integer
+    const double magic = kVfSeries[6];
     const double d = (double)fmaxf(v, lo) - top;
     const double big = fma(d, c32, magic);
     const int n = __double2loint(big);
     const double f = fma(d, c32, magic - big);
-    // (ln2 / 32)^k / k!
-    double p = fma(f, 3.9737099845494154e-11, 9.172562701824643e-09);
-    p = fma(f, p, 1.6938509724371819e-06);
-    p = fma(f, p, 0.00023459619820224677);
-    p = fma(f, p, 0.02166084939249829);
-    p = fma(f, p, 1.0);
+    double p = fma(f, kVfSeries[0], kVfSeries[1]);
+    p = fma(f, p, kVfSeries[2]);
+    p = fma(f, p, kVfSeries[3]);
+    p = fma(f, p, kVfSeries[4]);
+    p = fma(f, p, kVfSeries[5]);
     p *= table[n & 31];
     const bool any = v >= lo;
     return __hiloint2double(any ? __double2hiint(p) + ((n >> 5) << 20) : 0, any ? __double2loint(p) : 0);
@@ -320,7 +325,7 @@ __device__ __forceinline__ void vf_four(const float* x, int V, int i, bool align
   }
 }
 
-__global__ void __launch_bounds__(kVdThreads)
+__global__ void __launch_bounds__(kVdThreads, 2)
 verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
   // sums of the CTA's segments; where they fit (cached) the terms of its share of both rows
   extern __shared__ __align__(16) double vd_smem[];
@@ -418,11 +423,11 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
     w = vf_warp_sum(w);
     if (lane == 0) { sums[warp] = v; sums[kWarps + warp] = w; }
     __syncthreads();
-    if (warp == 0) {                                      // 16 warps: lanes 0-15 the first sum, 16-31 the second
-      double t = sums[lane];
+    if (warp == 0) {                                      // the first half of the lanes the first sum, the others the second
+      double t = lane < 2 * kWarps ? sums[lane] : 0.0;
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if ((lane & 15) == 0) shared_tot[at + (lane >> 4)] = t;
+      for (int o = kWarps / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      if (lane < 2 * kWarps && lane % kWarps == 0) shared_tot[at + lane / kWarps] = t;
     }
     cluster.sync();
     rv = rw = 0.0;
@@ -448,19 +453,41 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
   double weight = 0.0;                                    // of q's terms beside p's
   if (minus_q) {
     double zp = 0.0, zq = 0.0;
-#pragma unroll 2
-    for (int s = s0 + warp; s < s1; s += kWarps) {
-      double vp[4], vq[4];
-      look(tp, xp, ap, s, vp);
-      look(tq, xq, aq, s, vq);
-      zp += (vp[0] + vp[1]) + (vp[2] + vp[3]);
-      zq += (vq[0] + vq[1]) + (vq[2] + vq[3]);
-      if (cached) {
-        double2* at = keep + (size_t)(s - s0) * 128 + lane;
-        at[0] = make_double2(vp[0], vp[1]);
-        at[32] = make_double2(vp[2], vp[3]);
-        at[64] = make_double2(vq[0], vq[1]);
-        at[96] = make_double2(vq[2], vq[3]);
+    // the loads of kAhead segments go out together (rows on 16-byte boundaries, segments inside the row)
+    constexpr int kAhead = 3;
+    for (int base = s0 + warp; base < s1; base += kAhead * kWarps) {
+      float fp[kAhead][4], fq[kAhead][4];
+      const bool quick = ap && aq && (base + (kAhead - 1) * kWarps + 1) * kVdSeg <= a.V;
+      if (quick) {
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+          const int i = (base + x * kWarps) * 32 + lane;
+          const float4 u = __ldg(reinterpret_cast<const float4*>(xp) + i), w = __ldg(reinterpret_cast<const float4*>(xq) + i);
+          fp[x][0] = u.x; fp[x][1] = u.y; fp[x][2] = u.z; fp[x][3] = u.w;
+          fq[x][0] = w.x; fq[x][1] = w.y; fq[x][2] = w.z; fq[x][3] = w.w;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int s = base + x * kWarps;
+        if (s >= s1) break;
+        double vp[4], vq[4];
+        if (quick) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { vp[e] = tp(fp[x][e], table); vq[e] = tq(fq[x][e], table); }
+        } else {
+          look(tp, xp, ap, s, vp);
+          look(tq, xq, aq, s, vq);
+        }
+        zp += (vp[0] + vp[1]) + (vp[2] + vp[3]);
+        zq += (vq[0] + vq[1]) + (vq[2] + vq[3]);
+        if (cached) {
+          double2* at = keep + (size_t)(s - s0) * 128 + lane;
+          at[0] = make_double2(vp[0], vp[1]);
+          at[32] = make_double2(vp[2], vp[3]);
+          at[64] = make_double2(vq[0], vq[1]);
+          at[96] = make_double2(vq[2], vq[3]);
+        }
       }
     }
     double rp, rq, all_p = 0.0, all_q = 0.0;
@@ -693,26 +720,28 @@ verify_kept_kernel(const __grid_constant__ VfArgs a) {
       f(x[id], id, 0);
     }
   };
-  unsigned int mine[kVkMaxima] = {};
-  each([&](float v, int, int u) { mine[u % kVkMaxima] = max(mine[u % kVkMaxima], vf_key(v)); });
+  float mine[kVkMaxima];
+#pragma unroll
+  for (int i = 0; i < kVkMaxima; ++i) mine[i] = -INFINITY;
+  each([&](float v, int, int u) { mine[u % kVkMaxima] = fmaxf(mine[u % kVkMaxima], v); });
   unsigned int best = 0u;
 #pragma unroll
-  for (int i = 0; i < kVkMaxima; ++i) best = max(best, mine[i]);
+  for (int i = 0; i < kVkMaxima; ++i) best = max(best, vf_key(mine[i]));
   best = __reduce_max_sync(0xffffffffu, best);
   if (lane == 0) s.best[warp] = best;
   if (tid == 0) s.count = 0u;
   __syncthreads();
   best = __reduce_max_sync(0xffffffffu, s.best[lane % kVkWarps]);
   const float top = vf_value(best);
-  // (a maximum of no entries is key 0, below every entry's; where V < 4,096 one of the k largest maxima
-  // may be such, and everything is listed then)
+  // (a maximum of no entries is -infinity; where that is among the k largest everything is listed)
   unsigned int equal;
   const unsigned int floor_key = vk_select(s, (unsigned)k, equal, [&](auto f) {
 #pragma unroll
-    for (int i = 0; i < kVkMaxima; ++i) f(mine[i]);
+    for (int i = 0; i < kVkMaxima; ++i) f(vf_key(mine[i]));
   });
+  const float floor_value = vf_value(floor_key);
   each([&](float v, int id, int) {
-    if (vf_key(v) >= floor_key) {
+    if (fmaxf(v, -INFINITY) >= floor_value) {              // (NaN counts as -infinity)
       const unsigned int at = atomicAdd(&s.count, 1u);
       if (at < kVkList) s.list[at] = vf_rank(v, id);
     }
