@@ -266,12 +266,6 @@ __device__ const double kVfTable[32] = {
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
 };
 
-// (ln2 / 32)^k / k! for k = 5 .. 1, 1, and 1.5 * 2^52, which rounds to an integer: in constant memory a
-// 64-bit product takes them as they are; written out, two moves bring each (64 sequences, 58.3 us
-// against CONST_NOW).
-__constant__ double kVfSeries[7] = {3.9737099845494154e-11, 9.172562701824643e-09, 1.6938509724371819e-06,
-                                    0.00023459619820224677, 0.02166084939249829, 1.0, 6755399441055744.0};
-
 // A row's terms 2^((v - top) c) in 64 bits.  32 (v - top) c = n + f with |f| <= 1/2; 2^(n / 32) from a
 // table of 32 and a power of two, 2^(f / 32) by its series to the fifth power (the sixth term is below
 // 2.3e-15) (table-driven exponential, P. T. P. Tang, 1989).  Some 20 instructions, ten of them 64-bit.
@@ -292,16 +286,17 @@ struct VfTerm {
   }
   __device__ __forceinline__ double operator()(float v, const double* table) const {
     if (infinite) return fmaxf(v, -INFINITY) == (float)top ? 1.0 : 0.0;
-    const double magic = kVfSeries[6];
+    const double magic = 6755399441055744.0;              // 1.5 * 2^52: rounds to an integer
     const double d = (double)fmaxf(v, lo) - top;
     const double big = fma(d, c32, magic);
     const int n = __double2loint(big);
     const double f = fma(d, c32, magic - big);
-    double p = fma(f, kVfSeries[0], kVfSeries[1]);
-    p = fma(f, p, kVfSeries[2]);
-    p = fma(f, p, kVfSeries[3]);
-    p = fma(f, p, kVfSeries[4]);
-    p = fma(f, p, kVfSeries[5]);
+    // (ln2 / 32)^k / k!
+    double p = fma(f, 3.9737099845494154e-11, 9.172562701824643e-09);
+    p = fma(f, p, 1.6938509724371819e-06);
+    p = fma(f, p, 0.00023459619820224677);
+    p = fma(f, p, 0.02166084939249829);
+    p = fma(f, p, 1.0);
     p *= table[n & 31];
     const bool any = v >= lo;
     return __hiloint2double(any ? __double2hiint(p) + ((n >> 5) << 20) : 0, any ? __double2loint(p) : 0);
@@ -1036,7 +1031,7 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
   if (e != cudaSuccess) return (int)e;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = dependent_launch_enabled();
+  attr[0].val.programmaticStreamSerializationAllowed = C * B <= kSmCount ? dependent_launch_enabled() : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = C;
   attr[1].val.clusterDim.y = 1;

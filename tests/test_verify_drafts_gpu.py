@@ -139,6 +139,29 @@ def test_batches(ops, B, K):
         assert (accepted > 0).any() and (accepted < torch.tensor(counts)).any()
 
 
+@pytest.mark.parametrize("proposed", [True, False])
+@pytest.mark.parametrize("like", [0.02, 0.5])
+def test_many_long_rows(ops, like, proposed):
+    """Enough rows that the later places wait for the first ones' verdicts: sequences that go on past
+    them, that end among them, and that have fewer drafts."""
+    B, K, V = 72, 5, 49152
+    counts = [(b * 5) % (K + 1) for b in range(B)]
+    s = make(B, K, V, counts, seed=int(100 * like), temperature=0.9, top_k=0, like=like)
+    accepted = check(ops, s, 0.9, 0, proposed)
+    if proposed and like < 0.1:
+        assert (accepted >= 3).any()
+    s["cu"] = s["cu"].clone()
+    fault = torch.zeros(1, dtype=torch.int32, device="cuda")
+    s["drafts"] = s["drafts"].clone()
+    s["drafts"][5, 1] = V
+    got = verify(ops, s, 0.9, 0, s["draft_logits"] if proposed else None, fault)
+    want = by_definition(s["logits"], s["cu"], s["drafts"], s["accept_u"], s["next_u"], 0.9, 0,
+                         s["draft_logits"] if proposed else None)
+    rows = [b for b in range(B) if b != 5]
+    assert all(torch.equal(g.cpu()[rows], w[rows]) for g, w in zip(got, want))
+    assert int(fault.item()) in (0, 1) and int(got[0][5]) <= 1
+
+
 def test_a_draft_like_the_model_always_stands(ops):
     s = make(16, 4, 2048, [4] * 16, seed=3, temperature=0.7, top_k=0, like=0.0)
     accepted = check(ops, s, 0.7, 0)
