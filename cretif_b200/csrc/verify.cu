@@ -254,29 +254,32 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const __grid_constan
 // ---- second launch, whole vocabulary: a cluster a sequence, its CTAs share the vocabulary
 constexpr int kVdThreads = 512, kVdSeg = 128;             // entries a warp takes at once
 
-// 2^(i / 32)
-__device__ const double kVfTable[32] = {
-    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
-    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
-    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
-    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
-    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
-    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
-    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
-    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+// 2^(i / 16) and 2^(i / 256): their products are the table of 256 that a CTA makes for itself.
+__device__ const double kVfCoarse[16] = {
+    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
+    1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
+    1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+    1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474,
+};
+__device__ const double kVfFine[16] = {
+    1.0, 1.0027112750502025, 1.0054299011128027, 1.0081558981184175,
+    1.0108892860517005, 1.0136300849514894, 1.016378314910953, 1.019133996077738,
+    1.0218971486541166, 1.0246677928971357, 1.0274459491187637, 1.030231637686041,
+    1.0330248790212284, 1.0358256936019572, 1.0386341019613787, 1.041450124688316,
 };
 
-// A row's terms 2^((v - top) c) in 64 bits.  32 (v - top) c = n + f with |f| <= 1/2; 2^(n / 32) from a
-// table of 32 and a power of two, 2^(f / 32) by its series to the fifth power (the sixth term is below
-// 2.3e-15) (table-driven exponential, P. T. P. Tang, 1989).  Some 20 instructions, ten of them 64-bit.
+// A row's terms 2^((v - top) c) in 64 bits.  256 (v - top) c = n + f with |f| <= 1/2; 2^(n / 256) from the
+// table and a power of two, 2^(f / 256) by its series to the third power (the fourth term is below
+// 1.4e-13) (table-driven exponential, P. T. P. Tang, 1989).  What bounds the drawing is how many
+// instructions its warps issue: some 16 a term, eight of them 64-bit.
 struct VfTerm {
-  double c32, top;              // 32 log2 e / T, the row's maximum
+  double c256, top;             // 256 log2 e / T, the row's maximum
   float lo;                     // entries below it (2^-1000 of the largest) and NaN count 0
   bool infinite;                // the maximum is: entries equal to it count 1, all others 0
   __device__ __forceinline__ void set(float top_, double c, float reach) {       // reach: 1000 / c
     infinite = fabsf(top_) == INFINITY;
     top = top_;
-    c32 = 32.0 * c;
+    c256 = 256.0 * c;
     lo = top_;
     if (!infinite) {
       lo = top_ - reach;
@@ -284,22 +287,33 @@ struct VfTerm {
       while (lo < top_ && ((double)lo - (double)top_) * c < -1020.0) lo = nextafterf(lo, INFINITY);
     }
   }
+  __device__ __forceinline__ double plain(float v, const double* table) const {  // of an entry that is not below lo
+    const double magic = 6755399441055744.0;              // 1.5 * 2^52: rounds to an integer
+    const double d = (double)v - top;
+    const double big = fma(d, c256, magic);
+    const int n = __double2loint(big);
+    const double f = fma(d, c256, magic - big);
+    // (ln2 / 256)^k / k!
+    double p = fma(f, 3.308302680541371e-09, 3.665565596910106e-06);
+    p = fma(f, p, 0.0027076061740622863);
+    p = fma(f, p, 1.0);
+    p *= table[n & 255];
+    return __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
+  }
   __device__ __forceinline__ double operator()(float v, const double* table) const {
     if (infinite) return fmaxf(v, -INFINITY) == (float)top ? 1.0 : 0.0;
-    const double magic = 6755399441055744.0;              // 1.5 * 2^52: rounds to an integer
-    const double d = (double)fmaxf(v, lo) - top;
-    const double big = fma(d, c32, magic);
-    const int n = __double2loint(big);
-    const double f = fma(d, c32, magic - big);
-    // (ln2 / 32)^k / k!
-    double p = fma(f, 3.9737099845494154e-11, 9.172562701824643e-09);
-    p = fma(f, p, 1.6938509724371819e-06);
-    p = fma(f, p, 0.00023459619820224677);
-    p = fma(f, p, 0.02166084939249829);
-    p = fma(f, p, 1.0);
-    p *= table[n & 31];
-    const bool any = v >= lo;
-    return __hiloint2double(any ? __double2hiint(p) + ((n >> 5) << 20) : 0, any ? __double2loint(p) : 0);
+    return v >= lo ? plain(v, table) : 0.0;
+  }
+  // Four at once, by a whole warp.
+  __device__ __forceinline__ void four(const float (&v)[4], double (&to)[4], const double* table) const {
+    const bool all = v[0] >= lo && v[1] >= lo && v[2] >= lo && v[3] >= lo;
+    if (!infinite && __all_sync(0xffffffffu, all)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e] = plain(v[e], table);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e] = (*this)(v[e], table);
+    }
   }
 };
 
@@ -324,7 +338,7 @@ __global__ void __launch_bounds__(kVdThreads, 2)
 verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
   // sums of the CTA's segments; where they fit (cached) the terms of its share of both rows
   extern __shared__ __align__(16) double vd_smem[];
-  __shared__ double table[32];
+  __shared__ double table[256];
   __shared__ double sums[2 * kVdThreads / 32];
   __shared__ double shared_tot[4];                        // this CTA's: p and q, what is drawn from
   __shared__ double weight_s;
@@ -334,7 +348,7 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
   const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int kWarps = kVdThreads / 32;
-  if (tid < 32) table[tid] = kVfTable[tid];
+  if (tid < 256) table[tid] = kVfCoarse[tid >> 4] * kVfFine[tid & 15];
   if (tid == 0) first_bad = 0x7fffffff;
   dependent_begin();
   int row0, n;
@@ -437,8 +451,7 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
   auto look = [&](const VfTerm& row, const float* x, bool aligned, int s, double (&v)[4]) {
     float f[4];
     vf_four(x, a.V, s * 32 + lane, aligned, f);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = row(f[e], table);
+    row.four(f, v, table);
     if ((s + 1) * kVdSeg > a.V) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -468,8 +481,8 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
         if (s >= s1) break;
         double vp[4], vq[4];
         if (quick) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { vp[e] = tp(fp[x][e], table); vq[e] = tq(fq[x][e], table); }
+          tp.four(fp[x], vp, table);
+          tq.four(fq[x], vq, table);
         } else {
           look(tp, xp, ap, s, vp);
           look(tq, xq, aq, s, vq);
@@ -1015,9 +1028,10 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
     return launch_status();
   }
   launch_dependent(big ? verify_rows_kernel<12, false> : verify_rows_kernel<4, false>, grid, dim3(kVsThreads), 0, st, a);
-  // CTAs a sequence: enough to fill the chip about once, at least 1,024 entries each
+  // CTAs a sequence: as many as a cluster holds, 1,024 entries each at least.  (Four for 64 sequences, whose
+  // terms then do not fit beside one another and are computed twice: 61.6 us against 59.0.)
   int C = 8;
-  while (C > 1 && (B * C > 4 * kSmCount || V < 1024 * C)) C >>= 1;
+  while (C > 1 && V < 1024 * C) C >>= 1;
   const int segs = ((V + kVdSeg - 1) / kVdSeg + C - 1) / C + 1;
   // segments' sums, and before them the rows' numbers
   const long long room_ll = segs > 2LL * K + 1 ? segs : 2LL * K + 1;
