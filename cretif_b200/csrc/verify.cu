@@ -1041,8 +1041,16 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
   const int cached = a.draft_logits && (size_t)segs * kVdSeg * 16 <= 100 * 1024;
   const size_t smem = (size_t)room * 8 + (cached ? (size_t)segs * kVdSeg * 16 : 0);
   if (smem > 200 * 1024) return kBadArgument;
-  cudaError_t e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
+  constexpr int kDevices = 64;
+  static size_t limit[kDevices];                          // (asked for once a device)
+  if (dev >= kDevices || smem > limit[dev < kDevices ? dev : 0]) {
+    e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < kDevices) limit[dev] = smem;
+  }
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = C * B <= kSmCount ? dependent_launch_enabled() : 0;
