@@ -1,7 +1,9 @@
 """Bookkeeping of cache storage: a pool of fixed-size token blocks and a set of slots.
 
 Both are plain host-side allocators with strict checks: nothing can be handed
-out twice, given back twice, or lost.  The reference has one sequence and one
+out twice, given back more often than it is held, or lost.  A block may have several
+holders (sequences that share their first tokens); it is free again when the last gives
+it back.  The reference has one sequence and one
 length counter (src/kv_cache.cu:201-212) and "frees" by resetting that counter
 (:237-243); with many sequences the storage has to be accounted for explicitly.
 """
@@ -26,7 +28,8 @@ class BlockPool:
             raise ValueError("a block pool needs at least one block")
         self.n_blocks = n_blocks
         self._free: List[int] = list(range(n_blocks - 1, -1, -1))  # pop() gives the lowest
-        self._held = [False] * n_blocks
+        self._holders = [0] * n_blocks
+        self.shared_count = 0                     # holders beyond the first, of all blocks
 
     @property
     def free_count(self) -> int:
@@ -44,21 +47,39 @@ class BlockPool:
                             f"{self.n_blocks} are free")
         out = [self._free.pop() for _ in range(n)]
         for b in out:
-            self._held[b] = True
+            self._holders[b] = 1
         return out
+
+    def holders(self, block: int) -> int:
+        return self._holders[block]
+
+    def share(self, blocks) -> None:
+        """One more holder for each of ``blocks``, which are held."""
+        blocks = list(blocks)
+        for b in blocks:
+            if not 0 <= b < self.n_blocks or not self._holders[b]:
+                raise CacheError(f"block {b} is not held and cannot be shared")
+        for b in blocks:
+            self._holders[b] += 1
+        self.shared_count += len(blocks)
 
     def give_back(self, blocks) -> None:
         blocks = list(blocks)
         for b in blocks:
             if not 0 <= b < self.n_blocks:
                 raise CacheError(f"block {b} does not belong to this pool")
-            if not self._held[b]:
+            if not self._holders[b]:
                 raise CacheError(f"block {b} is given back but is not held")
         if len(set(blocks)) != len(blocks):
             raise CacheError("a block is given back twice in one call")
+        gone = []
         for b in blocks:
-            self._held[b] = False
-        self._free.extend(sorted(blocks, reverse=True))
+            self._holders[b] -= 1
+            if self._holders[b]:
+                self.shared_count -= 1
+            else:
+                gone.append(b)
+        self._free.extend(gone)
         self._free.sort(reverse=True)
 
     def check(self) -> None:
@@ -67,7 +88,7 @@ class BlockPool:
         if len(free) != len(self._free):
             raise CacheError("a block is on the free list twice")
         for b in range(self.n_blocks):
-            if self._held[b] == (b in free):
+            if (self._holders[b] > 0) == (b in free):
                 raise CacheError(f"block {b} is {'both held and free' if b in free else 'lost'}")
 
 

@@ -151,6 +151,64 @@ class _KVGroup:
         self.n_blocks_of[slot] = 0
         self.dirty.add(slot)
 
+    def fork_needs(self, length: int) -> int:
+        """Blocks that a sequence sharing one of ``length`` tokens needs for itself: the last one, if
+        it is not full."""
+        return 1 if (length // self.tokens_per_entry) % self.block_tokens else 0
+
+    def fork(self, slot: int, new: List[int], length: int) -> None:
+        """Give the ``new`` slots ``slot``'s full blocks, and a copy each of its last one if that is
+        not full."""
+        full, part = divmod(length // self.tokens_per_entry, self.block_tokens)
+        lo = int(self.first_block[slot])
+        shared = self.table_host[slot, lo:full].tolist()
+        copies = self.pool.take(len(new)) if part else []
+        for i, s in enumerate(new):
+            self.pool.share(shared)
+            self.table_host[s, :] = -1
+            self.table_host[s, lo:full] = shared
+            self.first_block[s] = lo
+            self.n_blocks_of[s] = full
+            if part:
+                self.table_host[s, full] = copies[i]
+                self.n_blocks_of[s] = full + 1
+            self.dirty.add(s)
+        if part:
+            self.copy_block(int(self.table_host[slot, full]), copies)
+
+    def copy_block(self, src: int, dst: List[int]) -> None:
+        """Block ``src``'s entries of every layer into the blocks ``dst``."""
+        at = torch.as_tensor(dst, dtype=torch.int64)
+        if self.k.device.type == "cuda":
+            at = at.pin_memory().to(self.k.device, non_blocking=True)
+        for t in (self.k,) if self.v is self.k else (self.k, self.v):
+            t.index_copy_(1, at, t[:, src:src + 1].repeat(1, len(dst), 1, 1, 1))
+
+    def truncate_needs(self, slot: int, length: int) -> int:
+        """Blocks that cutting ``slot`` to ``length`` tokens takes: its last block is copied if other
+        sequences hold it too, since it will be written again."""
+        at = length // self.block_tokens
+        return 1 if length % self.block_tokens and self.pool.holders(int(self.table_host[slot, at])) > 1 else 0
+
+    def truncate(self, slot: int, length: int) -> None:
+        """Cut ``slot`` to ``length`` tokens.  Blocks behind stay mapped for the tokens to come, unless
+        another sequence holds one of them."""
+        at, keep = length // self.block_tokens, -(-length // self.block_tokens)
+        mapped = self.table_host[slot, at:int(self.n_blocks_of[slot])].tolist()
+        if not any(self.pool.holders(b) > 1 for b in mapped):
+            return
+        if keep > at and self.pool.holders(mapped[0]) > 1:
+            own = self.pool.take(1)
+            self.copy_block(mapped[0], own)
+            self.pool.give_back([mapped[0]])
+            self.table_host[slot, at] = own[0]
+        behind = mapped[keep - at:]
+        if behind:
+            self.pool.give_back(behind)
+            self.table_host[slot, keep:int(self.n_blocks_of[slot])] = -1
+            self.n_blocks_of[slot] = keep
+        self.dirty.add(slot)
+
     def flush(self) -> None:
         if not self.dirty:
             return
@@ -255,6 +313,76 @@ class SequenceCache:
         if not self.slots.is_live(slot):
             raise CacheError(f"slot {slot} is not in use")
         return int(self.lengths[slot])
+
+    # -- sequences that share their first tokens -----------------------------------
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """``n`` new slots that continue ``slot`` from where it is: its full blocks are held in common,
+        a last block that is not full, and the fixed-size states, are copied.  All or nothing."""
+        length = self.length(slot)
+        if n < 1:
+            raise ValueError(f"cannot fork a sequence {n} times")
+        if n > self.slots.free_count:
+            raise CacheFull(f"need {n} sequence slots, only {self.slots.free_count} of "
+                            f"{self.max_slots} are free")
+        for g in self._kv_groups:
+            if n * g.fork_needs(length) > g.pool.free_count:
+                raise CacheFull(f"forking slot {slot} {n} times needs {n} more cache blocks, only "
+                                f"{g.pool.free_count} of {g.pool.n_blocks} are free")
+        new = [self.slots.take() for _ in range(n)]
+        for g in self._kv_groups:
+            g.fork(slot, new, length)
+            g.flush()
+        self.lengths[new] = length
+        if self._state:
+            at = torch.as_tensor(new, dtype=torch.int64)
+            if self.device.type == "cuda":
+                at = at.pin_memory().to(self.device, non_blocking=True)
+            for t in self._state.values():
+                t.index_copy_(0, at, t[slot:slot + 1].repeat(n, *[1] * (t.dim() - 1)))
+        return new
+
+    def truncate(self, slot: int, length: int) -> None:
+        """Cut a sequence to its first ``length`` tokens (rejected drafts).  Refused, with nothing
+        changed, where the past cannot come back: a model that keeps states or pooled entries, or a
+        window whose keys before ``length`` have been given back."""
+        now = self.length(slot)
+        if not 0 <= length <= now:
+            raise CacheError(f"slot {slot} has {now} tokens and cannot be cut to {length}")
+        if length == now:
+            return
+        if self._state or self._pool_of:
+            raise CacheError("a model that keeps states or pooled entries cannot go back")
+        for g in self._kv_groups:
+            w = g.request.window
+            if w > 0 and int(g.first_block[slot]) * self.block_tokens > max(0, length - w + 1):
+                raise CacheError(f"slot {slot}: keys of the window before {length} tokens have been "
+                                 "given back")
+            if g.truncate_needs(slot, length) > g.pool.free_count:
+                raise CacheFull("no cache block is free for the last block of the cut sequence")
+        for g in self._kv_groups:
+            g.truncate(slot, length)
+            g.flush()
+        self.lengths[slot] = length
+
+    def shared_groups(self, slots: Sequence[int]) -> List[Tuple[List[int], int]]:
+        """Which of ``slots`` (by their places in the list) have first blocks in common, and how many
+        tokens those hold: what the attention over shared prefixes is planned for.  Sequences that
+        share more among some of them than all do count with what all do."""
+        g = next((g for g in self._kv_groups if g.request.window == 0 and g.tokens_per_entry == 1
+                  and g.pool.shared_count), None)
+        if g is None or len(slots) < 2:
+            return []
+        rows = g.table_host[np.asarray(slots, dtype=np.int64)]
+        first = rows[:, 0]
+        out = []
+        for blk in np.unique(first[first >= 0]):
+            members = np.flatnonzero(first == blk)
+            if members.size < 2:
+                continue
+            alike = (rows[members] == rows[members[0]]).all(axis=0) & (rows[members[0]] >= 0)
+            n = int(alike.size if alike.all() else np.argmin(alike))
+            out.append((members.tolist(), n * self.block_tokens))
+        return out
 
     # -- a step ----------------------------------------------------------------
     def begin_step(self, entries: Sequence[Tuple[int, int]]) -> None:
@@ -366,7 +494,7 @@ class SequenceCache:
         }
 
     def check(self) -> None:
-        """Every block is free or mapped by exactly one live slot; no slot is lost."""
+        """Every block is free or mapped by as many live slots as hold it; no slot is lost."""
         self.slots.check()
         for g in self._kv_groups:
             g.pool.check()
@@ -377,7 +505,9 @@ class SequenceCache:
                 if held and not self.slots.is_live(s):
                     raise CacheError(f"free slot {s} still maps blocks {held}")
                 mapped.extend(held)
-            if len(set(mapped)) != len(mapped):
-                raise CacheError("a block is mapped by two sequences")
-            if len(mapped) != g.pool.held_count:
-                raise CacheError(f"{g.pool.held_count} blocks are held but {len(mapped)} are mapped")
+            for b in set(mapped):
+                if mapped.count(b) != g.pool.holders(b):
+                    raise CacheError(f"block {b} is mapped by {mapped.count(b)} sequences and held by "
+                                     f"{g.pool.holders(b)}")
+            if len(set(mapped)) != g.pool.held_count:
+                raise CacheError(f"{g.pool.held_count} blocks are held but {len(set(mapped))} are mapped")

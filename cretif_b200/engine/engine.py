@@ -144,6 +144,10 @@ def require_cuda(device) -> torch.device:
     return dev
 
 
+# Steps in which no sequence brings more tokens than this may take the attention over shared prefixes
+# (a last token and its drafts); longer ones are prompts.
+SHARED_MAX_NEW = 16
+
 Entry = Tuple[int, Sequence[int]]
 
 
@@ -197,6 +201,17 @@ class Engine:
     def free_slot(self, slot: int) -> None:
         self.cache.free_slot(slot)
 
+    def fork_slot(self, slot: int, n: int = 1) -> list:
+        """``n`` new slots that continue ``slot`` from where it is: several answers to one prompt, which
+        lies in the cache once.  Steps of few tokens a sequence read what such slots share once for
+        all of them (bfloat16, attention without a window)."""
+        return self.cache.fork(slot, n)
+
+    def truncate_slot(self, slot: int, length: int) -> None:
+        """Take ``slot`` back to its first ``length`` tokens: the drafts that did not stand.  Models
+        with recurrent states or pooled entries cannot."""
+        self.cache.truncate(slot, length)
+
     # -- the step ------------------------------------------------------------------
     def context_bucket(self, context: int) -> int:
         """The context length a decode step is planned for: the next power of two (from 512)
@@ -218,6 +233,15 @@ class Engine:
             seq_start=seq_start, cu_seqlens=cu_seqlens, is_decode=is_decode, max_new=max_new,
             max_context=max_context, fault=self.fault, dtype=self.dtype, device=self.device,
             seq_slot_host=tuple(slots), seq_start_host=tuple(starts), seq_new_host=tuple(news))
+
+    def shared_prefixes(self, slots, starts, news):
+        """What the attention of a step may read once for several sequences: (groups, tokens a sequence
+        brings, cached tokens), or None.  Only for bfloat16: in float32 a token's bits do not depend on
+        the rest of its step."""
+        if self.dtype != torch.bfloat16 or max(news) > SHARED_MAX_NEW:
+            return None
+        groups = self.cache.shared_groups(slots)
+        return (groups, tuple(int(n) for n in news), tuple(int(s) for s in starts)) if groups else None
 
     def run(self, pairs, launch):
         """The one way a step runs: the cache makes room for ``pairs`` (slot, new tokens),
@@ -282,6 +306,9 @@ class Engine:
             max_new=int(new.max()), max_context=int((starts + new).max()), slots=slots,
             starts=(int(s) for s in starts), news=(int(n) for n in new))
         want_rows = take(rows.size)
+        shared = self.shared_prefixes(slots, ctx.seq_start_host, ctx.seq_new_host)
+        if shared is not None:
+            ctx.extras["shared"] = shared
         return ctx, want_rows, int(rows.size)
 
     def step(self, entries: Sequence[Entry], want: Union[str, Sequence[Sequence[int]]] = "last",
@@ -325,6 +352,14 @@ class Engine:
         if sum(news) > self.graph_max_tokens:
             return None
         w = want if isinstance(want, str) else tuple(tuple(int(i) for i in x) for x in want)
+        if not news or min(news) < 1:
+            return None                               # (refused by make_context)
+        slots = [int(s) for s, _ in entries]
+        shared = None
+        if all(self.cache.slots.is_live(s) for s in slots):
+            shared = self.shared_prefixes(slots, [0] * len(slots), news)
+        if shared is not None:
+            w = (w, tuple((tuple(m), p) for m, p in shared[0]))
         bucket = 0
         if all(n == 1 for n in news):
             longest = max((int(self.cache.lengths[int(s)]) for s, _ in entries), default=0) + 1
@@ -348,6 +383,12 @@ class Engine:
             self.cache.lengths[s] -= n              # as they were when the step began
         try:
             ctx, want_rows, _ = self.make_context(entries, want, meta=meta)
+            # (the step that ran made its plans: a capture copies nothing to the device)
+            if "shared" in ran.extras:
+                ctx.extras["shared"] = ran.extras["shared"]
+                ctx.extras["shared_plans"] = ran.extras.get("shared_plans", {})
+            else:
+                ctx.extras.pop("shared", None)
         finally:
             for s, n in saved.items():
                 self.cache.lengths[s] = n
@@ -358,7 +399,8 @@ class Engine:
             with capturing(graph, self._graph_pool, self._graph_stream):
                 logits = self.model.forward(ctx, self.cache, None if all_rows else want_rows)
         cur.wait_stream(self._graph_stream)
-        self._graphs[key] = {"graph": graph, "meta": meta, "logits": logits}
+        self._graphs[key] = {"graph": graph, "meta": meta, "logits": logits,
+                             "plans": ctx.extras.get("shared_plans")}
         while len(self._graphs) > self.max_step_graphs:
             self._graphs.popitem(last=False)
 

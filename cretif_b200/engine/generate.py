@@ -34,6 +34,7 @@ class GenerationResult:
     finish_reason: Optional[str] = None        # "stop" or "length"
 
 
+MAX_SHARED_GRAPHS = 8   # decode graphs kept of batches that share prefixes
 MAX_BACKENDS = 4      # sets of decode graphs kept per engine (one per temperature / top_k)
 
 
@@ -142,6 +143,8 @@ class DecodeRunner:
         use_graph = use_graph and engine.model.graph_safe
         self.engine, self.sampler, self.use_graph = engine, sampler, use_graph
         self.graphs: Dict[tuple, torch.cuda.CUDAGraph] = {}
+        self.plans: Dict[tuple, dict] = {}        # of batches that share prefixes, by what they share
+        self.shared = None
         self.bufs: Dict[int, dict] = {}
         self.stream = torch.cuda.Stream(device=engine.device)
         self.pool = torch.cuda.graph_pool_handle() if use_graph else None
@@ -170,6 +173,12 @@ class DecodeRunner:
         b["request"].copy_(torch.from_numpy(np.asarray(requests, dtype=np.int64)).pin_memory(),
                            non_blocking=True)
         self.B = B
+        self.shared = self.engine.shared_prefixes([int(s) for s in slots], [int(p) for p in positions], [1] * B)
+        if len(self.plans) > 64:                   # (of batches long gone; graphs keep their own)
+            self.plans.clear()
+
+    def _shared_key(self) -> tuple:
+        return () if self.shared is None else tuple((tuple(m), p) for m, p in self.shared[0])
 
     def _body(self, b: dict, B: int, context: int) -> None:
         eng = self.engine
@@ -177,6 +186,9 @@ class DecodeRunner:
                           tok_seq=b["tok_seq"], seq_slot=b["seq_slot"],
                           seq_start=b["seq_start"], cu_seqlens=b["cu"], is_decode=True,
                           max_new=1, max_context=context)
+        if self.shared is not None:
+            ctx.extras["shared"] = self.shared
+            ctx.extras["shared_plans"] = self.plans.setdefault((B,) + self._shared_key(), {})
         logits = eng.model.forward(ctx, eng.cache, None)
         b["logits"] = logits
         self.sampler(logits, b["sampled"], b["request"], b["draw"])
@@ -190,7 +202,7 @@ class DecodeRunner:
         if not self.use_graph:
             self._body(b, B, context)
             return b["sampled"]
-        key = (B, self.engine.context_bucket(context))
+        key = (B, self.engine.context_bucket(context), self._shared_key())
         if key not in self.graphs:
             # Warm up outside the capture (lazy initialisation, kernel loading), restoring
             # the state the warm-up advanced, then capture.
@@ -212,8 +224,11 @@ class DecodeRunner:
                     self._body(b, B, context)
             cur.wait_stream(self.stream)
             b["ints"].copy_(saved)
-            self.graphs[key] = g
-        self.graphs[key].replay()
+            self.graphs[key] = (g, dict(self.plans.get((B,) + self._shared_key(), {})))
+            shared = [k for k in self.graphs if k[2]]
+            if len(shared) > MAX_SHARED_GRAPHS:    # (what batches share seldom comes again)
+                del self.graphs[shared[0]]
+        self.graphs[key][0].replay()
         return b["sampled"]
 
 

@@ -107,6 +107,33 @@ def distance_edges(rows: int, far: float):
 FAST_BIAS_MAX_DISTANCES = 4096
 
 
+# A step of single tokens takes the attention over shared prefixes where that spares this much reading, or
+# where the prefix is this long: below, two launches and the joining cost more than the keys (ordinary decode
+# attention against shared, us: 9 heads on 3, 8 sequences on 2,048 tokens (11 MB) 6.9 / 7.8, 32 on 1,024 (24 MB)
+# 8.5 / 7.9; 32 on 32, 2 on 2,048 (17 MB) 9.7 / 9.8, 8 on 2,048 (117 MB) 26.2 / 10.6; 9 on 3, 2 on 8,192 (6 MB)
+# 15.2 / 9.8).  A step with drafts always takes it (4 tokens each, 8 sequences on 2,048 tokens: prompt attention
+# 22.9 / 10.2; on 64 tokens 5.9 / 4.4).
+SHARED_MIN_BYTES = 16 << 20
+SHARED_LONG = 4096
+
+
+def shared_plan(ctx, nh: int, nkv: int, hd: int, dtype):
+    """The step's plan for :func:`ops.attn_shared`, made once for layers of these sizes; None where the
+    step shares nothing that is worth it."""
+    shared = ctx.extras.get("shared")
+    if shared is None:
+        return None
+    plans = ctx.extras.setdefault("shared_plans", {})
+    key = (nh, nkv, hd)
+    if key not in plans:
+        groups, news, starts = shared
+        spared = sum((len(m) - 1) * p for m, p in groups) * nkv * hd * 4
+        plans[key] = None
+        if max(news) > 1 or spared >= SHARED_MIN_BYTES or max(p for _, p in groups) >= SHARED_LONG:
+            plans[key] = ops.shared_prefix_plan(groups, news, starts, nh, nkv, hd, dtype, ctx.device)
+    return plans[key]
+
+
 def run_attention(q, o, ctx, kv, nh, nkv, hd, scale, window, dtype, sink=None, vd=0, bias=None,
                   bias_edges=None, bias_dense=None, slope=None, slope_log2e=None, pool=None):
     """Causal (windowed) attention of the step's queries ``q`` [T, nh·hd] over the cache view
@@ -131,6 +158,14 @@ def run_attention(q, o, ctx, kv, nh, nkv, hd, scale, window, dtype, sink=None, v
     # what a decode step's keys are shared out by: with pooled entries, the keys it really reads
     context = ctx.max_context if pool is None else min(
         ctx.max_context, window + 64 + ctx.max_context // pool.pool)
+    if (fast and window == 0 and kv.window == 0 and bias is None and slope is None and pool is None
+            and hd <= 128 and hd % 16 == 0 and kv.block_tokens == 64 and q.stride(0) % 8 == 0
+            and q.data_ptr() % 16 == 0):
+        plan = shared_plan(ctx, nh, nkv, hd, dtype)
+        if plan is not None:
+            ops.attn_shared(q, o, kv.k, kv.v, kv.table, ctx.tok_pos, ctx.cu_seqlens, ctx.seq_slot, plan,
+                            scale, kv.block_tokens, ctx.fault, sink=sink)
+            return
     if fast:
         if ctx.is_decode and ops.attn_decode_supported(hd, kv.block_tokens, min(nh // nkv, 8)) \
                 and (nh // nkv <= 8 or nkv == 1):
