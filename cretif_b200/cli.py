@@ -68,6 +68,8 @@ def main(argv=None) -> int:
     ap.add_argument("--preset", default=None,
                     help="named configuration to use with --random-weights (tiny-a, tiny-b, "
                          "smollm2-135m, smollm2-360m, smollm2-1.7b)")
+    ap.add_argument("--samples", type=int, default=1,
+                    help="answers to the prompt, which is run once for all of them (default 1)")
     ap.add_argument("--stop-ids", default=None,
                     help="comma-separated token ids that end generation (default: the model's "
                          "eos_token_id)")
@@ -129,15 +131,16 @@ def main(argv=None) -> int:
     torch.cuda.synchronize()
     t0 = time.time()
     stops = None if args.stop_ids is None else [int(t) for t in args.stop_ids.split(",") if t]
-    res = engine.generate([ids], max_tokens=args.max_tokens, temperature=args.temperature,
-                          top_k=args.top_k, seed=args.seed, stop_ids=stops)[0]
+    answers = engine.generate([ids], max_tokens=args.max_tokens, temperature=args.temperature,
+                              top_k=args.top_k, seed=args.seed, stop_ids=stops, samples=args.samples)
     torch.cuda.synchronize()
     dt = time.time() - t0
     print(f"prompt ids: {ids}")
-    print(f"generated ids: {res.tokens}  (finish: {res.finish_reason})")
-    if tokenizer is not None:
-        print(tokenizer.decode(res.tokens))
-    total = len(ids) + len(res.tokens) - 1          # as src/main.cu:317-324 counts
+    for res in answers:
+        print(f"generated ids: {res.tokens}  (finish: {res.finish_reason})")
+        if tokenizer is not None:
+            print(tokenizer.decode(res.tokens))
+    total = len(ids) + sum(len(r.tokens) - 1 for r in answers)   # as src/main.cu:317-324 counts
     print(f"{total} tokens in {dt * 1e3:.1f} ms: {total / dt:.1f} tok/s")
     return 0
 

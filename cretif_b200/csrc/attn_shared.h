@@ -17,7 +17,7 @@ constexpr int kShBlk = 64;                 // tokens of a cache block
 
 // A range of blocks of a group's prefix for some of the group's rows.  Row r of a key/value head is
 // query head kvh * g + r % g of token rows[row_base + r / g].
-struct SharedPrefixItem {
+struct alignas(16) SharedPrefixItem {
   int row_base, row0, n_rows;
   int seq;                                 // a member: its table is read
   int blk0, blk1;                          // blocks [blk0, blk1)
@@ -25,7 +25,7 @@ struct SharedPrefixItem {
   int pad;
 };
 // Some rows of one sequence over its own keys: row r is head kvh * g + r % g of token tok0 + r / g.
-struct SharedOwnItem {
+struct alignas(16) SharedOwnItem {
   int seq, tok0, row0, n_rows;
   int prefix, pieces;                      // tokens that are other items' work, and pieces they are in
   int least;                               // the least position of the sequence: the tokens it shares
@@ -56,10 +56,12 @@ struct SharedArgs {
 };
 
 // The physical block at place `at` of a slot's table; 0 and a fault bit where there is none.
+// (What the step's earlier kernels and copies wrote is read from L2 here: the own keys' kernel starts under the
+// prefix kernel and has no wait of its own in front.)
 __device__ __forceinline__ int shared_block_of(const SharedArgs& a, int slot, int at) {
   int blk = -1;
   if (slot >= 0 && slot < a.n_slots && at >= 0 && at < a.table_stride)
-    blk = a.table[(size_t)slot * a.table_stride + at];
+    blk = __ldcg(a.table + (size_t)slot * a.table_stride + at);
   if (blk < 0 || blk >= a.n_blocks) {
     atomicOr(a.fault, (unsigned)kFaultBlockTable);
     blk = 0;
@@ -67,7 +69,7 @@ __device__ __forceinline__ int shared_block_of(const SharedArgs& a, int slot, in
   return blk;
 }
 __device__ __forceinline__ int shared_block(const SharedArgs& a, int seq, int at) {
-  return shared_block_of(a, a.seq_slot[seq], at);
+  return shared_block_of(a, __ldcg(a.seq_slot + seq), at);
 }
 
 // One past the last own key that an item's row at position `last` sees.  A position inside the shared

@@ -439,7 +439,12 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   const int which = JOIN ? index : index / a.own_splits;
   const bool none = which >= a.n_own;                     // (a warp of its own: WPI is 1)
   // (the plan is never written by a kernel)
-  const SharedOwnItem it = a.own[none ? 0 : which];
+  SharedOwnItem it;
+  {
+    const int4* from = reinterpret_cast<const int4*>(a.own + (none ? 0 : which));
+    *reinterpret_cast<int4*>(&it.seq) = __ldcg(from);
+    *reinterpret_cast<int4*>(&it.prefix) = __ldcg(from + 1);
+  }
   constexpr int kRing = kSoStages * kSoStage<HDG, KEYS>;
   unsigned char* ring = smem + cta_warp * kRing;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kSoWarps * kRing) + cta_warp * kSoStages;
@@ -460,8 +465,8 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     return;
   }
   const int prefix = it.prefix, blk0 = prefix / kShBlk;
-  const int slot = a.seq_slot[it.seq];
-  const int last = a.tok_pos[it.tok0 + (it.row0 + it.n_rows - 1) / g];
+  const int slot = __ldcg(a.seq_slot + it.seq);
+  const int last = __ldcg(a.tok_pos + it.tok0 + (it.row0 + it.n_rows - 1) / g);
   const int end = shared_own_end(a, it, last);
   // KEYS keys a warp and step: keys KEYS i .. of the own ones, i = first, first + stride, ...
   const int first = split * WPI + warp, stride = splits * WPI;
@@ -496,14 +501,14 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int row = r + 8 * i, rr = it.row0 + row;
     const bool there = row < it.n_rows;
     const int t = it.tok0 + (there ? rr / g : 0);
-    pos[i] = there ? a.tok_pos[t] : -1;
+    pos[i] = there ? __ldcg(a.tok_pos + t) : -1;
     const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.ldq +
                                (size_t)(kvh * g + (there ? rr % g : 0)) * hd;
 #pragma unroll
     for (int d = 0; d < HDG * 4; ++d) {
       const bool in = there && 16 * d < hd;
-      qa[d][i][0] = in ? *reinterpret_cast<const uint32_t*>(src + 16 * d + 2 * c) : 0u;
-      qa[d][i][1] = in ? *reinterpret_cast<const uint32_t*>(src + 16 * d + 8 + 2 * c) : 0u;
+      qa[d][i][0] = in ? __ldcg(reinterpret_cast<const uint32_t*>(src + 16 * d + 2 * c)) : 0u;
+      qa[d][i][1] = in ? __ldcg(reinterpret_cast<const uint32_t*>(src + 16 * d + 8 + 2 * c)) : 0u;
     }
   }
   float o[HDG * 8][2 * NR];                               // [8 channels][row: 2c, 2c + 1]

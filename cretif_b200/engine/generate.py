@@ -62,8 +62,12 @@ class GenerationLoop:
     def _rounded(self, n: int) -> int:
         return -(-n // self.block_tokens) * self.block_tokens
 
-    def plan_batches(self, prompt_lens: Sequence[int], max_tokens: int) -> List[List[int]]:
-        """Cut request indices, in order, into batches the cache can hold."""
+    def plan_batches(self, prompt_lens: Sequence[int], max_tokens: int, samples: int = 1) -> List[List[int]]:
+        """Cut request indices, in order, into batches the cache can hold.  ``samples`` requests a
+        prompt, one after the other: they start together, and hold the prompt's full blocks once."""
+        if not 1 <= samples <= self.max_batch:
+            raise ValueError(f"{samples} answers a prompt: from 1 up to the {self.max_batch} sequences that "
+                             "may start together")
         batches: List[List[int]] = []
         cur: List[int] = []
         used = 0
@@ -73,27 +77,31 @@ class GenerationLoop:
             if n > self.max_len:
                 raise ValueError(f"request {i}: the prompt has {n} tokens, the longest "
                                  f"sequence allowed is {self.max_len}")
-            need = self._rounded(self._reserve_len(n, max_tokens))
+            whole = self._rounded(self._reserve_len(n, max_tokens))
+            need = whole + (samples - 1) * (whole - n // self.block_tokens * self.block_tokens)
             if need > self.capacity_tokens:
                 raise ValueError(f"request {i} needs {need} cache tokens, the cache holds "
                                  f"{self.capacity_tokens}")
-            if cur and (len(cur) >= self.max_batch or used + need > self.capacity_tokens):
+            if cur and (len(cur) + samples > self.max_batch or used + need > self.capacity_tokens):
                 batches.append(cur)
                 cur, used = [], 0
-            cur.append(i)
+            cur.extend(range(i * samples, (i + 1) * samples))
             used += need
         if cur:
             batches.append(cur)
         return batches
 
-    def run(self, prompts: Sequence[Sequence[int]], max_tokens: int) -> List[GenerationResult]:
+    def run(self, prompts: Sequence[Sequence[int]], max_tokens: int, samples: int = 1) -> List[GenerationResult]:
+        """The results of every prompt, ``samples`` of them one after the other."""
+        batches = self.plan_batches([len(p) for p in prompts], max_tokens, samples) if max_tokens > 0 else []
+        prompts = [p for p in prompts for _ in range(samples)]
         results = [GenerationResult(prompt_len=len(p)) for p in prompts]
         if max_tokens <= 0:
             for r in results:
                 r.finish_reason = "length"
             return results
-        for batch in self.plan_batches([len(p) for p in prompts], max_tokens):
-            self._run_batch(batch, prompts, max_tokens, results)
+        for batch in batches:
+            self._run_batch(batch, prompts, max_tokens, results, samples)
         return results
 
     def _record(self, res: GenerationResult, token: int, max_tokens: int) -> bool:
@@ -107,10 +115,11 @@ class GenerationLoop:
             res.finish_reason = "length"       # no room to feed this token back
         return res.finish_reason is not None
 
-    def _run_batch(self, batch, prompts, max_tokens, results) -> None:
+    def _run_batch(self, batch, prompts, max_tokens, results, samples: int = 1) -> None:
         be = self.backend
         reserve = [self._reserve_len(len(prompts[i]), max_tokens) for i in batch]
-        be.start_batch(batch, [prompts[i] for i in batch], reserve)
+        more = () if samples == 1 else (samples,)
+        be.start_batch(batch, [prompts[i] for i in batch], reserve, *more)
         try:
             first = be.prefill()
             active: List[int] = []
@@ -257,8 +266,10 @@ class EngineBackend:
         self._ready: List[Dict[int, int]] = []    # finished and read, not yet handed out
         self._to_free: List[int] = []
 
-    def start_batch(self, request_ids, prompts, reserve_lens) -> None:
+    def start_batch(self, request_ids, prompts, reserve_lens, samples: int = 1) -> None:
+        """``samples`` requests a prompt: the first of them runs it, the others continue from there."""
         eng = self.engine
+        self.samples = samples
         self.request_ids = list(request_ids)
         self.prompts = [list(p) for p in prompts]
         self.reserve = [int(n) for n in reserve_lens]
@@ -271,9 +282,12 @@ class EngineBackend:
         self._host_at = 0
         try:
             for i, n in enumerate(reserve_lens):
+                if i % samples:                                  # (forked behind the prompt)
+                    self.slots.append(None)
+                    continue
                 s = eng.alloc_slot()
                 self.slots.append(s)
-                eng.cache.reserve(s, n, flush=i + 1 == len(reserve_lens))   # one copy for all
+                eng.cache.reserve(s, n, flush=i + samples >= len(reserve_lens))   # one copy for all
         except Exception:
             self.end_batch()
             raise
@@ -283,8 +297,15 @@ class EngineBackend:
 
     def prefill(self) -> List[int]:
         eng = self.engine
-        logits = eng.step(list(zip(self.slots, self.prompts)), "last", check=False)
+        n = self.samples
+        logits = eng.step(list(zip(self.slots[::n], self.prompts[::n])), "last", check=False)
         B = len(self.slots)
+        if n > 1:
+            logits = logits.repeat_interleave(n, dim=0)
+            for first in range(0, B, n):
+                self.slots[first + 1:first + n] = eng.fork_slot(self.slots[first], n - 1)
+            for i in range(B):
+                eng.cache.reserve(self.slots[i], self.reserve[i], flush=i + 1 == B)
         out = torch.empty(B, dtype=torch.int32, device=eng.device)
         req = torch.from_numpy(np.asarray(self.request_ids, dtype=np.int64)).pin_memory().to(
             eng.device, non_blocking=True)
@@ -394,8 +415,10 @@ class EngineBackend:
 def generate(engine, prompts: Sequence[Sequence[int]], max_tokens: int = 100,
              temperature: float = 0.0, top_k: int = 0, seed: int = 42,
              stop_ids: Optional[Iterable[int]] = None, max_batch: int = 64,
-             use_graph: bool = True) -> List[GenerationResult]:
-    """Generate up to ``max_tokens`` tokens for every prompt (lists of token ids).
+             use_graph: bool = True, samples: int = 1) -> List[GenerationResult]:
+    """Generate up to ``max_tokens`` tokens for every prompt (lists of token ids), ``samples`` answers
+    to each (results one prompt after the other): the prompt is run once, its full cache blocks are held
+    in common, and each answer has random numbers of its own.
 
     Option names and defaults are the reference's (``generate(prompt, max_tokens=100,
     temperature=0, top_k=0)``, include/cuinfer/model.h:116-119); ``stop_ids`` defaults
@@ -415,4 +438,4 @@ def generate(engine, prompts: Sequence[Sequence[int]], max_tokens: int = 100,
     backends[key].sampler.set_seed(params.seed)
     loop = GenerationLoop(backends[key], stops, engine.cache.max_tokens, engine.cache.max_len,
                           engine.cache.block_tokens, max_batch)
-    return loop.run(prompts, max_tokens)
+    return loop.run(prompts, max_tokens, samples)

@@ -120,13 +120,10 @@ SHARED_LONG = 4096
 def shared_plan(ctx, nh: int, nkv: int, hd: int, dtype):
     """The step's plan for :func:`ops.attn_shared`, made once for layers of these sizes; None where the
     step shares nothing that is worth it."""
-    shared = ctx.extras.get("shared")
-    if shared is None:
-        return None
     plans = ctx.extras.setdefault("shared_plans", {})
     key = (nh, nkv, hd)
     if key not in plans:
-        groups, news, starts = shared
+        groups, news, starts = ctx.extras["shared"]
         spared = sum((len(m) - 1) * p for m, p in groups) * nkv * hd * 4
         plans[key] = None
         if max(news) > 1 or spared >= SHARED_MIN_BYTES or max(p for _, p in groups) >= SHARED_LONG:
@@ -158,7 +155,7 @@ def run_attention(q, o, ctx, kv, nh, nkv, hd, scale, window, dtype, sink=None, v
     # what a decode step's keys are shared out by: with pooled entries, the keys it really reads
     context = ctx.max_context if pool is None else min(
         ctx.max_context, window + 64 + ctx.max_context // pool.pool)
-    if (fast and window == 0 and kv.window == 0 and bias is None and slope is None and pool is None
+    if (fast and window == 0 and "shared" in ctx.extras and kv.window == 0 and bias is None and slope is None and pool is None
             and hd <= 128 and hd % 16 == 0 and kv.block_tokens == 64 and q.stride(0) % 8 == 0
             and q.data_ptr() % 16 == 0):
         plan = shared_plan(ctx, nh, nkv, hd, dtype)

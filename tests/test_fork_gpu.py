@@ -254,6 +254,55 @@ def test_generate_beside_forks(model_dirs):
     eng.cache.check()
 
 
+@pytest.mark.parametrize("name", ["A", "B", "C", "W"])
+def test_several_answers_a_prompt(model_dirs, plain_models, always_shared, name):
+    """float32: each greedy answer is the plain model's, each sampled one what its request gives alone.
+    bfloat16: the best tokens or within the bound; the prompts' blocks are held once."""
+    prompts = [tiny.tokens(name, n, 6) for n in (70, 9, 66)]
+    cfg, w = plain_models[name]
+    eng = engine(model_dirs, name, "float32")
+    res = eng.generate(prompts, max_tokens=6, stop_ids=[], samples=3)
+    assert len(res) == 9
+    for i, r in enumerate(res):
+        assert r.tokens == plain_llama.greedy(cfg, w, prompts[i // 3], 6) and r.prompt_len == len(prompts[i // 3])
+    one = eng.generate([p for p in prompts for _ in range(3)], max_tokens=20, temperature=0.8, top_k=30, seed=5, stop_ids=[])
+    many = eng.generate(prompts, max_tokens=20, temperature=0.8, top_k=30, seed=5, stop_ids=[], samples=3)
+    assert [r.tokens for r in many] == [r.tokens for r in one]
+    assert len({tuple(r.tokens) for r in many[:3]}) > 1     # numbers of their own
+    stop = many[1].tokens[3]
+    cut = eng.generate(prompts, max_tokens=20, temperature=0.8, top_k=30, seed=5, stop_ids=[stop], samples=3)
+    for c, r in zip(cut, many):
+        assert c.tokens == (r.tokens[:r.tokens.index(stop) + 1] if stop in r.tokens else r.tokens)
+    eng.cache.check()
+    assert not eng.cache.slots.live()
+    eng = engine(model_dirs, name, "bfloat16")
+    for use_graph in (True, False):
+        res = eng.generate(prompts, max_tokens=8, stop_ids=[], samples=4, use_graph=use_graph)
+        for i, r in enumerate(res):
+            rows = plain_llama.forward(cfg, w, prompts[i // 4] + r.tokens[:-1], storage=torch.bfloat16).numpy()
+            rows = rows[len(prompts[i // 4]) - 1:]
+            bound = 4e-2 * float(np.abs(rows).max())
+            assert all(row.max() - row[t] <= bound for row, t in zip(rows, r.tokens))
+    eng.cache.check()
+    assert not eng.cache.slots.live()
+
+
+def test_answers_that_fit_only_because_they_share(model_dirs):
+    from cretif_b200.engine import Engine
+    eng = Engine(model_dirs["B"], dtype="bfloat16", max_tokens=512)      # eight blocks
+    prompt = tiny.tokens("B", 200, 2)
+    res = eng.generate([prompt], max_tokens=30, stop_ids=[], samples=5)  # four blocks and one for each of four more
+    assert len(res) == 5 and all(len(r.tokens) == 30 for r in res)
+    with pytest.raises(ValueError, match="cache holds"):
+        eng.generate([prompt], max_tokens=30, stop_ids=[], samples=6)
+    with pytest.raises(ValueError, match="answers a prompt"):
+        eng.generate([prompt], max_tokens=30, stop_ids=[], samples=65)
+    with pytest.raises(ValueError, match="answers a prompt"):
+        eng.generate([prompt], max_tokens=30, stop_ids=[], samples=0)
+    eng.cache.check()
+    assert not eng.cache.slots.live()
+
+
 def test_refusals(model_dirs):
     from cretif_b200.cache import CacheError
     eng = engine(model_dirs, "B", "bfloat16")
