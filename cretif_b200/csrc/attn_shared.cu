@@ -14,7 +14,7 @@ constexpr int kShRows = 32, kShThreads = 256;
 // 32-bit pieces: a block of 256 threads per (item, key/value head), up to 32 rows and 64 keys a step.
 // A warp has rows w, w + 8, w + 16, w + 24, those that there are: a lane two keys of their scores and VD
 // channels of their outputs, so a softmax is the warp's own.  The next step's keys and values are on
-// their way in registers.  (Eight answers at 1,984 tokens: F32_NOW us; 16 x 16 threads on 32 rows whatever
+// their way in registers.  (Eight answers at 1,984 tokens: 13.2 us; 16 x 16 threads on 32 rows whatever
 // there were took 25, most of it on the own keys' three rows.)
 template <int VD>
 __global__ void __launch_bounds__(kShThreads)

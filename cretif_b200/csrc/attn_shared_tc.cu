@@ -223,7 +223,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 
   if (warp == 4) {
     // Block ids come 32 at a time, a lane each, and a window ahead of their use: read one by one they
-    // cost two dependent loads a step (64 answers at 8,000: WINDOW_BEFORE us with, WINDOW_AFTER without).
+    // cost two dependent loads a step (64 answers with drafts at 30,016: 123 us with, 114.5 without).
     auto window = [&](int w) { return 32 * w + lane < n ? shared_block(a, it.seq, it.blk0 + 32 * w + lane) : 0; };
     int here = window(0), next = window(1), s = 0;        // windows of V's block, and the one behind it
     for (int p = 0; p <= n; ++p) {
@@ -416,7 +416,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 // of its own and needs no other warp until the end: scores and P V are m16n8k16 products with the
 // rows as their rows (NR = 1: up to 8 rows, and the products' other 8 are empty).
 // (Keys and values straight into the operands' registers, with no shared memory, took 120 registers and
-// kept 4 KB a warp in flight: 22 us against NOW_OWN for 64 sequences on 32 heads with 95 own keys.)
+// kept 4 KB a warp in flight: 22 us against 20.5 for 64 sequences on 32 heads with 95 own keys.)
 // WPI warps share an item, a CTA has four.  Four an item where there are few; one where there are items
 // enough to fill the chip with warps.
 // With JOIN the item's warps hold all of the rows' own keys and join the rows' prefix pieces (the kernel is

@@ -636,7 +636,7 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
 // (value, id).  Where they are too many for the list (equal logits in masses) the k-th largest is
 // found digit by digit over the whole row.
 // (512 threads: three CTAs of them fit an SM, and one's sort runs under another's loads.  218 rows of 49,152:
-// KEPT_NOW us, with 1,024 threads, one CTA an SM, 35.)
+// 21.4 us, with 1,024 threads, one CTA an SM, 35.)
 constexpr int kVkThreads = 512, kVkWarps = kVkThreads / 32, kVkList = 4096;
 constexpr int kVkMaxima = kVfMaxTopK / kVkThreads;        // maxima a thread keeps: together at least top_k
 
