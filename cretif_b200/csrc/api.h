@@ -579,8 +579,8 @@ int cretif_verify_drafts(const float* logits, int ld, int n_rows, const int* cu,
 // [max_pieces, T * nh, 2]: scratch.
 int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int ldo, const void* kc,
                        const void* vc, long long n_blocks, const int* table, int table_stride,
-                       int n_slots, const int* tok_pos, const int* seq_slot, const int* plan,
-                       int n_pre, int n_own, int own_rows, int own_splits, int max_pieces,
+                       int table_width, int n_slots, const int* tok_pos, const int* seq_slot,
+                       const int* plan, int n_pre, int n_own, int own_rows, int own_splits, int max_pieces,
                        int n_rows, int T, int nh, int nkv, int hd, int bt, float scale,
                        const float* sink, float* part_o, float* part_ml, unsigned int* fault,
                        void* stream);

@@ -288,7 +288,7 @@ using namespace cretif;
 
 extern "C" int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int ldo, const void* kc,
                                   const void* vc, long long n_blocks, const int* table,
-                                  int table_stride, int n_slots, const int* tok_pos,
+                                  int table_stride, int table_width, int n_slots, const int* tok_pos,
                                   const int* seq_slot, const int* plan, int n_pre, int n_own,
                                   int own_rows, int own_splits, int max_pieces, int n_rows, int T, int nh,
                                   int nkv, int hd, int bt, float scale, const float* sink,
@@ -305,7 +305,7 @@ extern "C" int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int
   if (!part_o && (dt == kF32 || n_pre > 0 || own_splits > 1)) return kBadArgument;
   SharedArgs a{};
   a.q = q; a.kc = kc; a.vc = vc; a.out = out; a.ldq = ldq; a.ldo = ldo; a.n_blocks = n_blocks;
-  a.table = table; a.table_stride = table_stride; a.n_slots = n_slots;
+  a.table = table; a.table_stride = table_stride; a.table_width = table_width; a.n_slots = n_slots;
   a.tok_pos = tok_pos; a.seq_slot = seq_slot;
   a.pre = reinterpret_cast<const SharedPrefixItem*>(plan);
   a.own = reinterpret_cast<const SharedOwnItem*>(plan + 8 * (size_t)n_pre);

@@ -39,7 +39,7 @@ struct SharedArgs {
   int ldq, ldo;
   long long n_blocks;
   const int* table;
-  int table_stride, n_slots;
+  int table_stride, table_width, n_slots;     // (a row's places lie a stride apart; a view's may be fewer)
   const int *tok_pos, *seq_slot;
   // the plan: prefix items, own items (of up to own_rows rows), the tokens of the groups, [T] prefix
   // pieces of a token
@@ -60,7 +60,7 @@ struct SharedArgs {
 // prefix kernel and has no wait of its own in front.)
 __device__ __forceinline__ int shared_block_of(const SharedArgs& a, int slot, int at) {
   int blk = -1;
-  if (slot >= 0 && slot < a.n_slots && at >= 0 && at < a.table_stride)
+  if (slot >= 0 && slot < a.n_slots && at >= 0 && at < a.table_width)
     blk = __ldcg(a.table + (size_t)slot * a.table_stride + at);
   if (blk < 0 || blk >= a.n_blocks) {
     atomicOr(a.fault, (unsigned)kFaultBlockTable);
@@ -73,9 +73,10 @@ __device__ __forceinline__ int shared_block(const SharedArgs& a, int seq, int at
 }
 
 // One past the last own key that an item's row at position `last` sees.  A position inside the shared
-// tokens is a caller's mistake: the fault bit is set and there are none.
+// tokens or behind the table is a caller's mistake: the fault bit is set and there are none (walked
+// all the same, a position of 2^31 would keep a warp for seconds).
 __device__ __forceinline__ int shared_own_end(const SharedArgs& a, const SharedOwnItem& it, int last) {
-  if (last >= it.least && last < 0x7fffff00) return last + 1;
+  if (last >= it.least && last < (long long)a.table_width * kShBlk && last < 0x7fffff00) return last + 1;
   atomicOr(a.fault, (unsigned)kFaultBlockTable);
   return it.prefix;
 }

@@ -39,7 +39,7 @@ def lib():
         L.cretif_verify_scratch.restype = ctypes.c_longlong
         # (with the types named, plain integers go through: half the time of wrapping each)
         p, i, ll, f, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_double
-        L.cretif_attn_shared.argtypes = [p, i, i, p, i, p, p, ll, p, i, i, p, p, p] + [i] * 11 + [f, p, p, p, p, p]
+        L.cretif_attn_shared.argtypes = [p, i, i, p, i, p, p, ll, p, i, i, i, p, p, p] + [i] * 11 + [f, p, p, p, p, p]
         L.cretif_verify_drafts.argtypes = [p, i, i, p, p, i, i, p, ll, ll, p, i, p, i, i, d, i, p, p, i, p, p, p]
         L.cretif_uniform01.argtypes = [ctypes.c_ulonglong, ctypes.c_longlong, ctypes.c_int]
         _lib = L
@@ -2030,7 +2030,7 @@ def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: Shar
         part_ml = part_o + 4 * n * hd
     _check((_lib or lib()).cretif_attn_shared(
         q.data_ptr(), ql[0], _DT[dt], out.data_ptr(), ol[0], kc.data_ptr(), vc.data_ptr(), ks[0],
-        table.data_ptr(), tl[0], ts[0], tok_pos.data_ptr(), seq_slot.data_ptr(),
+        table.data_ptr(), tl[0], ts[1], ts[0], tok_pos.data_ptr(), seq_slot.data_ptr(),
         plan.data.data_ptr(), *plan.launch, block_tokens, scale, 0 if sink is None else sink.data_ptr(), part_o, part_ml,
         fault.data_ptr(), _stream_of(dev)), "attn_shared", plan.kernels)
 

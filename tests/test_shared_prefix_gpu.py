@@ -195,6 +195,26 @@ def test_bad_pages_set_the_fault_word(ops):
             assert int(fault.item()) == 4, spoil
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=["bf16", "f32"])
+def test_a_table_that_is_a_view_ends_where_the_view_does(ops, dtype):
+    s = Step([([0, 1], 128)], own=[10, 70], news=[1, 2], nh=4, nkv=2, hd=64, dtype=dtype, seed=20, poison=0.0)
+    width = s.table.shape[1]
+    wide = torch.zeros((s.table.shape[0], 3 * width), dtype=torch.int32, device="cuda")   # (block 0 beside it)
+    wide[:, width:2 * width] = s.table
+    whole = s.check(ops)
+    s.table = wide[:, width:2 * width]
+    assert torch.equal(s.check(ops), whole)
+    plan, fault = s.plan(ops), torch.zeros(1, dtype=torch.int32, device="cuda")
+    pos = s.tok_pos.clone()
+    for at in (64 * width, 128 * width - 1, 2 ** 31 - 257, 2 ** 31 - 1):
+        s.tok_pos = pos.clone()
+        s.tok_pos[0] = at
+        out = s.run(ops, plan, fault=fault.zero_())
+        assert int(fault.item()) == 4, at
+        assert torch.equal(out[1:], whole[1:])             # (the other sequence's tokens)
+    s.tok_pos = pos
+
+
 def test_refusals(ops):
     s = Step([([0, 1], 128)], own=[10, 70], news=[1, 1], nh=4, nkv=2, hd=64, dtype=torch.bfloat16, seed=19)
     plan = s.plan(ops)
