@@ -273,9 +273,11 @@ static int launch_join(const SharedArgs& a, cudaStream_t st) {
 
 template <int VD>
 static int launch_shared_f32(const SharedArgs& a, cudaStream_t st) {
-  const size_t smem = ((size_t)(kShRows + kShBlk) * (a.hd + 4) + (size_t)kShBlk * a.hd + kShRows * kShBlk) * 4;
+  auto bytes = [](int hd) { return ((size_t)(kShRows + kShBlk) * (hd + 4) + (size_t)kShBlk * hd + kShRows * kShBlk) * 4; };
+  const size_t smem = bytes(a.hd);
+  // (the limit of the largest heads for all: another thread's call may be asking for its own)
   const cudaError_t e = cudaFuncSetAttribute(shared_pieces_kernel<VD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)smem);
+                                             (int)bytes(32 * VD));
   if (e != cudaSuccess) return (int)e;
   launch_dependent(shared_pieces_kernel<VD>, dim3(a.n_pre + a.n_own * a.own_splits, a.nkv), dim3(kShThreads), smem, st,
                    a);

@@ -704,15 +704,16 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 constexpr int kShDevices = 64;
 
 template <typename... Params, typename... Args>
-static int sp_launch(unsigned* limit, void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args&&... args) {
+static int sp_launch(bool* asked, void (*kernel)(Params...), dim3 grid, int threads, size_t smem, size_t most, cudaStream_t st, Args&&... args) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
-  // (the limit is asked for once a device and kernel: `limit` says up to what)
-  if (dev >= kShDevices || smem > limit[dev < kShDevices ? dev : 0]) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // (asked for once a device, and always for the `most` that any launch takes: two threads that ask for what they
+  // each need could leave the smaller one)
+  if (dev >= kShDevices || !asked[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     if (e != cudaSuccess) return (int)e;
-    if (dev < kShDevices) limit[dev] = (unsigned)smem;
+    if (dev < kShDevices) asked[dev] = true;
   }
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -734,14 +735,14 @@ enum SoCut { kSoWide, kSoNarrow, kSoWarp };               // 32 keys, 16 keys, a
 template <int HDG, int NR, int KEYS, int WPI, bool JOIN>
 static int launch_own_as(const SharedArgs& a, cudaStream_t st) {
   constexpr size_t smem = (size_t)kSoWarps * kSoStages * (kSoStage<HDG, KEYS> + 8) + kSoWarps * 4 + 1024;
-  static unsigned limit[kShDevices];
+  static bool asked[kShDevices];
   CUtensorMap mk, mv;
   const int rows = (int)(a.n_blocks * a.nkv * kShBlk);
   if (make_tile_map_bf16(&mk, a.kc, rows, a.hd, a.hd, KEYS) || make_tile_map_bf16(&mv, a.vc, rows, a.hd, a.hd, KEYS))
     return kBadArgument;
   const int ctas = JOIN ? (a.n_own * WPI + kSoWarps - 1) / kSoWarps : a.n_own * a.own_splits;
-  return sp_launch(limit, shared_own_mma_kernel<HDG, NR, KEYS, WPI, JOIN>, dim3(ctas, a.nkv), kSoThreads, smem, st, mk,
-                   mv, a, (int)(a.n_pre > 0));
+  return sp_launch(asked, shared_own_mma_kernel<HDG, NR, KEYS, WPI, JOIN>, dim3(ctas, a.nkv), kSoThreads, smem, smem, st,
+                   mk, mv, a, (int)(a.n_pre > 0));
 }
 
 template <int HDG, int NR>
@@ -765,8 +766,10 @@ int launch_shared_bf16(const SharedArgs& a, cudaStream_t st) {
         make_tile_map_bf16(&mv, a.vc, (int)cache_rows, a.hd, a.hd, kShBlk))
       return kBadArgument;
     const SpSmem L((a.hd + 63) / 64);
-    static unsigned limit[kShDevices];
-    const int e = sp_launch(limit, shared_prefix_tc_kernel, dim3(a.n_pre, a.nkv), kSpThreads, L.total, st, mk, mv, a);
+    static const int kSpMost = SpSmem(1).total > SpSmem(2).total ? SpSmem(1).total : SpSmem(2).total;
+    static bool asked[kShDevices];
+    const int e = sp_launch(asked, shared_prefix_tc_kernel, dim3(a.n_pre, a.nkv), kSpThreads, L.total,
+                            kSpMost, st, mk, mv, a);
     if (e) return e;
   }
   if (a.own_rows <= 8) return a.hd <= 64 ? launch_own<1, 1>(a, st) : launch_own<2, 1>(a, st);

@@ -1040,16 +1040,19 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
   // (two CTAs fit an SM with up to 100 KB of terms each)
   const int cached = a.draft_logits && (size_t)segs * kVdSeg * 16 <= 100 * 1024;
   const size_t smem = (size_t)room * 8 + (cached ? (size_t)segs * kVdSeg * 16 : 0);
-  if (smem > 200 * 1024) return kBadArgument;
+  constexpr size_t kVdMost = 200 * 1024;
+  if (smem > kVdMost) return kBadArgument;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
+  // (the limit is asked for once a device, and always for the most: two threads that ask for what they each need
+  // could leave the smaller one)
   constexpr int kDevices = 64;
-  static size_t limit[kDevices];                          // (asked for once a device)
-  if (dev >= kDevices || smem > limit[dev < kDevices ? dev : 0]) {
-    e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static bool asked[kDevices];
+  if (dev >= kDevices || !asked[dev]) {
+    e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kVdMost);
     if (e != cudaSuccess) return (int)e;
-    if (dev < kDevices) limit[dev] = smem;
+    if (dev < kDevices) asked[dev] = true;
   }
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

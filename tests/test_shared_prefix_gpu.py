@@ -195,6 +195,33 @@ def test_bad_pages_set_the_fault_word(ops):
             assert int(fault.item()) == 4, spoil
 
 
+def test_two_threads_with_heads_of_other_sizes(ops):
+    # (the kernels' shared memory goes by the head size)
+    import threading
+    steps = [Step([([0, 1, 2], 320)], own=[10, 70, 0], news=[2, 1, 1], nh=4, nkv=2, hd=hd, dtype=dtype, seed=21,
+                  poison=0.0) for hd in (16, 64, 80, 128) for dtype in TYPES]
+    want = [s.check(ops) for s in steps]
+    bad = []
+
+    def work(order):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    for i in order:
+                        if not torch.equal(steps[i].run(ops), want[i]):
+                            bad.append(i)
+        except Exception as e:                             # (a thread's error would be lost)
+            bad.append(repr(e))
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(list(range(8))[::d],)) for d in (1, -1)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert not bad
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=["bf16", "f32"])
 def test_a_table_that_is_a_view_ends_where_the_view_does(ops, dtype):
     s = Step([([0, 1], 128)], own=[10, 70], news=[1, 2], nh=4, nkv=2, hd=64, dtype=dtype, seed=20, poison=0.0)
