@@ -1866,9 +1866,11 @@ class SharedPrefixPlan:
     """How a step's rows and keys are dealt out, made by :func:`shared_prefix_plan`: device index
     arrays and launch sizes that depend on how many tokens the sequences bring and on what they
     share, not on slots, positions or values.  One plan serves every layer, and every later step of
-    the same make-up."""
+    the same make-up, on any stream; a captured call reads it at every replay, so it has to live as
+    long as the graph."""
 
-    __slots__ = ("data", "device", "sizes", "launch", "pieces", "kernels", "prefix_blocks", "T", "B")
+    __slots__ = ("data", "device", "sizes", "launch", "pieces", "kernels", "prefix_blocks", "T", "B",
+                 "stream", "made")
 
 
 def _blocks_an_item(tiles, ctas: int, turns: int = 1, begin: float = 4.0, join: float = 0.8) -> int:
@@ -1961,14 +1963,18 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
     share) pairs; the shared tokens are whole cache blocks of 64 that the members' tables name alike.
     A sequence is in one group at most.  ``news``: the tokens every sequence brings, ``starts``: its
     cached tokens (at least the shared ones).  How many ranges a sequence's own keys are cut into goes
-    by ``starts``; a plan stays right, if not best, while they grow."""
+    by ``starts``; a plan stays right, if not best, while they grow.  It copies to the device, so it is made
+    before a capture, not within."""
+    groups, news, starts = [(list(m), int(p)) for m, p in groups], [int(n) for n in news], [int(n) for n in starts]
     if dtype not in _DT:
         raise KernelError(f"shared prefix: tensors of dtype {dtype} have no kernel")
     if hd % 16 or not 16 <= hd <= 128:
         raise KernelError(f"shared prefix: head_dim {hd} is not a multiple of 16 up to 128")
     dev = torch.device(device)
     ctas = 2 * (sm_count(dev) if dev.type == "cuda" else 148)
-    groups, walk = [(list(m), int(p)) for m, p in groups], False
+    if dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise KernelError("shared prefix: a plan is made before a capture (its arrays are copied from the host)")
+    walk = False
     if dtype == torch.bfloat16 and all(p <= WALKED_TOKENS for _, p in groups) and sum(
             p * len(m) for m, p in groups) * nkv * hd * 4 <= WALKED_BYTES:
         walk = True
@@ -1982,6 +1988,9 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
     packed = torch.tensor(pre + own + rows + tok_pieces, dtype=torch.int32)
     plan.data = packed.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else packed
     plan.device, plan.T, plan.B = plan.data.device, len(tok_pieces), len(prefix_of)
+    if dev.type == "cuda":
+        plan.stream = _stream_of(plan.data.get_device())
+        plan.made = torch.cuda.current_stream(plan.device).record_event()
     plan.sizes = (nh, nkv, hd, plan.T, plan.B, dtype, plan.data.get_device())
     # as the C entry takes them: items, splits, pieces, tokens of the groups, T, heads, head size
     plan.launch = (len(pre) // 8, len(own) // 8, own_rows, splits, pieces, len(rows), plan.T, nh, nkv, hd)
@@ -2022,6 +2031,12 @@ def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: Shar
                                   and sink.is_contiguous() and sink.get_device() == dev))):
         _attn_shared_refused(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan, scale, block_tokens, fault,
                              sink)
+    stream = _stream_of(dev)
+    if stream != plan.stream and not torch.cuda.is_current_stream_capturing():
+        # (a capture begins when the device is idle, and cannot wait for what lies before it)
+        here = torch.cuda.current_stream(plan.device)
+        here.wait_event(plan.made)
+        plan.data.record_stream(here)
     part_o = part_ml = 0
     if plan.pieces:
         n = plan.pieces * T * nh
@@ -2032,7 +2047,7 @@ def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: Shar
         q.data_ptr(), ql[0], _DT[dt], out.data_ptr(), ol[0], kc.data_ptr(), vc.data_ptr(), ks[0],
         table.data_ptr(), tl[0], ts[1], ts[0], tok_pos.data_ptr(), seq_slot.data_ptr(),
         plan.data.data_ptr(), *plan.launch, block_tokens, scale, 0 if sink is None else sink.data_ptr(), part_o, part_ml,
-        fault.data_ptr(), _stream_of(dev)), "attn_shared", plan.kernels)
+        fault.data_ptr(), stream), "attn_shared", plan.kernels)
 
 
 def _attn_shared_refused(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan, scale, block_tokens, fault,

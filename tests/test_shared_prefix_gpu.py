@@ -195,6 +195,31 @@ def test_bad_pages_set_the_fault_word(ops):
             assert int(fault.item()) == 4, spoil
 
 
+def test_a_plan_made_on_another_stream(ops):
+    s = Step([([0, 1, 2], 640)], own=[10, 70, 0], news=[2, 1, 1], nh=4, nkv=2, hd=64, dtype=torch.bfloat16, seed=22,
+             poison=0.0)
+    want, side = s.check(ops), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)                      # (the plan's copy waits behind it)
+        plan = s.plan(ops)
+    got = s.run(ops, plan)
+    del plan                                               # its memory is not the side stream's again before
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            s.plan(ops).data.fill_(0)
+    assert torch.equal(got, want)
+
+
+def test_no_plan_within_a_capture(ops):
+    s = Step([([0, 1], 128)], own=[10, 70], news=[1, 1], nh=4, nkv=2, hd=64, dtype=torch.bfloat16, seed=23)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        torch.zeros(4, device="cuda")                      # (a capture of nothing at all warns)
+        with pytest.raises(ops.KernelError, match="before a capture"):
+            s.plan(ops)
+
+
 def test_two_threads_with_heads_of_other_sizes(ops):
     # (the kernels' shared memory goes by the head size)
     import threading

@@ -83,3 +83,11 @@ def test_cpu_tensors_are_refused():
         ops.attn_shared(z(2, 256), z(2, 256), z(4, 2, 64, 64), z(4, 2, 64, 64), z(2, 4, dtype=torch.int32),
                         z(2, dtype=torch.int32), z(3, dtype=torch.int32), z(2, dtype=torch.int32), plan, 0.125, 64,
                         z(1, dtype=torch.int32))
+
+
+def test_numbers_in_any_kind_of_sequence():
+    want = ops.shared_prefix_plan([([0, 1], 512)], [1, 3], [512, 600], 4, 2, 64, torch.bfloat16, "cpu")
+    for kind in (tuple, iter, torch.tensor):
+        got = ops.shared_prefix_plan(iter([(kind([0, 1]), torch.tensor(512))]), kind([1, 3]), kind([512, 600]), 4, 2,
+                                     64, torch.bfloat16, "cpu")
+        assert torch.equal(got.data, want.data) and got.launch == want.launch
