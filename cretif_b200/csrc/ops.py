@@ -1554,7 +1554,8 @@ def verify_drafts(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens, t
     id among equals) and the token is the arg max.  NaN counts as -infinity; a row whose largest
     entries are infinite is uniform over them.  A draft outside the vocabulary does not stand, a
     sequence without rows or with more than K drafts gives no token (-1); both set the token bit of
-    ``fault``."""
+    ``fault``.  Up to 65,535 sequences and a ``top_k`` of 1,024 or none; without one, at a temperature, up
+    to 8,191 drafts a sequence and 16 million ids."""
     if fault is None:
         fault = fault_word(logits.device)
     f32, i32 = torch.float32, torch.int32
@@ -2010,7 +2011,9 @@ def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: Shar
     are in the cache already.  ``sink`` (float32 [heads], optional): exp(sink_h)
     joins head h's softmax denominator.  bfloat16 or float32, head sizes in multiples of 16 up to 128,
     any number of query heads on a key/value head.  A table entry that names no block, or a position
-    inside the shared tokens, sets the block-table bit of ``fault``."""
+    inside the shared tokens or behind the table, sets the block-table bit of ``fault``.  What the cache holds behind a sequence's
+    last token may be anything; its tokens' own values are finite (those a token does not see yet are
+    taken zero times)."""
     nh, nkv, hd, T, B, dt, dev = plan.sizes
     i32 = torch.int32
     # one look at everything that has to hold; what does not is named by the slow way

@@ -299,6 +299,41 @@ def test_captured_on_another_stream(ops):
         assert torch.equal(accepted, want[0]) and torch.equal(tokens, want[1])
 
 
+def test_the_most_sequences_and_drafts(ops):
+    B = 65535
+    gen = torch.Generator().manual_seed(31)
+    logits = torch.randn((B + 1, 2), generator=gen)
+    p0 = torch.softmax(logits.double() / 0.7, dim=-1)[:, 0]
+    u = torch.rand(B + 1, generator=gen)
+    u = torch.where((u.double() - p0).abs() < 1e-3, torch.zeros_like(u), u)     # (away from the border)
+
+    def step(n):
+        return dict(logits=logits[:n].cuda(), cu=torch.arange(n + 1, dtype=torch.int32, device="cuda"),
+                    drafts=torch.zeros((n, 0), dtype=torch.int32, device="cuda"),
+                    accept_u=torch.zeros((n, 0), device="cuda"), next_u=u[:n].cuda())
+    for temperature, top_k, want in ((0.7, 0, u.double() >= p0), (0.7, 1, logits[:, 1] > logits[:, 0]),
+                                     (0.0, 0, logits[:, 1] > logits[:, 0])):
+        accepted, tokens = verify(ops, step(B), temperature, top_k)
+        assert torch.equal(tokens.cpu()[:, 0], want[:B].int()) and not accepted.any()
+        with pytest.raises(ops.KernelError):
+            verify(ops, step(B + 1), temperature, top_k)
+    for K, fits in ((8191, True), (8192, False)):
+        logits = torch.tensor([0.0, 40.0, 1.0]).repeat(K + 1, 1)
+        drafts = torch.ones((1, K), dtype=torch.int32)
+        drafts[0, 8000] = 0
+        s = dict(logits=logits.cuda(), cu=torch.tensor([0, K + 1], dtype=torch.int32, device="cuda"),
+                 drafts=drafts.cuda(), accept_u=torch.full((1, K), 0.5, device="cuda"),
+                 next_u=torch.full((1,), 0.5, device="cuda"))
+        for temperature, top_k in ((1.0, 0), (1.0, 2), (0.0, 0)):
+            if not fits and not top_k and temperature:
+                with pytest.raises(ops.KernelError):
+                    verify(ops, s, temperature, top_k)
+                continue
+            accepted, tokens = verify(ops, s, temperature, top_k)
+            assert accepted.tolist() == [8000]
+            assert (tokens[0, :8001] == 1).all() and (tokens[0, 8001:] == -1).all()
+
+
 def test_verifier_class(ops):
     from cretif_b200.sampling import DraftVerifier, SamplingParams
     s = make(4, 3, 300, [3, 2, 3, 3], seed=11, temperature=0.6, top_k=25)
