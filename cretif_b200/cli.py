@@ -12,7 +12,7 @@ of its last position as JSON (:242-301; default file ``cuinfer_logits.json``).
 
 Added options: ``--temperature``, ``--top-k``, ``--seed`` (the reference's
 ``generate`` arguments, which its program leaves at their defaults), ``--dtype``,
-``--cache-tokens``, ``--stop-ids``, and ``--random-weights SEED`` with ``--preset NAME`` or
+``--cache-tokens``, ``--stop-ids``, ``--samples`` (answers to the prompt), and ``--random-weights SEED`` with ``--preset NAME`` or
 ``--config FILE``, which first writes a model folder with seeded random weights to
 ``model_dir``.
 """

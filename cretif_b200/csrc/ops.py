@@ -1980,7 +1980,8 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
             p * len(m) for m, p in groups) * nkv * hd * 4 <= WALKED_BYTES:
         walk = True
     tile_rows, own_rows = (128, 16) if dtype == torch.bfloat16 else (32, 32)
-    if dtype == torch.bfloat16 and nkv > 0 and max(news, default=1) * nh // nkv <= 8:
+    if dtype == torch.bfloat16 and nkv > 0 and (max(news, default=1) * nh // nkv <= 8
+                                                or sum(-(-n * nh // nkv // 16) for n in news) * nkv <= ctas // 2):
         own_rows = 8
     pre, own, splits, pieces, rows, tok_pieces, prefix_of = _shared_items(groups, news, starts, nh, nkv, hd, tile_rows,
                                                                           own_rows, ctas, walk,
