@@ -748,11 +748,16 @@ static int launch_own_as(const SharedArgs& a, cudaStream_t st) {
 template <int HDG, int NR>
 static int launch_own(const SharedArgs& a, cudaStream_t st) {
   const long long items = (long long)a.n_own * a.nkv;
-  if (a.own_splits > 1) return launch_own_as<HDG, NR, 32, 4, false>(a, st);
+  // (own keys are cut where there are few items, and few items have up to 8 rows)
+  if (a.own_splits > 1) {
+    if constexpr (NR == 1) return launch_own_as<HDG, NR, 32, 4, false>(a, st);
+    else return kBadArgument;
+  }
   const SoCut cut = items > 8 * kSmCount ? kSoWarp : items > (HDG == 1 ? 2 : 1) * kSmCount ? kSoNarrow : kSoWide;
   if (cut == kSoWarp) return launch_own_as<HDG, NR, 16, 1, true>(a, st);
-  if (cut == kSoNarrow) return launch_own_as<HDG, NR, 16, 4, true>(a, st);
-  return launch_own_as<HDG, NR, 32, 4, true>(a, st);
+  if constexpr (HDG == 1 || NR == 1)
+    if (cut == kSoWide) return launch_own_as<HDG, NR, 32, 4, true>(a, st);
+  return launch_own_as<HDG, NR, 16, 4, true>(a, st);
 }
 
 // The prefix pieces and the own keys; joins the rows where the own keys are in one piece.

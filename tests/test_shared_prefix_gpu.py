@@ -59,6 +59,15 @@ def test_prefixes(ops, prefix, dtype):
          seed=prefix).check(ops)
 
 
+@pytest.mark.parametrize("hd", [64, 112])
+@pytest.mark.parametrize("batch", [18, 38, 80, 320])
+def test_many_rows_a_sequence(ops, batch, hd):
+    # (18 x 4 items of 16 rows are fewer than the SMs, 38 x 4 more, 80 x 4 and 320 x 4 take narrower steps)
+    s = Step([(list(range(batch)), 320)], own=[(37 * b) % 200 for b in range(batch)],
+             news=[1 + (b + 2) % 3 for b in range(batch)], nh=20, nkv=4, hd=hd, dtype=torch.bfloat16, seed=24)
+    s.check(ops)
+
+
 def test_nothing_shared(ops):
     Step([], own=[0, 1, 64, 500], news=[1, 4, 1, 2], nh=9, nkv=3, hd=64, dtype=torch.bfloat16, seed=3).check(ops)
 
