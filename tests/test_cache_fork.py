@@ -1,4 +1,6 @@
 """Sequences that share their first tokens, and sequences that go back: the cache's bookkeeping."""
+import random
+
 import pytest
 import torch
 
@@ -205,3 +207,47 @@ def test_going_back_is_refused_where_the_past_is_gone():
         cache.truncate(b, 100)                             # no block is left for the copy
     assert cache.length(b) == 128
     cache.check()
+
+
+@pytest.mark.parametrize("window", [False, True])
+@pytest.mark.parametrize("seed", range(6))
+def test_any_order_of_steps_forks_cuts_and_frees(seed, window):
+    rng = random.Random(seed)
+    cache = make(1024, window=window)
+    held = {}                                              # slot -> the values its tokens were written with
+    for turn in range(120):
+        live = sorted(held)
+        what = rng.choice(["new", "write", "write", "fork", "cut", "free", "reserve"])
+        s = rng.choice(live) if live else None
+        try:
+            if what == "new" or s is None:
+                held[cache.alloc_slot()] = []
+            elif what == "write":
+                n, at = rng.randint(1, 90), len(held[s])
+                write(cache, s, n, 1000.0 * turn)
+                held[s] = held[s] + [1000.0 * turn + p for p in range(at, at + n)]
+            elif what == "fork":
+                for new in cache.fork(s, rng.randint(1, 3)):
+                    held[new] = list(held[s])
+            elif what == "cut":
+                n = rng.randint(0, len(held[s]))
+                cache.truncate(s, n)
+                held[s] = held[s][:n]
+            elif what == "reserve":
+                cache.reserve(s, min(1024, len(held[s]) + rng.randint(0, 200)))
+            else:
+                cache.free_slot(s)
+                del held[s]
+        except CacheError:                                 # (no room, or a window's keys are gone: nothing has changed)
+            pass
+        cache.check()
+        for b in held:
+            assert cache.length(b) == len(held[b])
+            for g, got in zip(cache._kv_groups, read(cache, b)):
+                assert got == held[b][len(held[b]) - len(got):]
+                if b not in g.dirty:                       # (what is goes up before the next step)
+                    assert torch.equal(g.table[b], torch.from_numpy(g.table_host[b]))
+        slots = rng.sample(sorted(held), len(held))
+        for members, p in cache.shared_groups(slots) if len(slots) > 1 else []:
+            assert len(members) > 1 and 0 < p <= min(len(held[slots[m]]) for m in members)
+            assert all(held[slots[m]][:p] == held[slots[members[0]]][:p] for m in members)
