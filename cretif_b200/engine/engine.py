@@ -243,6 +243,14 @@ class Engine:
         groups = self.cache.shared_groups(slots)
         return (groups, tuple(int(n) for n in news), tuple(int(s) for s in starts)) if groups else None
 
+    @staticmethod
+    def shared_make_up(shared) -> tuple:
+        """(the groups, the most tokens a sequence has of its own) of ``shared_prefixes``'s answer."""
+        groups, news, starts = shared
+        prefix = {b: p for members, p in groups for b in members}
+        return (tuple((tuple(m), p) for m, p in groups),
+                max(s + n - prefix.get(b, 0) for b, (s, n) in enumerate(zip(starts, news))))
+
     def run(self, pairs, launch):
         """The one way a step runs: the cache makes room for ``pairs`` (slot, new tokens),
         ``launch()`` puts the step's kernels on the stream, the cache counts the tokens."""
@@ -357,9 +365,10 @@ class Engine:
         slots = [int(s) for s, _ in entries]
         shared = None
         if all(self.cache.slots.is_live(s) for s in slots):
-            shared = self.shared_prefixes(slots, [0] * len(slots), news)
+            shared = self.shared_prefixes(slots, [self.cache.length(s) for s in slots], news)
         if shared is not None:
-            w = (w, tuple((tuple(m), p) for m, p in shared[0]))
+            groups, own = self.shared_make_up(shared)
+            w = (w, groups, self.context_bucket(own))      # (plans are made for so many own keys)
         bucket = 0
         if all(n == 1 for n in news):
             longest = max((int(self.cache.lengths[int(s)]) for s, _ in entries), default=0) + 1

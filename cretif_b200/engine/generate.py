@@ -153,7 +153,7 @@ class DecodeRunner:
         self.engine, self.sampler, self.use_graph = engine, sampler, use_graph
         self.graphs: Dict[tuple, torch.cuda.CUDAGraph] = {}
         self.plans: Dict[tuple, dict] = {}        # of batches that share prefixes, by what they share
-        self.shared = None
+        self.shared = self.make_up = None
         self.bufs: Dict[int, dict] = {}
         self.stream = torch.cuda.Stream(device=engine.device)
         self.pool = torch.cuda.graph_pool_handle() if use_graph else None
@@ -183,11 +183,18 @@ class DecodeRunner:
                            non_blocking=True)
         self.B = B
         self.shared = self.engine.shared_prefixes([int(s) for s in slots], [int(p) for p in positions], [1] * B)
+        self.make_up = None if self.shared is None else self.engine.shared_make_up(self.shared)
+        self.longest = max(int(p) for p in positions) + 1
         if len(self.plans) > 64:                   # (of batches long gone; graphs keep their own)
             self.plans.clear()
 
-    def _shared_key(self) -> tuple:
-        return () if self.shared is None else tuple((tuple(m), p) for m, p in self.shared[0])
+    def _shared_key(self, context: int) -> tuple:
+        """What a plan, and a graph that holds it, are kept by when the longest sequence holds ``context``
+        tokens: what is shared, and the bucket of the own keys that the plan was made for."""
+        if self.make_up is None:
+            return ()
+        groups, own = self.make_up
+        return groups + (self.engine.context_bucket(own + context - self.longest),)
 
     def _body(self, b: dict, B: int, context: int) -> None:
         eng = self.engine
@@ -196,8 +203,9 @@ class DecodeRunner:
                           seq_start=b["seq_start"], cu_seqlens=b["cu"], is_decode=True,
                           max_new=1, max_context=context)
         if self.shared is not None:
-            ctx.extras["shared"] = self.shared
-            ctx.extras["shared_plans"] = self.plans.setdefault((B,) + self._shared_key(), {})
+            groups, news, starts = self.shared
+            ctx.extras["shared"] = groups, news, tuple(s + context - self.longest for s in starts)
+            ctx.extras["shared_plans"] = self.plans.setdefault((B,) + self._shared_key(context), {})
         logits = eng.model.forward(ctx, eng.cache, None)
         b["logits"] = logits
         self.sampler(logits, b["sampled"], b["request"], b["draw"])
@@ -211,7 +219,8 @@ class DecodeRunner:
         if not self.use_graph:
             self._body(b, B, context)
             return b["sampled"]
-        key = (B, self.engine.context_bucket(context), self._shared_key())
+        shared_key = self._shared_key(context)
+        key = (B, self.engine.context_bucket(context), shared_key)
         if key not in self.graphs:
             # Warm up outside the capture (lazy initialisation, kernel loading), restoring
             # the state the warm-up advanced, then capture.
@@ -233,7 +242,7 @@ class DecodeRunner:
                     self._body(b, B, context)
             cur.wait_stream(self.stream)
             b["ints"].copy_(saved)
-            self.graphs[key] = (g, dict(self.plans.get((B,) + self._shared_key(), {})))
+            self.graphs[key] = (g, dict(self.plans.get((B,) + shared_key, {})))
             shared = [k for k in self.graphs if k[2]]
             if len(shared) > MAX_SHARED_GRAPHS:    # (what batches share seldom comes again)
                 del self.graphs[shared[0]]

@@ -122,6 +122,27 @@ def test_captured_steps_of_forks(model_dirs, always_shared):
         assert torch.equal(x, y)
 
 
+def test_plans_follow_the_answers_lengths(model_dirs, always_shared, calls):
+    """A plan cuts own keys by how many there are: steps of the same shape get another one as they grow."""
+    eng = engine(model_dirs, "C", "bfloat16")
+    a = eng.alloc_slot()
+    eng.step([(a, tiny.tokens("C", 64, 3))])
+    b = eng.fork_slot(a)[0]
+    for _ in range(3):
+        eng.step([(s, [5, 6]) for s in (a, b)])
+    few = {id(p) for p in calls}
+    eng.step([(s, tiny.tokens("C", 600, 3)) for s in (a, b)])
+    del calls[:]
+    eng.step([(s, [5, 6]) for s in (a, b)])
+    assert calls and not few & {id(p) for p in calls}
+    for s in (a, b):
+        eng.free_slot(s)
+    for use_graph in (True, False):
+        del calls[:]
+        eng.generate([tiny.tokens("C", 64, 3)], max_tokens=600, stop_ids=[], samples=2, use_graph=use_graph)
+        assert len({id(p) for p in calls}) == 2             # up to 512 tokens of their own, and beyond
+
+
 def draft(rng, right, wrong, vocab):
     """Drafts of which some are the model's next tokens and some are not."""
     return [t if rng.random() < 0.7 else int(rng.integers(0, vocab)) for t in right] + [int(t) for t in wrong]
