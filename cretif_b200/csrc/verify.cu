@@ -81,6 +81,11 @@ __device__ __forceinline__ float vf_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float vf_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ VfPart vf_merge(VfPart a, VfPart b, float c) {
   VfPart r;
   r.m = fmaxf(a.m, b.m);
@@ -106,87 +111,108 @@ __device__ __forceinline__ const float* vf_row(const VfArgs& a, int i) {
 // ---- first launch: maximum and sum, or arg max, of a slice of a row.  A thread asks for all of its
 // NV vectors at once.  Rows may begin anywhere: the vectors begin at the first 16-byte boundary, the
 // up to three entries before it and behind the last vector are the first slice's.
-constexpr int kVsThreads = 256;
+constexpr int kVsThreads = 256, kVsWarps = kVsThreads / 32;
 
-template <int NV, bool GREEDY>
-__global__ void __launch_bounds__(kVsThreads)
-verify_rows_kernel(const __grid_constant__ VfArgs a) {
-  __shared__ VfPart part[kVsThreads / 32];
-  __shared__ unsigned long long best_s[kVsThreads / 32];
-  dependent_begin();
-  const int tid = threadIdx.x, slice = blockIdx.y;
-  const float* x = vf_row(a, blockIdx.x);
-  if (!x) return;
-  const int head = min(a.V, (int)((0u - (unsigned)((uintptr_t)x >> 2)) & 3u));
-  const int n4 = (a.V - head) >> 2;
-  const float4* x4 = reinterpret_cast<const float4*>(x + head);
-  const int v0 = slice * a.slice_vectors, v1 = min(n4, v0 + a.slice_vectors);
-  const float c = (float)a.log2_t;
-  const float ninf = -INFINITY;
-  VfPart mine{ninf, 0.f};
-  unsigned long long best = 0ull;
-  // (entries behind the slice are NaN: they count for nothing, not even in a row of -infinity)
-  const float none = __uint_as_float(0x7fffffffu);
-  for (int base = v0; base < v1; base += NV * kVsThreads) {
-    float v[4 * NV];
-    int n_mine = 0;
+// A thread's entries of a slice, -infinity behind its end.
+template <int NV>
+struct VsSlice {
+  float v[4 * NV];
+  float extra;                  // an entry before or behind the vectors
+  int at, end, head, extra_id;  // the first vector, the slice's end, entries before the row's first vector
+
+  __device__ __forceinline__ void load(const VfArgs& a, const float* x, int slice) {
+    const int tid = threadIdx.x;
+    const float none = -INFINITY;
+    head = min(a.V, (int)((0u - (unsigned)((uintptr_t)x >> 2)) & 3u));
+    const int n4 = (a.V - head) >> 2;
+    const float4* x4 = reinterpret_cast<const float4*>(x + head);
+    at = slice * a.slice_vectors + tid;
+    end = min(n4, (slice + 1) * a.slice_vectors);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int at = base + i * kVsThreads + tid;
       float4 f = make_float4(none, none, none, none);
-      if (at < v1) { f = __ldcs(x4 + at); n_mine += 4; }
+      if (at + i * kVsThreads < end) f = __ldcs(x4 + at + i * kVsThreads);
       v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
     }
-    if (GREEDY) {
+    extra_id = -1;
+    if (slice == 0 && tid < a.V - 4 * n4) {
+      extra_id = tid < head ? tid : 4 * n4 + tid;
+      extra = __ldg(x + extra_id);
+    }
+  }
+  __device__ __forceinline__ bool there(int i) const { return at + (i >> 2) * kVsThreads < end; }
+  __device__ __forceinline__ float largest() const {
+    float m[2] = {-INFINITY, -INFINITY};                  // (NaN is passed over)
 #pragma unroll
-      for (int i = 0; i < 4 * NV; ++i) {
-        const int at = base + (i >> 2) * kVsThreads + tid;
-        const unsigned long long k = at < v1 ? vf_rank(v[i], head + 4 * at + (i & 3)) : 0ull;
-        best = k > best ? k : best;
+    for (int i = 0; i < 4 * NV; i += 2) m[(i >> 1) & 1] = vf_max3(m[(i >> 1) & 1], v[i], v[i + 1]);
+    return fmaxf(m[0], m[1]);
+  }
+  __device__ __forceinline__ unsigned long long best() const {
+    const float m = largest();
+    int first = -1;
+#pragma unroll
+    for (int i = 4 * NV - 1; i >= 0; --i)
+      if (v[i] == m) first = i;
+    if (m == -INFINITY) {                                 // (all are, or are not there, or NaN)
+      first = -1;
+#pragma unroll
+      for (int i = 4 * NV - 1; i >= 0; --i)
+        if (there(i)) first = i;
+    }
+    unsigned long long b = first < 0 ? 0ull : vf_rank(m, head + 4 * (at + (first >> 2) * kVsThreads) + (first & 3));
+    if (extra_id >= 0) {
+      const unsigned long long k = vf_rank(extra, extra_id);
+      b = k > b ? k : b;
+    }
+    return b;
+  }
+  __device__ __forceinline__ VfPart sum(float c) const {
+    const float ninf = -INFINITY, m = largest();
+    VfPart mine{m, 0.f};
+    if (fabsf(m) != INFINITY) {
+      // two entries an instruction (x - max is rounded before it is scaled: the largest counts exactly 1)
+      float2 z[2] = {{0.f, 0.f}, {0.f, 0.f}};
+      const float2 neg = make_float2(-m, -m), cc = make_float2(c, c);
+#pragma unroll
+      for (int i = 0; i < 4 * NV; i += 2) {
+        const float2 d = __fmul2_rn(__fadd2_rn(make_float2(v[i], v[i + 1]), neg), cc);
+        z[(i >> 1) & 1] = __fadd2_rn(z[(i >> 1) & 1], make_float2(vf_ex2(d.x), vf_ex2(d.y)));
+      }
+      const float2 s = __fadd2_rn(z[0], z[1]);
+      mine.z = s.x + s.y;
+      if (mine.z != mine.z) {                             // a NaN's term is nothing
+        mine.z = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * NV; ++i) mine.z += vf_ex2((fmaxf(v[i], ninf) - m) * c);
       }
     } else {
-      // NaN in place: fmaxf passes it over; its term must be nothing as well
-      float m = ninf;
+      // equal infinities count 1 each (a NaN that is the row's as -infinity)
+      int equal = 0;
 #pragma unroll
-      for (int i = 0; i < 4 * NV; ++i) m = fmaxf(m, v[i]);
-      VfPart p{m, 0.f};
-      if (fabsf(m) != INFINITY) {
-        float z[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4 * NV; ++i) z[i & 1] += vf_ex2((fmaxf(v[i], ninf) - m) * c);
-        p.z = z[0] + z[1];
-      } else if (n_mine) {
-        // equal infinities count 1 each (a NaN that is the row's as -infinity)
-        int equal = 0;
-#pragma unroll
-        for (int i = 0; i < 4 * NV; ++i)
-          equal += base + (i >> 2) * kVsThreads + tid < v1 && fmaxf(v[i], ninf) == m;
-        p.z = (float)equal;
-      }
-      if (n_mine) mine = vf_merge(mine, p, c);
+      for (int i = 0; i < 4 * NV; ++i) equal += there(i) && fmaxf(v[i], ninf) == m;
+      mine.z = (float)equal;
     }
+    if (extra_id >= 0) mine = vf_merge(mine, VfPart{fmaxf(extra, ninf), 1.f}, c);
+    return mine;
   }
-  if (slice == 0) {
-    const int tail = a.V - head - 4 * n4;
-    if (tid < head + tail) {
-      const int id = tid < head ? tid : 4 * n4 + tid;
-      const float v = x[id];
-      if (GREEDY) {
-        const unsigned long long k = vf_rank(v, id);
-        best = k > best ? k : best;
-      } else {
-        mine = vf_merge(mine, VfPart{fmaxf(v, ninf), 1.f}, c);
-      }
-    }
-  }
+};
+
+// The slice's numbers out of its threads', into place `to`.
+template <int NV, bool GREEDY>
+__device__ __forceinline__ void vs_finish(const VfArgs& a, const VsSlice<NV>& s, float c, size_t to) {
+  __shared__ VfPart part[kVsWarps];
+  __shared__ unsigned long long best_s[kVsWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (GREEDY) {
+    unsigned long long best = s.best();
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
       best = k > best ? k : best;
     }
-    if ((tid & 31) == 0) best_s[tid >> 5] = best;
+    if (lane == 0) best_s[warp] = best;
   } else {
+    VfPart mine = s.sum(c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       VfPart p;
@@ -194,19 +220,31 @@ verify_rows_kernel(const __grid_constant__ VfArgs a) {
       p.z = __shfl_xor_sync(0xffffffffu, mine.z, o);
       mine = vf_merge(mine, p, c);
     }
-    if ((tid & 31) == 0) part[tid >> 5] = mine;
+    if (lane == 0) part[warp] = mine;
   }
   __syncthreads();
-  if (tid == 0) {
-    const size_t at = (size_t)blockIdx.x * a.slices + slice;
+  if (threadIdx.x == 0) {
     if (GREEDY) {
-      for (int w = 1; w < kVsThreads / 32; ++w) best = best_s[w] > best ? best_s[w] : best;
-      static_cast<unsigned long long*>(a.stats)[at] = best;
+      unsigned long long best = best_s[0];
+      for (int w = 1; w < kVsWarps; ++w) best = best_s[w] > best ? best_s[w] : best;
+      static_cast<unsigned long long*>(a.stats)[to] = best;
     } else {
-      for (int w = 1; w < kVsThreads / 32; ++w) mine = vf_merge(mine, part[w], c);
-      static_cast<VfPart*>(a.stats)[at] = mine;
+      VfPart mine = part[0];
+      for (int w = 1; w < kVsWarps; ++w) mine = vf_merge(mine, part[w], c);
+      static_cast<VfPart*>(a.stats)[to] = mine;
     }
   }
+}
+
+template <int NV, bool GREEDY>
+__global__ void __launch_bounds__(kVsThreads)
+verify_rows_kernel(const __grid_constant__ VfArgs a) {
+  dependent_begin();
+  const float* x = vf_row(a, blockIdx.x);
+  if (!x) return;
+  VsSlice<NV> s;
+  s.load(a, x, blockIdx.y);
+  vs_finish<NV, GREEDY>(a, s, (float)a.log2_t, (size_t)blockIdx.x * a.slices + blockIdx.y);
 }
 
 // ---- second launch, greedy: a warp a sequence
@@ -968,14 +1006,15 @@ verify_kept_draw_kernel(const __grid_constant__ VfArgs a) {
 }
 
 // How the first launch cuts rows: vectors of four a slice, and slices.  A CTA takes 12 vectors a
-// thread where there are rows enough to fill the chip with such CTAs, else 4.
-static void vf_cut(const VfArgs& a, int rows, int& vectors, int& slices) {
+// thread where there are rows enough to fill the chip with such CTAs, else 4.  Whether it does.
+constexpr int kVsMany = 12, kVsFew = 4;
+static bool vf_cut(const VfArgs& a, int rows, int& vectors, int& slices) {
   const long long n4 = a.V / 4 + 1;
-  const long long big = (n4 + 12 * kVsThreads - 1) / (12 * kVsThreads);
-  const bool few = big * rows < 2 * kSmCount;
-  const long long per = (few ? 4 : 12) * kVsThreads;
+  const bool many = (n4 + kVsMany * kVsThreads - 1) / (kVsMany * kVsThreads) * rows >= 2 * kSmCount;
+  const long long per = (many ? kVsMany : kVsFew) * kVsThreads;
   vectors = (int)per;
   slices = (int)((n4 + per - 1) / per);
+  return many;
 }
 
 }  // namespace cretif
@@ -988,7 +1027,7 @@ extern "C" long long cretif_verify_scratch(int n_rows, int B, int K, int V, int 
   if (n_rows <= 0 || B < 0 || K < 0 || V <= 0) return 0;
   const long long rows = (long long)n_rows + (draft_rows ? (long long)B * K : 0);
   if (top_k > 0 && top_k < V) return rows * (long long)(sizeof(VfKept) + 8LL * top_k);
-  return rows * 8LL * (V / 4 / (4 * kVsThreads) + 1);
+  return rows * 8LL * (V / 4 / (kVsFew * kVsThreads) + 1);
 }
 
 extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, const int* cu,
@@ -1019,15 +1058,14 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
     launch_dependent(verify_kept_draw_kernel, dim3(B), dim3(kVlThreads), 0, st, a);
     return launch_status();
   }
-  vf_cut(a, (int)rows, a.slice_vectors, a.slices);
-  const dim3 grid((unsigned)rows, a.slices);
-  const bool big = a.slice_vectors == 12 * kVsThreads;
+  const bool many = vf_cut(a, (int)rows, a.slice_vectors, a.slices);
+  auto kernel = greedy ? (many ? verify_rows_kernel<kVsMany, true> : verify_rows_kernel<kVsFew, true>)
+                       : (many ? verify_rows_kernel<kVsMany, false> : verify_rows_kernel<kVsFew, false>);
+  launch_dependent(kernel, dim3((unsigned)rows, a.slices), dim3(kVsThreads), 0, st, a);
   if (greedy) {
-    launch_dependent(big ? verify_rows_kernel<12, true> : verify_rows_kernel<4, true>, grid, dim3(kVsThreads), 0, st, a);
     launch_dependent(verify_greedy_kernel, dim3((B + 3) / 4), dim3(128), 0, st, a);
     return launch_status();
   }
-  launch_dependent(big ? verify_rows_kernel<12, false> : verify_rows_kernel<4, false>, grid, dim3(kVsThreads), 0, st, a);
   // CTAs a sequence: as many as a cluster holds, 1,024 entries each at least.  (Four for 64 sequences, whose
   // terms then do not fit beside one another and are computed twice: 61.6 us against 59.0.)
   int C = 8;
