@@ -1555,7 +1555,7 @@ def verify_drafts(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens, t
     entries are infinite is uniform over them.  A draft outside the vocabulary does not stand, a
     sequence without rows or with more than K drafts gives no token (-1); both set the token bit of
     ``fault``.  Up to 65,535 sequences and a ``top_k`` of 1,024 or none; without one, at a temperature, up
-    to 8,191 drafts a sequence and 16 million ids."""
+    to 8,191 drafts a sequence and 13 million ids."""
     if fault is None:
         fault = fault_word(logits.device)
     f32, i32 = torch.float32, torch.int32

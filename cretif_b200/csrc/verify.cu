@@ -20,6 +20,8 @@
 // The reference has no counterpart (its sampling: src/embedding.cu:343-406).
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "api.h"
 #include "common.cuh"
 
@@ -290,7 +292,7 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const __grid_constan
 }
 
 // ---- second launch, whole vocabulary: a cluster a sequence, its CTAs share the vocabulary
-constexpr int kVdThreads = 512, kVdSeg = 128;             // entries a warp takes at once
+constexpr int kVdSeg = 128;                               // entries a warp takes at once
 
 // 2^(i / 16) and 2^(i / 256): their products are the table of 256 that a CTA makes for itself.
 __device__ const double kVfCoarse[16] = {
@@ -372,21 +374,27 @@ __device__ __forceinline__ void vf_four(const float* x, int V, int i, bool align
   }
 }
 
-__global__ void __launch_bounds__(kVdThreads, 2)
-verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
-  // sums of the CTA's segments; where they fit (cached) the terms of its share of both rows
-  extern __shared__ __align__(16) double vd_smem[];
+// max(p - w q, 0) is summed in the one pass over the rows that sums p and q, before w = sum p / sum q is known in
+// 64 bits: with w0 from the first launch's sums, off by some 1e-7 of it, and beside it the q of the entries where
+// p > w0 q, so that a sum of max(p - w q, 0) is that of max(p - w0 q, 0) less (w - w0) times that of the q: what
+// is left out are entries whose p and w q differ by less than 1e-7 of themselves, by less than that.  The
+// segment that is drawn from is computed again with w.  (Two passes, the terms between them in 100 KB of shared
+// memory that leave an SM two CTAs: 55.5 us against 48.1 for 64 sequences of seven drafts, 11.6 against 11.2 for one.)
+template <int kVdThreads, int kCtas, int kAhead>
+__global__ void __launch_bounds__(kVdThreads, kCtas)
+verify_draw_kernel(const __grid_constant__ VfArgs a) {
+  extern __shared__ __align__(16) double2 vd_smem[];      // the segments' two sums; before them the rows' numbers
+  constexpr int kWarps = kVdThreads / 32;
+  static_assert(4 * kWarps % 32 == 0, "whole warps go through the sums");
   __shared__ double table[256];
-  __shared__ double sums[2 * kVdThreads / 32];
-  __shared__ double shared_tot[4];                        // this CTA's: p and q, what is drawn from
-  __shared__ double weight_s;
+  __shared__ double sums[4 * kWarps];
+  __shared__ double shared_tot[4];                        // this CTA's sums: p, q, max(p - w0 q, 0), q where p > w0 q
   __shared__ bool left_s;
   __shared__ int first_bad;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kWarps = kVdThreads / 32;
-  if (tid < 256) table[tid] = kVfCoarse[tid >> 4] * kVfFine[tid & 15];
+  for (int i = tid; i < 256; i += kVdThreads) table[i] = kVfCoarse[i >> 4] * kVfFine[i & 15];
   if (tid == 0) first_bad = 0x7fffffff;
   dependent_begin();
   int row0, n;
@@ -459,32 +467,14 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
   VfTerm tp, tq;
   tp.set(rows[j].m, a.log2_t, a.reach);
   tq = tp;
-  if (minus_q) tq.set(rows[n + 1 + j].m, a.log2_t, a.reach);
+  double w0 = 0.0;
+  if (minus_q) {
+    tq.set(rows[n + 1 + j].m, a.log2_t, a.reach);
+    w0 = (double)rows[j].z / (double)rows[n + 1 + j].z;
+  }
   __syncthreads();                                        // (the rows' numbers give way to the segments')
   const int segs = (a.V + kVdSeg - 1) / kVdSeg;
   const int s0 = (int)((long long)segs * rank / C), s1 = (int)((long long)segs * (rank + 1) / C);
-  // Two sums of all the cluster's threads, for warp 0; each in this CTA's shared_tot[at] and [at + 1].
-  // Lane r < C of warp 0 has CTA r's afterwards.
-  auto gather = [&](double v, double w, int at, double& rv, double& rw) {
-    v = vf_warp_sum(v);
-    w = vf_warp_sum(w);
-    if (lane == 0) { sums[warp] = v; sums[kWarps + warp] = w; }
-    __syncthreads();
-    if (warp == 0) {                                      // the first half of the lanes the first sum, the others the second
-      double t = lane < 2 * kWarps ? sums[lane] : 0.0;
-#pragma unroll
-      for (int o = kWarps / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if (lane < 2 * kWarps && lane % kWarps == 0) shared_tot[at + lane / kWarps] = t;
-    }
-    cluster.sync();
-    rv = rw = 0.0;
-    if (warp == 0 && lane < C) {
-      const double* there = cluster.map_shared_rank(shared_tot, lane);
-      rv = there[at];
-      rw = there[at + 1];
-    }
-  };
-  double2* keep = reinterpret_cast<double2*>(vd_smem + seg_room);   // [segment][row][lane][2]
   // the four terms of a lane in a segment of a row (0 behind the vocabulary)
   auto look = [&](const VfTerm& row, const float* x, bool aligned, int s, double (&v)[4]) {
     float f[4];
@@ -496,109 +486,107 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
         if (s * kVdSeg + 4 * lane + e >= a.V) v[e] = 0.0;
     }
   };
-  double weight = 0.0;                                    // of q's terms beside p's
-  if (minus_q) {
-    double zp = 0.0, zq = 0.0;
-    // the loads of kAhead segments go out together (rows on 16-byte boundaries, segments inside the row)
-    constexpr int kAhead = 3;
-    for (int base = s0 + warp; base < s1; base += kAhead * kWarps) {
-      float fp[kAhead][4], fq[kAhead][4];
-      const bool quick = ap && aq && (base + (kAhead - 1) * kWarps + 1) * kVdSeg <= a.V;
-      if (quick) {
-#pragma unroll
-        for (int x = 0; x < kAhead; ++x) {
-          const int i = (base + x * kWarps) * 32 + lane;
-          const float4 u = __ldg(reinterpret_cast<const float4*>(xp) + i), w = __ldg(reinterpret_cast<const float4*>(xq) + i);
-          fp[x][0] = u.x; fp[x][1] = u.y; fp[x][2] = u.z; fp[x][3] = u.w;
-          fq[x][0] = w.x; fq[x][1] = w.y; fq[x][2] = w.z; fq[x][3] = w.w;
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < kAhead; ++x) {
-        const int s = base + x * kWarps;
-        if (s >= s1) break;
-        double vp[4], vq[4];
-        if (quick) {
-          tp.four(fp[x], vp, table);
-          tq.four(fq[x], vq, table);
-        } else {
-          look(tp, xp, ap, s, vp);
-          look(tq, xq, aq, s, vq);
-        }
-        zp += (vp[0] + vp[1]) + (vp[2] + vp[3]);
-        zq += (vq[0] + vq[1]) + (vq[2] + vq[3]);
-        if (cached) {
-          double2* at = keep + (size_t)(s - s0) * 128 + lane;
-          at[0] = make_double2(vp[0], vp[1]);
-          at[32] = make_double2(vp[2], vp[3]);
-          at[64] = make_double2(vq[0], vq[1]);
-          at[96] = make_double2(vq[2], vq[3]);
-        }
-      }
-    }
-    double rp, rq, all_p = 0.0, all_q = 0.0;
-    gather(zp, zq, 0, rp, rq);
-    if (warp == 0) {
-      for (int r = 0; r < C; ++r) {                       // (in the same order everywhere)
-        all_p += __shfl_sync(0xffffffffu, rp, r);
-        all_q += __shfl_sync(0xffffffffu, rq, r);
-      }
-      if (lane == 0) weight_s = all_p / all_q;
-    }
-    __syncthreads();
-    weight = weight_s;
-  }
   for (int turn = rest ? 0 : 1; turn < 2; ++turn) {       // (the second where p and q leave nothing)
     const bool minus = turn == 0;
-    // what is drawn from: the four terms of a lane in a segment (a warp reads what it kept itself, and
-    // the segment that is drawn from after a barrier)
-    auto terms = [&](int s, double (&v)[4]) {
-      if (minus && minus_q) {
-        double vq[4];
-        if (cached) {
-          const double2* at = keep + (size_t)(s - s0) * 128 + lane;
-          const double2 p0 = at[0], p1 = at[32], q0 = at[64], q1 = at[96];
-          v[0] = p0.x; v[1] = p0.y; v[2] = p1.x; v[3] = p1.y;
-          vq[0] = q0.x; vq[1] = q0.y; vq[2] = q1.x; vq[3] = q1.y;
-        } else {
-          look(tp, xp, ap, s, v);
-          look(tq, xq, aq, s, vq);
+    double mine[4] = {0.0, 0.0, 0.0, 0.0};
+    // the loads of kAhead segments go out together
+    auto pass = [&](auto constant) {
+      constexpr bool kQ = decltype(constant)::value;
+      for (int first = s0 + warp; first < s1; first += kAhead * kWarps) {
+        float fp[kAhead][4], fq[kAhead][4];
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+          const int s = first + x * kWarps;
+          if (s >= s1) continue;
+          vf_four(xp, a.V, s * 32 + lane, ap, fp[x]);
+          if (kQ) vf_four(xq, a.V, s * 32 + lane, aq, fq[x]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const double r = fma(-weight, vq[e], v[e]);
-          v[e] = r > 0.0 ? r : 0.0;
+        for (int x = 0; x < kAhead; ++x) {
+          const int s = first + x * kWarps;
+          if (s >= s1) continue;
+          double vp[4], vq[4], r = 0.0, qa = 0.0;
+          tp.four(fp[x], vp, table);
+          if (kQ) tq.four(fq[x], vq, table);
+          const int id = s * kVdSeg + 4 * lane;
+          if ((s + 1) * kVdSeg > a.V) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (id + e >= a.V) { vp[e] = 0.0; if (kQ) vq[e] = 0.0; }
+          }
+          if (kQ) {
+            mine[0] += (vp[0] + vp[1]) + (vp[2] + vp[3]);
+            mine[1] += (vq[0] + vq[1]) + (vq[2] + vq[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const double over = fma(-w0, vq[e], vp[e]);
+              if (over > 0.0) { r += over; qa += vq[e]; }
+            }
+            qa = vf_warp_sum(qa);
+          } else {
+            if (minus && (unsigned)(d - id) < 4u) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (id + e == d) vp[e] = 0.0;
+            }
+            r = (vp[0] + vp[1]) + (vp[2] + vp[3]);
+          }
+          r = vf_warp_sum(r);
+          if (lane == 0) {
+            vd_smem[s - s0] = make_double2(r, qa);
+            mine[2] += r;
+            mine[3] += qa;
+          }
         }
-        return;
       }
-      look(tp, xp, ap, s, v);
-      if (minus) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (s * kVdSeg + 4 * lane + e == d) v[e] = 0.0;
+      if (kQ) {
+        mine[0] = vf_warp_sum(mine[0]);
+        mine[1] = vf_warp_sum(mine[1]);
       }
     };
-    double mine = 0.0;
-    for (int s = s0 + warp; s < s1; s += kWarps) {
-      double v[4];
-      terms(s, v);
-      const double sum = vf_warp_sum((v[0] + v[1]) + (v[2] + v[3]));
-      if (lane == 0) {
-        vd_smem[s - s0] = sum;
-        mine += sum;
+    if (minus && minus_q) pass(std::true_type{});
+    else pass(std::false_type{});
+    // ---- the cluster's sums: lane r < C of warp 0 has CTA r's
+    if (lane == 0) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sums[q * kWarps + warp] = mine[q];
+    }
+    __syncthreads();
+    if (warp == 0) {                                      // lanes of kWarps a sum
+#pragma unroll
+      for (int at = lane; at < 4 * kWarps; at += 32) {
+        double v = sums[at];
+#pragma unroll
+        for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (at % kWarps == 0) shared_tot[at / kWarps] = v;
       }
     }
-    double rv, unused, total = 0.0, base = 0.0, own = 0.0;
-    gather(mine, 0.0, 2, rv, unused);
+    cluster.sync();
+    double total = 0.0, base = 0.0, own = 0.0, weight = 0.0;
     int last_rank = -1;
-    for (int r = 0; r < C; ++r) {                         // (warp 0 has the numbers, and goes on alone)
-      const double t = __shfl_sync(0xffffffffu, rv, r);
-      if (r == rank) { base = total; own = t; }
-      if (t > 0.0) last_rank = r;
-      total += t;
+    if (warp == 0) {
+      double t4[4] = {0.0, 0.0, 0.0, 0.0};
+      if (lane < C) {
+        const double* there = cluster.map_shared_rank(shared_tot, lane);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) t4[q] = there[q];
+      }
+      double least = 0.0;
+      if (minus && minus_q) {
+        const double all_p = vf_warp_sum(t4[0]);
+        weight = all_p / vf_warp_sum(t4[1]);
+        t4[2] = fma(w0 - weight, t4[3], t4[2]);
+        least = 1e-13 * all_p;                            // (what rounding leaves of rows that are alike)
+      }
+      for (int r = 0; r < C; ++r) {                       // (in the same order everywhere)
+        const double t = __shfl_sync(0xffffffffu, t4[2], r);
+        if (r == rank) { base = total; own = t; }
+        if (t > 0.0) last_rank = r;
+        total += t;
+      }
+      if (lane == 0) left_s = total > least;
     }
     cluster.barrier_arrive();                             // its reads of the others' memory are done
-    if (tid == 0) left_s = total > 0.0;
     __syncthreads();
     const bool left = left_s;
     if (!left && turn == 0) { cluster.barrier_wait(); continue; }
@@ -613,7 +601,11 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
       int seg = -1, last_seg = -1;
       double seg_base = 0.0;
       for (int i0 = 0; i0 < s1 - s0 && seg < 0; i0 += 32) {
-        const double v = i0 + lane < s1 - s0 ? vd_smem[i0 + lane] : 0.0;
+        double v = 0.0;
+        if (i0 + lane < s1 - s0) {
+          const double2 both = vd_smem[i0 + lane];
+          v = minus && minus_q ? fma(w0 - weight, both.y, both.x) : both.x;
+        }
         double inc = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -633,8 +625,24 @@ verify_draw_kernel(const __grid_constant__ VfArgs a, int seg_room, int cached) {
       }
       const bool take_last = seg < 0;                     // (rounding passed the last border)
       if (take_last) seg = last_seg;
+      // what is drawn from in the segment, four entries a lane
       double v[4];
-      terms(s0 + seg, v);
+      look(tp, xp, ap, s0 + seg, v);
+      if (minus && minus_q) {
+        double vq[4];
+        look(tq, xq, aq, s0 + seg, vq);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vq[e] = fmax(fma(-weight, vq[e], v[e]), 0.0);
+        // (where nothing is left but what rounding made of a sum, any id with a probability)
+        if (__any_sync(0xffffffffu, vq[0] > 0.0 || vq[1] > 0.0 || vq[2] > 0.0 || vq[3] > 0.0)) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = vq[e];
+        }
+      } else if (minus) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((s0 + seg) * kVdSeg + 4 * lane + e == d) v[e] = 0.0;
+      }
       const double four = (v[0] + v[1]) + (v[2] + v[3]);
       double inc = four;
 #pragma unroll
@@ -1017,6 +1025,40 @@ static bool vf_cut(const VfArgs& a, int rows, int& vectors, int& slices) {
   return many;
 }
 
+constexpr size_t kVdMost = 200 * 1024;
+
+template <int kThreads, int kCtas, int kAhead>
+static int vd_launch(const VfArgs& a, int C, size_t smem, cudaStream_t st) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  // (the limit is asked for once a device, and always for the most: two threads that ask for what they each need
+  // could leave the smaller one)
+  constexpr int kDevices = 64;
+  static bool asked[kDevices];
+  if (dev >= kDevices || !asked[dev]) {
+    e = cudaFuncSetAttribute(verify_draw_kernel<kThreads, kCtas, kAhead>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kVdMost);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < kDevices) asked[dev] = true;
+  }
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = C * a.B <= kSmCount ? dependent_launch_enabled() : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C, a.B);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, verify_draw_kernel<kThreads, kCtas, kAhead>, a);
+  return e == cudaSuccess ? launch_status() : (int)e;
+}
+
 }  // namespace cretif
 
 using namespace cretif;
@@ -1066,46 +1108,15 @@ extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, con
     launch_dependent(verify_greedy_kernel, dim3((B + 3) / 4), dim3(128), 0, st, a);
     return launch_status();
   }
-  // CTAs a sequence: as many as a cluster holds, 1,024 entries each at least.  (Four for 64 sequences, whose
-  // terms then do not fit beside one another and are computed twice: 61.6 us against 59.0.)
+  // CTAs a sequence: as many as a cluster holds, 1,024 entries each at least
   int C = 8;
   while (C > 1 && V < 1024 * C) C >>= 1;
   const int segs = ((V + kVdSeg - 1) / kVdSeg + C - 1) / C + 1;
-  // segments' sums, and before them the rows' numbers
-  const long long room_ll = segs > 2LL * K + 1 ? segs : 2LL * K + 1;
-  if (room_ll > 16 * 1024) return kBadArgument;
-  const int room = ((int)room_ll + 1) & ~1;
-  // (two CTAs fit an SM with up to 100 KB of terms each)
-  const int cached = a.draft_logits && (size_t)segs * kVdSeg * 16 <= 100 * 1024;
-  const size_t smem = (size_t)room * 8 + (cached ? (size_t)segs * kVdSeg * 16 : 0);
-  constexpr size_t kVdMost = 200 * 1024;
-  if (smem > kVdMost) return kBadArgument;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return (int)e;
-  // (the limit is asked for once a device, and always for the most: two threads that ask for what they each need
-  // could leave the smaller one)
-  constexpr int kDevices = 64;
-  static bool asked[kDevices];
-  if (dev >= kDevices || !asked[dev]) {
-    e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kVdMost);
-    if (e != cudaSuccess) return (int)e;
-    if (dev < kDevices) asked[dev] = true;
-  }
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = C * B <= kSmCount ? dependent_launch_enabled() : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = C;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(C, B);
-  cfg.blockDim = dim3(kVdThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, verify_draw_kernel, a, room, cached);
-  return e == cudaSuccess ? launch_status() : (int)e;
+  // segments' sums, and before them the rows' numbers (half of 16 bytes each)
+  const long long room = segs > K + 1LL ? segs : K + 1LL;
+  if (K > 8191 || room * 16 > (long long)kVdMost) return kBadArgument;
+  const size_t smem = (size_t)room * 16;
+  // A CTA an SM of 512 threads, or four of 256, which are all there at once.  (One sequence 13.8 us with 256 threads,
+  // 64 sequences 54.3 with two CTAs of 512.)
+  return C * B <= kSmCount ? vd_launch<512, 1, 2>(a, C, smem, st) : vd_launch<256, 4, 1>(a, C, smem, st);
 }
