@@ -168,6 +168,21 @@ def test_a_draft_like_the_model_always_stands(ops):
     assert (accepted == 4).all()
 
 
+@pytest.mark.parametrize("V", [151, 5001, 49153])
+def test_nothing_left_of_rows_that_are_alike(ops, V):
+    # (rows of an odd length begin on other boundaries, so that 32-bit sums of the same numbers differ)
+    s = make(6, 3, V, [3, 2, 3, 1, 3, 3], seed=40, temperature=0.8, top_k=0, like=0.0)
+    cu = s["cu"].tolist()
+    for b in range(6):
+        bad = 7 * b + 1                                    # what neither row allows is not a draft that stands
+        s["drafts"][b, b % 2] = bad
+        s["logits"][cu[b]:cu[b + 1], bad] = float("-inf")
+        s["draft_logits"][b, :, bad] = float("-inf")
+        s["drafts"][b, 1 - b % 2] = bad + 1
+    accepted = check(ops, s, 0.8, 0)
+    assert accepted.tolist() == [min(b % 2, n) for b, n in enumerate([3, 2, 3, 1, 3, 3])]
+
+
 def test_equal_logits_are_kept_by_id(ops):
     """Ties at the top-k border keep the lowest ids; a flat row is uniform."""
     s = make(4, 2, 4096, [2, 2, 1, 0], seed=4, temperature=1.0, top_k=9)
