@@ -1879,7 +1879,7 @@ def _blocks_an_item(tiles, ctas: int, turns: int = 1, begin: float = 4.0, join: 
     each of its ranges at once) pairs.  The least of: the turns of ``ctas`` items times what one takes,
     which is its blocks and some ``begin`` more for setting up, and the joining of the pieces, eight at a
     time in ``turns`` turns of ``join`` each.  (16 heads of 128 on 2, 24 rows a sequence, 2,432 shared
-    tokens: 19 pieces 32.5 us, 8 pieces 23.0.)"""
+    tokens, own items of 16 rows: 19 pieces 32.5 us, 8 pieces 23.0.)"""
     longest = max((blocks for blocks, _ in tiles), default=1)
     best = (None, longest)
     for pieces in range(1, min(longest, ctas) + 1):
