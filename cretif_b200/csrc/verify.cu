@@ -376,10 +376,15 @@ __device__ __forceinline__ void vf_four(const float* x, int V, int i, bool align
 
 // max(p - w q, 0) is summed in the one pass over the rows that sums p and q, before w = sum p / sum q is known in
 // 64 bits: with w0 from the first launch's sums, off by some 1e-7 of it, and beside it the q of the entries where
-// p > w0 q, so that a sum of max(p - w q, 0) is that of max(p - w0 q, 0) less (w - w0) times that of the q: what
-// is left out are entries whose p and w q differ by less than 1e-7 of themselves, by less than that.  The
+// p > w0 q, so that a sum of max(p - w q, 0) is that of max(p - w0 q, 0) less (w - w0) times that of the q.  That
+// is wrong, by at most |w - w0| q, in the entries where p lies between w q and w0 q: they are counted with the
+// wrong sign, or not at all.  Together that is |w - w0| sum q at most; where it could be more than kVdSlack of what
+// is left to draw from, the pass is made again with w in w0's place (rows that are nearly alike).  The
 // segment that is drawn from is computed again with w.  (Two passes, the terms between them in 100 KB of shared
 // memory that leave an SM two CTAs: 55.5 us against 48.1 for 64 sequences of seven drafts, 11.6 against 11.2 for one.)
+constexpr double kVdSlack = 1.0 / (1 << 17);
+// What rounding leaves of numbers that are alike, as a share of them: 64-bit sums of some hundred additions in a row.
+constexpr double kVdNothing = 1e-13;
 template <int kVdThreads, int kCtas, int kAhead>
 __global__ void __launch_bounds__(kVdThreads, kCtas)
 verify_draw_kernel(const __grid_constant__ VfArgs a) {
@@ -389,7 +394,9 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
   __shared__ double table[256];
   __shared__ double sums[4 * kWarps];
   __shared__ double shared_tot[4];                        // this CTA's sums: p, q, max(p - w0 q, 0), q where p > w0 q
-  __shared__ bool left_s;
+  enum { kDraw, kNothingLeft, kAgain };
+  __shared__ int step_s;
+  __shared__ double weight_s;
   __shared__ int first_bad;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
@@ -571,12 +578,15 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) t4[q] = there[q];
       }
-      double least = 0.0;
+      double least = 0.0, slack = 0.0;
       if (minus && minus_q) {
-        const double all_p = vf_warp_sum(t4[0]);
-        weight = all_p / vf_warp_sum(t4[1]);
+        const double all_p = vf_warp_sum(t4[0]), all_q = vf_warp_sum(t4[1]);
+        weight = all_p / all_q;
+        // (a CTA with nothing to draw has exactly zero: below it, two CTAs would find the goal in their ranges)
         t4[2] = fma(w0 - weight, t4[3], t4[2]);
-        least = 1e-13 * all_p;                            // (what rounding leaves of rows that are alike)
+        if (!(t4[2] > kVdNothing * t4[0])) t4[2] = 0.0;
+        least = kVdNothing * all_p;
+        slack = fabs(w0 - weight) * all_q;
       }
       for (int r = 0; r < C; ++r) {                       // (in the same order everywhere)
         const double t = __shfl_sync(0xffffffffu, t4[2], r);
@@ -584,12 +594,22 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
         if (t > 0.0) last_rank = r;
         total += t;
       }
-      if (lane == 0) left_s = total > least;
+      // (all CTAs of the cluster have the same numbers and decide alike)
+      if (lane == 0) {
+        step_s = slack > kVdSlack * total ? kAgain : !minus || total > least ? kDraw : kNothingLeft;
+        weight_s = weight;
+      }
     }
     cluster.barrier_arrive();                             // its reads of the others' memory are done
     __syncthreads();
-    const bool left = left_s;
-    if (!left && turn == 0) { cluster.barrier_wait(); continue; }
+    if (step_s != kDraw) {
+      if (step_s == kAgain) {                             // (once: the same sums give the same w, and no slack)
+        w0 = weight_s;
+        --turn;
+      }
+      cluster.barrier_wait();
+      continue;
+    }
     // (a number that is not in [0, 1) counts as the nearest that is)
     double goal = (double)a.next_u[b] * total;
     if (!(goal >= 0.0)) goal = 0.0;
@@ -598,7 +618,7 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
     if (here && warp == 0) {
       // the segment, 32 at a time, and the place in it
       double run = base;
-      int seg = -1, last_seg = -1;
+      int seg = -1, last_seg = 0;
       double seg_base = 0.0;
       for (int i0 = 0; i0 < s1 - s0 && seg < 0; i0 += 32) {
         double v = 0.0;
