@@ -12,9 +12,10 @@
 // it is, so that a row of equal infinities is uniform; NaN counts as -infinity.
 //
 // Two launches.  The first looks at all rows: what decides whether a draft stands are its row's
-// maximum and sum (32-bit terms, off by about 1e-8 of the sum: a draft is judged otherwise once in
-// 1e8), with top_k the kept entries themselves.  The second decides and draws.  An id is drawn at one
-// of V borders, so sums that are off by 1e-8 would draw another id once in V 1e-8 draws (1 in 2,000
+// maximum and sum (32-bit terms, off by about 1e-7 of the sum), with top_k the kept entries
+// themselves (in 64 bits).  The second decides and draws.  Where u q and p lie so close that the 32-bit
+// sums cannot tell which is larger, the draft's rows are summed in 64 bits first.  An id is drawn at one
+// of V borders, so sums that are off by 1e-7 would draw another id once in V 1e-7 draws (1 in 200
 // at 49,152 ids): the one or two rows that a sequence draws from are summed again in 64 bits.
 //
 // The reference has no counterpart (its sampling: src/embedding.cu:343-406).
@@ -383,6 +384,11 @@ __device__ __forceinline__ void vf_four(const float* x, int V, int i, bool align
 // segment that is drawn from is computed again with w.  (Two passes, the terms between them in 100 KB of shared
 // memory that leave an SM two CTAs: 55.5 us against 48.1 for 64 sequences of seven drafts, 11.6 against 11.2 for one.)
 constexpr double kVdSlack = 1.0 / (1 << 17);
+// How far u q and p have to lie apart, as a share of p, for the first launch's sums to tell them.  A term's exponent x
+// is off by 3 |x| 2^-24 (its subtraction, its product, log2 e / T as a float), and the mean of |x| over a row's terms is
+// log2 V, 24, at most; each of up to 20 rescalings on a term's way (threads, warps, slices; 55 with 13 million
+// ids) adds an exponential's 2^-22 and two roundings: 2^-15 a row at most, and there are two.
+constexpr double kVdDoubt = 1.0 / (1 << 14);
 // What rounding leaves of numbers that are alike, as a share of them: 64-bit sums of some hundred additions in a row.
 constexpr double kVdNothing = 1e-13;
 template <int kVdThreads, int kCtas, int kAhead>
@@ -397,7 +403,7 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
   enum { kDraw, kNothingLeft, kAgain };
   __shared__ int step_s;
   __shared__ double weight_s;
-  __shared__ int first_bad;
+  __shared__ int first_bad;                               // 2 j: draft j does not stand; 2 j + 1: it may
   cg::cluster_group cluster = cg::this_cluster();
   const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -429,6 +435,7 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
       if (proposed) yd = a.draft_logits[b * a.ld_seq + j * a.ld_place + d];
     }
   };
+  int have = tid < n ? tid : -1;                          // whose numbers they are
   if (tid < n) draft(tid);
   for (int i = warp; i < (proposed ? 2 * n + 1 : n + 1); i += kWarps) {
     const size_t row = i <= n ? row0 + i : a.n_rows + (size_t)b * a.K + (i - n - 1);
@@ -445,24 +452,64 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
   }
   __syncthreads();
   // ---- which drafts stand
-  for (int j = tid; j < n; j += kVdThreads) {
-    if (j != tid) draft(j);
-    bool stands = false;
-    if (d >= 0 && d < a.V) {
-      VfTerm t;
-      t.set(rows[j].m, a.log2_t, a.reach);
-      const double px = t(xd, table) / (double)rows[j].z;
-      double qx = 1.0;
-      if (proposed) {
-        t.set(rows[n + 1 + j].m, a.log2_t, a.reach);
-        qx = t(yd, table) / (double)rows[n + 1 + j].z;
-      }
-      stands = (double)u * qx < px;
+  VfTerm tp, tq;
+  // draft j's p and q as they compare with u, given its rows' sums
+  auto judge = [&](int j, double zp, double zq, double& px, double& uq) {
+    if (j != have) { draft(j); have = j; }
+    px = 0.0;
+    uq = 0.0;
+    if (d < 0 || d >= a.V) return;
+    tp.set(rows[j].m, a.log2_t, a.reach);
+    px = tp(xd, table) / zp;
+    double qx = 1.0;
+    if (proposed) {
+      tq.set(rows[n + 1 + j].m, a.log2_t, a.reach);
+      qx = tq(yd, table) / zq;
     }
-    if (!stands) atomicMin(&first_bad, j);
+    uq = (double)u * qx;
+  };
+  // the 64-bit sum of a row, by the whole CTA (all CTAs of the cluster do the same)
+  auto row_sum = [&](const VfTerm& row, const float* x) {
+    const bool aligned = ((uintptr_t)x & 15) == 0;
+    double mine = 0.0;
+    for (int s = warp; s * kVdSeg < a.V; s += kWarps) {
+      float f[4];
+      double v[4];
+      vf_four(x, a.V, s * 32 + lane, aligned, f);
+      row.four(f, v, table);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (s * kVdSeg + 4 * lane + e < a.V) mine += v[e];
+    }
+    mine = vf_warp_sum(mine);
+    __syncthreads();
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+    double all = 0.0;
+    for (int w = 0; w < kWarps; ++w) all += sums[w];
+    return all;
+  };
+  int j;
+  for (int from = 0;; from = j + 1) {
+    for (int i = from + tid; i < n; i += kVdThreads) {
+      double px, uq;
+      judge(i, (double)rows[i].z, proposed ? (double)rows[n + 1 + i].z : 1.0, px, uq);
+      const bool doubt = px > 0.0 && fabs(uq - px) <= kVdDoubt * px;
+      if (doubt || !(uq < px)) atomicMin(&first_bad, 2 * i + (doubt ? 1 : 0));
+    }
+    __syncthreads();
+    const int code = first_bad;
+    j = min(code >> 1, n);
+    if (j == n || !(code & 1)) break;
+    double px, uq;
+    judge(j, 1.0, 1.0, px, uq);                           // (sets the terms)
+    const double zp = row_sum(tp, a.logits + (size_t)(row0 + j) * a.ld);
+    const double zq = proposed ? row_sum(tq, a.draft_logits + b * a.ld_seq + j * a.ld_place) : 1.0;
+    if (!(uq / zq < px / zp)) break;
+    __syncthreads();
+    if (tid == 0) first_bad = 0x7fffffff;
+    __syncthreads();
   }
-  __syncthreads();
-  const int j = min(first_bad, n);
   const bool rest = j < n;
   d = rest ? a.drafts[(size_t)b * a.ld_drafts + j] : -1;
   if (rest && (d < 0 || d >= a.V) && rank == 0 && tid == 0) atomicOr(a.fault, (unsigned)kFaultTokenRange);
@@ -471,7 +518,6 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
   const float* xp = a.logits + (size_t)(row0 + j) * a.ld;
   const float* xq = minus_q ? a.draft_logits + b * a.ld_seq + j * a.ld_place : xp;
   const bool ap = ((uintptr_t)xp & 15) == 0, aq = ((uintptr_t)xq & 15) == 0;
-  VfTerm tp, tq;
   tp.set(rows[j].m, a.log2_t, a.reach);
   tq = tp;
   double w0 = 0.0;

@@ -78,3 +78,69 @@ def test_the_same_answers_again(ops):
     first = verify(ops, s, 0.9, 0, s["draft_logits"])
     for _ in range(5):
         assert all(torch.equal(a, b) for a, b in zip(first, verify(ops, s, 0.9, 0, s["draft_logits"])))
+
+
+def at_the_border(B, K, V, seed, temperature, proposed):
+    """Every draft's number is within three steps of a 32-bit number of the one at which it no longer stands."""
+    gen = torch.Generator().manual_seed(seed)
+    logits = 2.5 * torch.randn((B * (K + 1), V), generator=gen)
+    draft_logits = logits.view(B, K + 1, V)[:, :K] + 0.5 * torch.randn((B, K, V), generator=gen)
+    drafts, u = torch.zeros((B, K), dtype=torch.int32), torch.zeros((B, K))
+    for b in range(B):
+        for j in range(K):
+            p = row_probabilities(logits[b * (K + 1) + j], temperature, 0)
+            if proposed:
+                q = row_probabilities(draft_logits[b, j], temperature, 0)
+                x = int(torch.where(p < 0.95 * q, q, torch.zeros_like(q)).argmax())
+                border = p[x] / q[x]
+            else:
+                x = int(p.argmax())
+                border = p[x]
+            drafts[b, j] = x
+            at = border.float()
+            # a third of them just below: they stand, and the next draft is judged
+            steps = [-3, -2, -1, 1, 0, 2, -1, 3][int(torch.randint(0, 8, (1,), generator=gen))]
+            for _ in range(abs(steps)):
+                at = torch.nextafter(at, torch.tensor(2.0 if steps > 0 else -1.0))
+            u[b, j] = at
+            assert abs(float(at) / float(border) - 1) > 1e-12    # (64-bit sums tell them)
+    nu = (torch.randint(0, 1 << 24, (B,), generator=gen).float() + 0.5) / (1 << 24)
+    return dict(logits=logits.cuda(), cu=((K + 1) * torch.arange(B + 1)).int().cuda(), drafts=drafts.cuda(),
+                draft_logits=draft_logits.contiguous().cuda(), accept_u=u.cuda(), next_u=nu.cuda())
+
+
+@pytest.mark.parametrize("proposed", [True, False])
+@pytest.mark.parametrize("B, K, V, temperature", [(40, 3, 49152, 0.7), (24, 3, 32003, 1.0), (3, 5, 49152, 1.7),
+                                                  (200, 2, 1001, 0.3), (16, 3, 151, 1.0)])
+def test_numbers_at_the_border(ops, B, K, V, temperature, proposed):
+    """A draft is judged as the definition has it however close its number lies."""
+    s = at_the_border(B, K, V, B + V, temperature, proposed)
+    q = s["draft_logits"] if proposed else None
+    accepted, tokens = verify(ops, s, temperature, 0, q)
+    want = by_definition(s["logits"], s["cu"], s["drafts"], s["accept_u"], s["next_u"], temperature, 0, q)
+    wrong = int((accepted.cpu() != want[0]).sum())
+    assert wrong == 0, f"{wrong} of {B} judged otherwise"
+    assert torch.equal(tokens.cpu(), want[1])
+    assert len(set(accepted.tolist())) > 1
+
+
+def test_a_border_behind_a_border_and_infinite_rows(ops):
+    """Rows whose largest entries are infinite are uniform over them; a number that is the border itself, exactly,
+    does not stand."""
+    B, K, V = 4, 2, 4099
+    gen = torch.Generator().manual_seed(9)
+    logits = torch.randn((B * (K + 1), V), generator=gen)
+    draft_logits = torch.randn((B, K, V), generator=gen)
+    logits[:, [5, 17, 100, 4000]] = float("inf")
+    draft_logits[:, :, [5, 17]] = float("inf")
+    drafts = torch.full((B, K), 17, dtype=torch.int32)
+    u = torch.full((B, K), 0.5)                            # p = 1/4, q = 1/2
+    u[1] = 0.5 - 2.0 ** -25
+    u[2, 1] = 0.5 - 2.0 ** -25
+    u[3, 0] = 0.5 - 2.0 ** -25
+    s = dict(logits=logits.cuda(), cu=((K + 1) * torch.arange(B + 1)).int().cuda(), drafts=drafts.cuda(),
+             draft_logits=draft_logits.cuda(), accept_u=u.cuda(), next_u=torch.tensor([0.1, 0.3, 0.6, 0.9]).cuda())
+    accepted, tokens = verify(ops, s, 1.0, 0, s["draft_logits"])
+    assert accepted.tolist() == [0, 2, 0, 1]
+    want = by_definition(s["logits"], s["cu"], s["drafts"], s["accept_u"], s["next_u"], 1.0, 0, s["draft_logits"])
+    assert torch.equal(accepted.cpu(), want[0]) and torch.equal(tokens.cpu(), want[1])
