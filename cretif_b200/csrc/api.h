@@ -567,18 +567,18 @@ int cretif_max_top_k(void);
 // next_u [B] in [0, 1).  accepted [B]; tokens [B, K + 1]: the drafts that stand, the token, then -1.
 // scratch: as many bytes as cretif_verify_scratch says, 8-byte aligned.
 long long cretif_verify_scratch(int n_rows, int B, int K, int V, int top_k, int draft_rows);
-int cretif_verify_drafts(const float* logits, int ld, int n_rows, const int* cu, const int* drafts,
-                         int ld_drafts, int K, const float* draft_logits, long long ld_seq,
-                         long long ld_place, const float* accept_u, int ld_u, const float* next_u,
+int cretif_verify_drafts(const float* logits, long long ld, int n_rows, const int* cu, const int* drafts,
+                         long long ld_drafts, int K, const float* draft_logits, long long ld_seq,
+                         long long ld_place, const float* accept_u, long long ld_u, const float* next_u,
                          int B, int V, double temperature, int top_k, int* accepted, int* tokens,
-                         int ld_tokens, void* scratch, unsigned int* fault, void* stream);
+                         long long ld_tokens, void* scratch, unsigned int* fault, void* stream);
 
 // Attention of few new tokens a sequence where groups of sequences share prefixes (attn_shared.cu).
 // plan: int32, n_pre prefix items of 8, n_own own items of 8 (each of up to own_rows rows), n_rows
 // tokens of the groups, [T] prefix pieces of a token.  part_o [max_pieces, T * nh, hd], part_ml
 // [max_pieces, T * nh, 2]: scratch.
-int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int ldo, const void* kc,
-                       const void* vc, long long n_blocks, const int* table, int table_stride,
+int cretif_attn_shared(const void* q, long long ldq, int dt, void* out, long long ldo, const void* kc,
+                       const void* vc, long long n_blocks, const int* table, long long table_stride,
                        int table_width, int n_slots, const int* tok_pos, const int* seq_slot,
                        const int* plan, int n_pre, int n_own, int own_rows, int own_splits, int max_pieces,
                        int n_rows, int T, int nh, int nkv, int hd, int bt, float scale,

@@ -288,9 +288,9 @@ static int launch_shared_f32(const SharedArgs& a, cudaStream_t st) {
 
 using namespace cretif;
 
-extern "C" int cretif_attn_shared(const void* q, int ldq, int dt, void* out, int ldo, const void* kc,
+extern "C" int cretif_attn_shared(const void* q, long long ldq, int dt, void* out, long long ldo, const void* kc,
                                   const void* vc, long long n_blocks, const int* table,
-                                  int table_stride, int table_width, int n_slots, const int* tok_pos,
+                                  long long table_stride, int table_width, int n_slots, const int* tok_pos,
                                   const int* seq_slot, const int* plan, int n_pre, int n_own,
                                   int own_rows, int own_splits, int max_pieces, int n_rows, int T, int nh,
                                   int nkv, int hd, int bt, float scale, const float* sink,

@@ -36,10 +36,11 @@ struct alignas(16) SharedOwnItem {
 struct SharedArgs {
   const void *q, *kc, *vc;
   void* out;
-  int ldq, ldo;
+  long long ldq, ldo;                      // (rows may lie more than 2^31 numbers apart)
   long long n_blocks;
   const int* table;
-  int table_stride, table_width, n_slots;     // (a row's places lie a stride apart; a view's may be fewer)
+  long long table_stride;
+  int table_width, n_slots;                // (a row's places lie a stride apart; a view's may be fewer)
   const int *tok_pos, *seq_slot;
   // the plan: prefix items, own items (of up to own_rows rows), the tokens of the groups, [T] prefix
   // pieces of a token

@@ -39,8 +39,8 @@ def lib():
         L.cretif_verify_scratch.restype = ctypes.c_longlong
         # (with the types named, plain integers go through: half the time of wrapping each)
         p, i, ll, f, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_double
-        L.cretif_attn_shared.argtypes = [p, i, i, p, i, p, p, ll, p, i, i, i, p, p, p] + [i] * 11 + [f, p, p, p, p, p]
-        L.cretif_verify_drafts.argtypes = [p, i, i, p, p, i, i, p, ll, ll, p, i, p, i, i, d, i, p, p, i, p, p, p]
+        L.cretif_attn_shared.argtypes = [p, ll, i, p, ll, p, p, ll, p, ll, i, i, p, p, p] + [i] * 11 + [f, p, p, p, p, p]
+        L.cretif_verify_drafts.argtypes = [p, ll, i, p, p, ll, i, p, ll, ll, p, ll, p, i, i, d, i, p, p, ll, p, p, p]
         L.cretif_uniform01.argtypes = [ctypes.c_ulonglong, ctypes.c_longlong, ctypes.c_int]
         _lib = L
     return _lib

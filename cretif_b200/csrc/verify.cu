@@ -34,21 +34,23 @@ constexpr int kVfMaxTopK = 1024;
 
 struct VfArgs {
   const float* logits;
-  int ld, n_rows;
+  long long ld;                 // (rows may lie more than 2^31 numbers apart)
+  int n_rows;
   const int* cu;
   const int* drafts;
-  int ld_drafts, K, B, V;
+  long long ld_drafts;
+  int K, B, V;
   const float* draft_logits;
   long long ld_seq, ld_place;
   const float* accept_u;
-  int ld_u;
+  long long ld_u;
   const float* next_u;
   double log2_t;                // log2 e / T, within what float32 holds
   float reach;                  // how far below the largest entry an entry counts: 1000 / log2_t
   int top_k;
   int* accepted;
   int* tokens;
-  int ld_tokens;
+  long long ld_tokens;
   unsigned int* fault;
   // what the first launch leaves: rows 0 .. n_rows - 1 are the logits', n_rows + b K + j draft j's
   void* stats;                  // [rows][slices] VfPart, with top_k [rows] VfKept, greedy [rows][slices] u64
@@ -1138,11 +1140,11 @@ extern "C" long long cretif_verify_scratch(int n_rows, int B, int K, int V, int 
   return rows * 8LL * (V / 4 / (kVsFew * kVsThreads) + 1);
 }
 
-extern "C" int cretif_verify_drafts(const float* logits, int ld, int n_rows, const int* cu,
-                                    const int* drafts, int ld_drafts, int K, const float* draft_logits,
+extern "C" int cretif_verify_drafts(const float* logits, long long ld, int n_rows, const int* cu,
+                                    const int* drafts, long long ld_drafts, int K, const float* draft_logits,
                                     long long ld_seq, long long ld_place, const float* accept_u,
-                                    int ld_u, const float* next_u, int B, int V, double temperature,
-                                    int top_k, int* accepted, int* tokens, int ld_tokens,
+                                    long long ld_u, const float* next_u, int B, int V, double temperature,
+                                    int top_k, int* accepted, int* tokens, long long ld_tokens,
                                     void* scratch, unsigned int* fault, void* stream) {
   if (B <= 0) return kOk;
   if (V <= 0 || ld < 0 || K < 0 || n_rows <= 0 || (B > 1 && ld_tokens < K + 1) || top_k < 0 ||
