@@ -1589,8 +1589,9 @@ def verify_drafts(logits, cu_rows, drafts, accept_u, next_u, accepted, tokens, t
     q = ld_seq = ld_place = 0
     if draft_logits is not None and temperature > 0 and K:   # (a greedy draft is judged by the arg max alone)
         q, ld_seq, ld_place = draft_logits.data_ptr(), ql[0], ql[1]
-    scratch = torch.empty(_verify_scratch(R, B, K, V, top_k if temperature > 0 else 0, q != 0), dtype=torch.float64,
-                          device=logits.device)
+    if temperature <= 0 or top_k >= V:                       # (of any size, beyond 32 bits too: all ids are kept)
+        top_k = 0
+    scratch = torch.empty(_verify_scratch(R, B, K, V, top_k, q != 0), dtype=torch.float64, device=logits.device)
     _check((_lib or lib()).cretif_verify_drafts(
         logits.data_ptr(), ll[0], R, cu_rows.data_ptr(), drafts.data_ptr(), dl[0], K, q, ld_seq, ld_place,
         accept_u.data_ptr(), ul[0], next_u.data_ptr(), B, V, temperature, top_k, accepted.data_ptr(), tokens.data_ptr(),

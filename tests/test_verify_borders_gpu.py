@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_verify_drafts_gpu import by_definition, row_probabilities, verify
+from test_verify_drafts_gpu import by_definition, make, row_probabilities, verify
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,12 @@ def test_a_border_behind_a_border_and_infinite_rows(ops):
     assert accepted.tolist() == [0, 2, 0, 1]
     want = by_definition(s["logits"], s["cu"], s["drafts"], s["accept_u"], s["next_u"], 1.0, 0, s["draft_logits"])
     assert torch.equal(accepted.cpu(), want[0]) and torch.equal(tokens.cpu(), want[1])
+
+
+@pytest.mark.parametrize("temperature", [0.8, 0.0])
+def test_a_top_k_beyond_the_vocabulary_is_none(ops, temperature):
+    s = make(6, 3, 2000, [3, 2, 3, 1, 3, 3], seed=21, temperature=temperature, top_k=0)
+    want = verify(ops, s, temperature, 0, s["draft_logits"])
+    for top_k in (2000, 2001, 2 ** 31, 2 ** 32 + 2, 2 ** 40):
+        got = verify(ops, s, temperature, top_k, s["draft_logits"])
+        assert all(torch.equal(a, b) for a, b in zip(want, got)), top_k
