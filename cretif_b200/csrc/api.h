@@ -575,12 +575,12 @@ int cretif_verify_drafts(const float* logits, long long ld, int n_rows, const in
 
 // Attention of few new tokens a sequence where groups of sequences share prefixes (attn_shared.cu).
 // plan: int32, n_pre prefix items of 8, n_own own items of 8 (each of up to own_rows rows), n_rows
-// tokens of the groups, [T] prefix pieces of a token.  part_o [max_pieces, T * nh, hd], part_ml
-// [max_pieces, T * nh, 2]: scratch.
+// tokens of the groups, their first pieces, [T + 1] first pieces of all tokens.  part_o [first[T], nh, hd],
+// part_ml [first[T], nh, 2]: scratch.
 int cretif_attn_shared(const void* q, long long ldq, int dt, void* out, long long ldo, const void* kc,
                        const void* vc, long long n_blocks, const int* table, long long table_stride,
                        int table_width, int n_slots, const int* tok_pos, const int* seq_slot,
-                       const int* plan, int n_pre, int n_own, int own_rows, int own_splits, int max_pieces,
+                       const int* plan, int n_pre, int n_own, int own_rows, int own_splits,
                        int n_rows, int T, int nh, int nkv, int hd, int bt, float scale,
                        const float* sink, float* part_o, float* part_ml, unsigned int* fault,
                        void* stream);

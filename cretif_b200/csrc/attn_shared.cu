@@ -25,7 +25,7 @@ shared_pieces_kernel(const SharedArgs a) {
   float* ks = qs + kShRows * ldk;             // [64][hd + 4]
   float* vs = ks + kShBlk * ldk;              // [64][hd]
   float* ps = vs + kShBlk * hd;               // [32][64]
-  __shared__ int toks[kShRows];
+  __shared__ int toks[kShRows], firsts[kShRows];   // a row's token, and that token's first piece
   const int kvh = blockIdx.y, g = a.nh / a.nkv, tid = threadIdx.x;
   const int warp = tid >> 5, lane = tid & 31;
   constexpr int kRows = kShRows / 8;          // of a warp
@@ -46,7 +46,7 @@ shared_pieces_kernel(const SharedArgs a) {
     const int blocks = (end - prefix + kShBlk - 1) / kShBlk;
     key0 = prefix + (int)((long long)blocks * split / a.own_splits) * kShBlk;
     key_end = min(end, prefix + (int)((long long)blocks * (split + 1) / a.own_splits) * kShBlk);
-    piece = a.max_pieces - a.own_splits + split;
+    piece = it.pieces + split;
   }
   // a thread's share of a step's tile: keys tid / quads, + step, ...; at most 8 of four channels
   const int slot = a.seq_slot[seq];
@@ -71,6 +71,7 @@ shared_pieces_kernel(const SharedArgs a) {
   if (tid < kShRows) {
     const int r = row0 + tid;
     toks[tid] = tid >= n_rows ? -1 : row_base >= 0 ? a.rows[row_base + r / g] : tok0 + r / g;
+    firsts[tid] = tid >= n_rows ? 0 : row_base >= 0 ? a.rows_first[row_base + r / g] : a.first[tok0 + r / g];
   }
   __syncthreads();
   for (int i = tid; i < kShRows * quads; i += kShThreads) {
@@ -189,7 +190,7 @@ shared_pieces_kernel(const SharedArgs a) {
   for (int i = 0; i < kRows; ++i)
     if (i < mine) {
       const int r = warp + 8 * i;
-      const size_t row = ((size_t)piece * a.T + toks[r]) * a.nh + kvh * g + (row0 + r) % g;
+      const size_t row = ((size_t)firsts[r] + piece) * a.nh + kvh * g + (row0 + r) % g;
       if (lane == 0) a.part_ml[row] = make_float2(m[i], l[i]);
       if (has_d) {
         float* to = a.part_o + row * hd + d0;
@@ -206,10 +207,8 @@ __global__ void __launch_bounds__(kShThreads) shared_join_kernel(const SharedArg
   dependent_begin();
   const int row = blockIdx.x * (kShThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= a.T * a.nh) return;
-  const int t = row / a.nh, h = row - t * a.nh, pre = a.tok_pieces[t];
-  const size_t stride = (size_t)a.T * a.nh;
-  const int own0 = a.max_pieces - a.own_splits, n = pre + a.own_splits;
-  auto at = [&](int i) { return (i < pre ? i : own0 + i - pre) * stride + row; };
+  const int t = row / a.nh, h = row - t * a.nh, first = a.first[t], n = a.first[t + 1] - first;
+  auto at = [&](int i) { return ((size_t)first + i) * a.nh + h; };
   // `side` groups of `wide` lanes (a power of two, at least hd / 4) take the pieces in turns
   int wide = 4;
   while (wide < a.hd >> 2) wide <<= 1;
@@ -292,12 +291,12 @@ extern "C" int cretif_attn_shared(const void* q, long long ldq, int dt, void* ou
                                   const void* vc, long long n_blocks, const int* table,
                                   long long table_stride, int table_width, int n_slots, const int* tok_pos,
                                   const int* seq_slot, const int* plan, int n_pre, int n_own,
-                                  int own_rows, int own_splits, int max_pieces, int n_rows, int T, int nh,
+                                  int own_rows, int own_splits, int n_rows, int T, int nh,
                                   int nkv, int hd, int bt, float scale, const float* sink,
                                   float* part_o, float* part_ml, unsigned int* fault, void* stream) {
   if (T <= 0) return kOk;
   if (nh <= 0 || nkv <= 0 || nh % nkv || hd % 16 || hd < 16 || hd > 128 || bt != kShBlk || own_rows <= 0 ||
-      n_pre < 0 || n_own <= 0 || own_splits <= 0 || max_pieces < own_splits || n_rows < 0 ||
+      n_pre < 0 || n_own <= 0 || own_splits <= 0 || n_rows < 0 ||
       nkv > 65535 || (long long)T * nh > (1LL << 30) || n_blocks <= 0 || !(scale > 0.f) ||
       (long long)n_pre + (long long)n_own * own_splits > 0x7fffffffLL)
     return kBadArgument;
@@ -312,8 +311,9 @@ extern "C" int cretif_attn_shared(const void* q, long long ldq, int dt, void* ou
   a.pre = reinterpret_cast<const SharedPrefixItem*>(plan);
   a.own = reinterpret_cast<const SharedOwnItem*>(plan + 8 * (size_t)n_pre);
   a.rows = plan + 8 * ((size_t)n_pre + n_own);
-  a.tok_pieces = a.rows + n_rows;
-  a.n_pre = n_pre; a.n_own = n_own; a.own_rows = own_rows; a.own_splits = own_splits; a.max_pieces = max_pieces; a.T = T;
+  a.rows_first = a.rows + n_rows;
+  a.first = a.rows_first + n_rows;
+  a.n_pre = n_pre; a.n_own = n_own; a.own_rows = own_rows; a.own_splits = own_splits; a.T = T;
   a.nh = nh; a.nkv = nkv; a.hd = hd; a.scale_log2 = scale * 1.4426950408889634f; a.sink = sink;
   a.part_o = part_o; a.part_ml = reinterpret_cast<float2*>(part_ml); a.fault = fault;
   if (dt == kF32)

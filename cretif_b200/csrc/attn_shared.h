@@ -29,7 +29,7 @@ struct alignas(16) SharedOwnItem {
   int seq, tok0, row0, n_rows;
   int prefix, pieces;                      // tokens that are other items' work, and pieces they are in
   int least;                               // the least position of the sequence: the tokens it shares
-  int pad;
+  int first;                               // token tok0's first piece
 };
 
 // What every kernel of a call reads.
@@ -42,17 +42,18 @@ struct SharedArgs {
   long long table_stride;
   int table_width, n_slots;                // (a row's places lie a stride apart; a view's may be fewer)
   const int *tok_pos, *seq_slot;
-  // the plan: prefix items, own items (of up to own_rows rows), the tokens of the groups, [T] prefix
-  // pieces of a token
+  // The plan: prefix items, own items (of up to own_rows rows), the tokens of the groups, and where the pieces
+  // lie: a token has as many as it needs, one behind the other, so that a long prefix of few sequences costs
+  // the others no room.  [n_rows] first piece of the groups' tokens, [T + 1] of all.
   const SharedPrefixItem* pre;
   const SharedOwnItem* own;
-  const int *rows, *tok_pieces;
-  int n_pre, n_own, own_rows, own_splits, max_pieces, T;
+  const int *rows, *rows_first, *first;
+  int n_pre, n_own, own_rows, own_splits, T;
   int nh, nkv, hd;
   float scale_log2;
   const float* sink;
-  float* part_o;                           // [pieces][T * nh][hd]
-  float2* part_ml;                         // [pieces][T * nh]
+  float* part_o;                           // [pieces of all tokens][nh][hd]
+  float2* part_ml;                         // [pieces of all tokens][nh]
   unsigned int* fault;
 };
 

@@ -310,7 +310,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       if (there) {
         const int token = a.rows[it.row_base + of];
         src = static_cast<const __nv_bfloat16*>(a.q) + (size_t)token * a.ldq + (size_t)head * hd;
-        at = ((size_t)it.piece * a.T + token) * a.nh + head;
+        at = ((size_t)a.rows_first[it.row_base + of] + it.piece) * a.nh + head;
       }
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
       if (n_sub == 1) {                                   // two channels a column
@@ -635,11 +635,11 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   if (WPI == 1) __syncwarp();
   else __syncthreads();
   const int quads = hd >> 2, n_pieces = JOIN ? it.pieces : 0;
-  const size_t rows_all = (size_t)a.T * a.nh;
+  const int pieces_a_token = it.pieces + (JOIN ? 0 : a.own_splits);
   for (int i = warp * 32 + lane; i < it.n_rows * quads; i += WPI * 32) {
     const int row = i / quads, ch = (i - row * quads) * 4, rr = it.row0 + row;
     const int t = it.tok0 + rr / g, h = kvh * g + rr % g;
-    const size_t at = (size_t)t * a.nh + h;
+    const size_t at = ((size_t)it.first + (size_t)(t - it.tok0) * pieces_a_token) * a.nh + h;
     float ref = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     // N parts at a time: one wait for their loads, one move of the reference
@@ -668,7 +668,7 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
       for (int e = 0; e < kAtOnce; ++e) {
         const bool in = p0 + e < n_pieces;
-        const size_t from = (size_t)(in ? p0 + e : p0) * rows_all + at;
+        const size_t from = (size_t)(in ? p0 + e : p0) * a.nh + at;
         ml[e] = __ldcg(&a.part_ml[from]);
         x[e] = __ldcg(reinterpret_cast<const float4*>(a.part_o + from * hd + ch));
         if (!in) ml[e] = make_float2(-INFINITY, 0.f);
@@ -694,7 +694,7 @@ shared_own_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       const uint2 packed = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
       *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)t * a.ldo + (size_t)h * hd + ch) = packed;
     } else {
-      const size_t to = (size_t)(a.max_pieces - a.own_splits + split) * rows_all + at;
+      const size_t to = (size_t)(it.pieces + split) * a.nh + at;
       if (ch == 0) a.part_ml[to] = make_float2(ref, den);
       *reinterpret_cast<float4*>(a.part_o + to * hd + ch) = acc;
     }

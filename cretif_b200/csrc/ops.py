@@ -39,7 +39,7 @@ def lib():
         L.cretif_verify_scratch.restype = ctypes.c_longlong
         # (with the types named, plain integers go through: half the time of wrapping each)
         p, i, ll, f, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_double
-        L.cretif_attn_shared.argtypes = [p, ll, i, p, ll, p, p, ll, p, ll, i, i, p, p, p] + [i] * 11 + [f, p, p, p, p, p]
+        L.cretif_attn_shared.argtypes = [p, ll, i, p, ll, p, p, ll, p, ll, i, i, p, p, p] + [i] * 10 + [f, p, p, p, p, p]
         L.cretif_verify_drafts.argtypes = [p, ll, i, p, p, ll, i, p, ll, ll, p, ll, p, i, i, d, i, p, p, ll, p, p, p]
         L.cretif_uniform01.argtypes = [ctypes.c_ulonglong, ctypes.c_longlong, ctypes.c_int]
         _lib = L
@@ -1987,21 +1987,27 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
     if dtype == torch.bfloat16 and nkv > 0 and (max(news, default=1) * nh // nkv <= 8
                                                 or sum(-(-n * nh // nkv // 16) for n in news) * nkv <= ctas // 2):
         own_rows = 8
-    pre, own, splits, pieces, rows, tok_pieces, prefix_of = _shared_items(groups, news, starts, nh, nkv, hd, tile_rows,
-                                                                          own_rows, ctas, walk,
-                                                                          8 if dtype == torch.bfloat16 else 2)
+    pre, own, splits, _, rows, tok_pieces, prefix_of = _shared_items(groups, news, starts, nh, nkv, hd, tile_rows,
+                                                                     own_rows, ctas, walk,
+                                                                     8 if dtype == torch.bfloat16 else 2)
+    whole = dtype == torch.bfloat16 and splits == 1      # the own keys' kernel joins, and leaves no piece
+    first = [0]                                          # a token's pieces lie one behind the other
+    for n in tok_pieces:
+        first.append(first[-1] + n + (0 if whole else splits))
+    if first[-1] >= 1 << 31:
+        raise KernelError(f"shared prefix: {first[-1]} pieces of {len(tok_pieces)} tokens")
+    own[7::8] = [first[t] for t in own[1::8]]
     plan = SharedPrefixPlan()
-    packed = torch.tensor(pre + own + rows + tok_pieces, dtype=torch.int32)
+    packed = torch.tensor(pre + own + rows + [first[t] for t in rows] + first, dtype=torch.int32)
     plan.data = packed.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else packed
     plan.device, plan.T, plan.B = plan.data.device, len(tok_pieces), len(prefix_of)
     if dev.type == "cuda":
         plan.stream = _stream_of(plan.data.get_device())
         plan.made = torch.cuda.current_stream(plan.device).record_event()
     plan.sizes = (nh, nkv, hd, plan.T, plan.B, dtype, plan.data.get_device())
-    # as the C entry takes them: items, splits, pieces, tokens of the groups, T, heads, head size
-    plan.launch = (len(pre) // 8, len(own) // 8, own_rows, splits, pieces, len(rows), plan.T, nh, nkv, hd)
-    whole = dtype == torch.bfloat16 and splits == 1      # the own keys' kernel joins, and leaves no piece
-    plan.pieces = pieces - 1 if whole else pieces
+    # as the C entry takes them: items, splits, tokens of the groups, T, heads, head size
+    plan.launch = (len(pre) // 8, len(own) // 8, own_rows, splits, len(rows), plan.T, nh, nkv, hd)
+    plan.pieces = first[-1]                              # of all tokens: what a call's scratch holds
     plan.kernels = (1 if whole else 2) + (1 if pre and dtype == torch.bfloat16 else 0)
     plan.prefix_blocks = max(prefix_of) // 64
     return plan
@@ -2047,7 +2053,7 @@ def attn_shared(q, out, kc, vc, table, tok_pos, cu_seqlens, seq_slot, plan: Shar
         plan.data.record_stream(here)
     part_o = part_ml = 0
     if plan.pieces:
-        n = plan.pieces * T * nh
+        n = plan.pieces * nh
         scratch = torch.empty(n * (hd + 2), dtype=torch.float32, device=plan.device)
         part_o = scratch.data_ptr()
         part_ml = part_o + 4 * n * hd
