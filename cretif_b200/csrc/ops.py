@@ -1960,6 +1960,12 @@ WALKED_TOKENS = 256
 WALKED_BYTES = 40 << 20
 
 
+def shared_prefix_walked(groups, nkv: int, hd: int) -> bool:
+    """Whether a bfloat16 step's prefixes are short enough to be walked."""
+    return all(p <= WALKED_TOKENS for _, p in groups) and sum(
+        p * len(m) for m, p in groups) * nkv * hd * 4 <= WALKED_BYTES
+
+
 def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, device) -> SharedPrefixPlan:
     """The plan of a step for :func:`attn_shared`.  ``groups``: (sequences of the step, tokens they
     share) pairs; the shared tokens are whole cache blocks of 64 that the members' tables name alike.
@@ -1976,10 +1982,7 @@ def shared_prefix_plan(groups, news, starts, nh: int, nkv: int, hd: int, dtype, 
     ctas = 2 * (sm_count(dev) if dev.type == "cuda" else 148)
     if dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
         raise KernelError("shared prefix: a plan is made before a capture (its arrays are copied from the host)")
-    walk = False
-    if dtype == torch.bfloat16 and all(p <= WALKED_TOKENS for _, p in groups) and sum(
-            p * len(m) for m, p in groups) * nkv * hd * 4 <= WALKED_BYTES:
-        walk = True
+    walk = dtype == torch.bfloat16 and shared_prefix_walked(groups, nkv, hd)
     tile_rows, own_rows = (128, 16) if dtype == torch.bfloat16 else (32, 32)
     # Own keys in items of 8 rows where the sequences have no more, or where items of 16 would not give every SM
     # one (15 heads on 5, 24 sequences of up to 15 rows: 18.3 us with 16, 16.9 with 8; 16 heads of 128 on 2, 33 of up

@@ -107,14 +107,45 @@ def distance_edges(rows: int, far: float):
 FAST_BIAS_MAX_DISTANCES = 4096
 
 
-# A step of single tokens takes the attention over shared prefixes where that spares this much reading, or
-# where the prefix is this long: below, two launches and the joining cost more than the keys (ordinary decode
-# attention against shared, us: 9 heads on 3, 8 sequences on 2,048 tokens (11 MB) 6.9 / 7.8, 32 on 1,024 (24 MB)
-# 8.5 / 7.9; 32 on 32, 2 on 2,048 (17 MB) 9.7 / 9.8, 8 on 2,048 (117 MB) 26.2 / 10.6; 9 on 3, 2 on 8,192 (6 MB)
-# 15.2 / 9.8).  A step with drafts always takes it (4 tokens each, 8 sequences on 2,048 tokens: prompt attention
-# 22.9 / 10.2; on 64 tokens 5.9 / 4.4).
-SHARED_MIN_BYTES = 16 << 20
-SHARED_LONG = 4096
+# What a step of single tokens has to spare of reading, for each microsecond or so that the attention over shared
+# prefixes takes more than the ordinary kernel besides.
+SHARED_MIN_BYTES = 4 << 20
+
+
+def shared_pays(groups, news, starts, nh: int, nkv: int, hd: int) -> bool:
+    """Whether a step takes the attention over shared prefixes, by what was measured of both (1,700 steps: 2 to 64
+    sequences, 1 to 29 groups and sequences that share nothing, 4 to 12,000 own tokens, up to 16 new ones, 9 head
+    layouts; a sequence's tokens are ``starts`` + ``news``).
+
+    Single tokens, heads of up to 64: a second launch for the prefix, and own keys, which the ordinary kernel
+    deals out over more CTAs, cost what 4 MB and 24 MB a thousand tokens of reading do; so does a tenth of what
+    is read either way.  (ordinary / shared, us: 9 heads on 3, 8 sequences on 2,048 tokens 6.9 / 7.8, 32 on 1,024 8.5 / 7.9;
+    32 on 32, 8 on 2,048 26.2 / 10.6, 6 on 576 and 1,700 own tokens 18.0 / 25.8.)  Of 415 steps 9 are slower than the
+    other kernel would be by more than 5 %, at most 1.35 times, and 38 are left to the ordinary kernel that would
+    gain.  Wider heads: the ordinary kernel needs more for few keys, so all walked prefixes gain (16 on 2, 32
+    sequences on 256 tokens 17.9 / 8.2), others from 8 MB on, long own keys that are twice what is spared excepted (16 on
+    16, 10 sequences, 3 of them on 4,800 tokens, 5,700 own ones 91 / 146).  Of 325 steps 15 are slower, at most 1.5 times.
+    Several tokens: always (4 tokens each, 8 sequences on 2,048 tokens, prompt attention 22.9 / 10.2; none of 521 steps
+    was slower), but for wide heads of few sequences that are short (16 on 16, 3 sequences, up to 16 new tokens on
+    448 tokens 11.3 / 15.0): 12 of 439 steps slower, at most 1.4 times.  Of 700 steps drawn afterwards 11 are
+    slower, at most 1.36 times."""
+    token = nkv * hd * 4                             # bytes of a token's keys and values
+    ends = [s + n for s, n in zip(starts, news)]
+    walked, wide = ops.shared_prefix_walked(groups, nkv, hd), hd > 64
+    if max(news) > 1:
+        return walked or not wide or len(ends) > 8 or max(ends) > 512
+    alone = list(ends)                               # tokens of a sequence's own
+    for members, prefix in groups:
+        for b in members:
+            alone[b] -= prefix
+    spared = sum((len(m) - 1) * p for m, p in groups) * token
+    if wide:
+        if max(alone) > 1000 and spared < sum(alone) * token / 2:
+            return False
+        return spared >= (0 if walked else 2) * SHARED_MIN_BYTES
+    read = (sum(alone) + sum(p for _, p in groups)) * token
+    need = (1 if walked else 2) + 6 * max(alone) / 1000 + read / 40e6
+    return spared >= need * SHARED_MIN_BYTES
 
 
 def shared_plan(ctx, nh: int, nkv: int, hd: int, dtype):
@@ -123,11 +154,9 @@ def shared_plan(ctx, nh: int, nkv: int, hd: int, dtype):
     plans = ctx.extras.setdefault("shared_plans", {})
     key = (nh, nkv, hd)
     if key not in plans:
-        groups, news, starts = ctx.extras["shared"]
-        spared = sum((len(m) - 1) * p for m, p in groups) * nkv * hd * 4
-        plans[key] = None
-        if max(news) > 1 or spared >= SHARED_MIN_BYTES or max(p for _, p in groups) >= SHARED_LONG:
-            plans[key] = ops.shared_prefix_plan(groups, news, starts, nh, nkv, hd, dtype, ctx.device)
+        shared = ctx.extras["shared"]
+        plans[key] = ops.shared_prefix_plan(*shared, nh, nkv, hd, dtype, ctx.device) if shared_pays(
+            *shared, nh, nkv, hd) else None
     return plans[key]
 
 
