@@ -34,6 +34,7 @@ import torch
 from ..cache import SequenceCache
 from ..config import load_config
 from ..csrc import ops
+from ..parts.attention import shared_pays
 from ..parts.base import StepContext
 from ..weights import load_weights
 from .model import Model, manifest
@@ -177,6 +178,7 @@ class Engine:
                                    self.device, block_tokens=block_tokens, max_slots=max_slots,
                                    max_len=longest)
         self.model.prepare(self.cache.max_len)
+        self._shared_heads = self.model.shared_heads()
         self.fault = ops.fault_word(self.device)
         self.vocab_size = self.spec.vocab_size
         # Steps whose shape (tokens per sequence, wanted places) repeats are captured as CUDA
@@ -235,13 +237,21 @@ class Engine:
             seq_slot_host=tuple(slots), seq_start_host=tuple(starts), seq_new_host=tuple(news))
 
     def shared_prefixes(self, slots, starts, news):
-        """What the attention of a step may read once for several sequences: (groups, tokens a sequence
-        brings, cached tokens), or None.  Only for bfloat16: in float32 a token's bits do not depend on
+        """What the attention of a step reads once for several sequences: (groups, tokens a sequence
+        brings, cached tokens), or None, also where no layer gains by it: such a step is one like any
+        other, and shares their graphs.  Only for bfloat16: in float32 a token's bits do not depend on
         the rest of its step."""
-        if self.dtype != torch.bfloat16 or max(news) > SHARED_MAX_NEW:
+        if self.dtype != torch.bfloat16 or max(news) > SHARED_MAX_NEW or not self._shared_heads:
             return None
         groups = self.cache.shared_groups(slots)
-        return (groups, tuple(int(n) for n in news), tuple(int(s) for s in starts)) if groups else None
+        if not groups:
+            return None
+        shared = groups, tuple(int(n) for n in news), tuple(int(s) for s in starts)
+        return shared if self.shares(shared) else None
+
+    def shares(self, shared) -> bool:
+        """Whether any layer reads what is shared once."""
+        return any(shared_pays(*shared, *heads) for heads in self._shared_heads)
 
     @staticmethod
     def shared_make_up(shared) -> tuple:

@@ -184,17 +184,26 @@ class DecodeRunner:
         self.B = B
         self.shared = self.engine.shared_prefixes([int(s) for s in slots], [int(p) for p in positions], [1] * B)
         self.make_up = None if self.shared is None else self.engine.shared_make_up(self.shared)
+        self.shares: Dict[int, Optional[tuple]] = {}   # by the bucket of own keys: what the step shares
         self.longest = max(int(p) for p in positions) + 1
         if len(self.plans) > 64:                   # (of batches long gone; graphs keep their own)
             self.plans.clear()
 
-    def _shared_key(self, context: int) -> tuple:
-        """What a plan, and a graph that holds it, are kept by when the longest sequence holds ``context``
-        tokens: what is shared, and the bucket of the own keys that the plan was made for."""
+    def _shared_at(self, context: int):
+        """(what the step shares, or None, and what a plan and a graph that holds it are kept by) when
+        the longest sequence holds ``context`` tokens: the groups, and the bucket of the own keys that
+        the plan was made for.  Where own keys have grown so long that no layer shares, nothing."""
         if self.make_up is None:
-            return ()
-        groups, own = self.make_up
-        return groups + (self.engine.context_bucket(own + context - self.longest),)
+            return None, ()
+        grown = context - self.longest
+        make_up, own = self.make_up
+        bucket = self.engine.context_bucket(own + grown)
+        if bucket not in self.shares:
+            groups, news, starts = self.shared
+            shared = groups, news, tuple(s + grown for s in starts)
+            self.shares[bucket] = shared if self.engine.shares(shared) else None
+        shared = self.shares[bucket]
+        return shared, () if shared is None else make_up + (bucket,)
 
     def _body(self, b: dict, B: int, context: int) -> None:
         eng = self.engine
@@ -202,10 +211,10 @@ class DecodeRunner:
                           tok_seq=b["tok_seq"], seq_slot=b["seq_slot"],
                           seq_start=b["seq_start"], cu_seqlens=b["cu"], is_decode=True,
                           max_new=1, max_context=context)
-        if self.shared is not None:
-            groups, news, starts = self.shared
-            ctx.extras["shared"] = groups, news, tuple(s + context - self.longest for s in starts)
-            ctx.extras["shared_plans"] = self.plans.setdefault((B,) + self._shared_key(context), {})
+        shared, key = self._shared_at(context)
+        if shared is not None:
+            ctx.extras["shared"] = shared
+            ctx.extras["shared_plans"] = self.plans.setdefault((B,) + key, {})
         logits = eng.model.forward(ctx, eng.cache, None)
         b["logits"] = logits
         self.sampler(logits, b["sampled"], b["request"], b["draw"])
@@ -219,7 +228,7 @@ class DecodeRunner:
         if not self.use_graph:
             self._body(b, B, context)
             return b["sampled"]
-        shared_key = self._shared_key(context)
+        _, shared_key = self._shared_at(context)
         key = (B, self.engine.context_bucket(context), shared_key)
         if key not in self.graphs:
             # Warm up outside the capture (lazy initialisation, kernel loading), restoring

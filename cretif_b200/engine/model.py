@@ -168,6 +168,17 @@ class Model:
                     out[(i, k, "shift")] = br.shift.cache_request()
         return out
 
+    def shared_heads(self) -> List[Tuple[int, int, int]]:
+        """(heads, key/value heads, head size) of the mixers that may take the attention over shared
+        prefixes, each once."""
+        out = set()
+        for part in self._parts:
+            for _, p in part.sub_mixers() if hasattr(part, "sub_mixers") else [(None, part)]:
+                heads = p.shared_heads() if hasattr(p, "shared_heads") else None
+                if heads is not None:
+                    out.add(heads)
+        return sorted(out)
+
     @staticmethod
     def _keepers(i: int, k: int, part):
         """(cache id, part) of everything that keeps something in branch k of entry i."""

@@ -148,6 +148,11 @@ def shared_pays(groups, news, starts, nh: int, nkv: int, hd: int) -> bool:
     return spared >= need * SHARED_MIN_BYTES
 
 
+def shared_takes(hd: int) -> bool:
+    """Whether the attention over shared prefixes has heads of this size."""
+    return hd <= 128 and hd % 16 == 0
+
+
 def shared_plan(ctx, nh: int, nkv: int, hd: int, dtype):
     """The step's plan for :func:`ops.attn_shared`, made once for layers of these sizes; None where the
     step shares nothing that is worth it."""
@@ -185,7 +190,7 @@ def run_attention(q, o, ctx, kv, nh, nkv, hd, scale, window, dtype, sink=None, v
     context = ctx.max_context if pool is None else min(
         ctx.max_context, window + 64 + ctx.max_context // pool.pool)
     if (fast and window == 0 and "shared" in ctx.extras and kv.window == 0 and bias is None and slope is None and pool is None
-            and hd <= 128 and hd % 16 == 0 and kv.block_tokens == 64 and q.stride(0) % 8 == 0
+            and shared_takes(hd) and kv.block_tokens == 64 and q.stride(0) % 8 == 0
             and q.data_ptr() % 16 == 0):
         plan = shared_plan(ctx, nh, nkv, hd, dtype)
         if plan is not None:
@@ -694,6 +699,11 @@ class Attention(Part):
                       self.dtype, self.sink, vd=self.vd, bias=self.bias,
                       bias_edges=self.bias_edges, bias_dense=self.bias_dense, slope=self.slope,
                       slope_log2e=self.slope_log2e, pool=kv.pool if self.pool else None)
+
+    def shared_heads(self):
+        """(heads, key/value heads, head size) of steps that may take the attention over shared prefixes."""
+        other = self.mask or self.pool or self.distance_bias or self.slope_spec or self.vd != self.hd
+        return None if other or not shared_takes(self.hd) else (self.nh, self.nkv, self.hd)
 
     def weight_bytes(self):
         return (self.w_qkv.numel() + self.w_o.numel()) * self.w_qkv.element_size()

@@ -10,7 +10,8 @@ embedding        ``forward(ids[T] int32, ctx) -> h[T, H] float32``
 norm             ``forward(h, delta, rows=None, write_h=True) -> n[R, H]``:
                  ``h += delta`` (when given), ``n = norm(h)`` in the compute dtype
 mixer            ``forward(x[T, H], ctx, cache) -> y[T, H]`` (any float dtype);
-                 ``cache_request()`` says what it keeps between steps
+                 ``cache_request()`` says what it keeps between steps, ``shared_heads()``, where it
+                 has one, which heads read prefixes that sequences share once for all of them
 feed_forward     ``forward(x[T, H], ctx) -> y[T, H]``
 position         used by a mixer; ``rotate_and_store(qkv, ctx, kv_view, ...)``
 head             ``forward(n[R, H], ctx) -> logits[R, V] float32``

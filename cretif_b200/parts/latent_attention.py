@@ -32,7 +32,7 @@ from ..cache import KVRequest
 from ..config.spec import PartSpec
 from ..csrc import ops
 from ..weights.loader import WeightSpec
-from .attention import run_attention
+from .attention import run_attention, shared_takes
 from .base import Part, build_part, register_part
 from .linear import linear_few as linear
 
@@ -135,6 +135,9 @@ class LatentAttention(Part):
     def prepare(self, max_positions: int) -> None:
         if self.position is not None:
             self.position.prepare(max_positions)
+
+    def shared_heads(self):
+        return None if self.window or not shared_takes(self.key_dim) else (self.nh, 1, self.key_dim)
 
     def cache_request(self):
         return KVRequest(1, self.key_dim, self.window, shared_values=True)
