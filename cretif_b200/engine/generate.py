@@ -152,7 +152,6 @@ class DecodeRunner:
         use_graph = use_graph and engine.model.graph_safe
         self.engine, self.sampler, self.use_graph = engine, sampler, use_graph
         self.graphs: Dict[tuple, torch.cuda.CUDAGraph] = {}
-        self.plans: Dict[tuple, dict] = {}        # of batches that share prefixes, by what they share
         self.shared = self.make_up = None
         self.bufs: Dict[int, dict] = {}
         self.stream = torch.cuda.Stream(device=engine.device)
@@ -186,8 +185,6 @@ class DecodeRunner:
         self.make_up = None if self.shared is None else self.engine.shared_make_up(self.shared)
         self.shares: Dict[int, Optional[tuple]] = {}   # by the bucket of own keys: what the step shares
         self.longest = max(int(p) for p in positions) + 1
-        if len(self.plans) > 64:                   # (of batches long gone; graphs keep their own)
-            self.plans.clear()
 
     def _shared_at(self, context: int):
         """(what the step shares, or None, and what a plan and a graph that holds it are kept by) when
@@ -211,10 +208,9 @@ class DecodeRunner:
                           tok_seq=b["tok_seq"], seq_slot=b["seq_slot"],
                           seq_start=b["seq_start"], cu_seqlens=b["cu"], is_decode=True,
                           max_new=1, max_context=context)
-        shared, key = self._shared_at(context)
+        shared, _ = self._shared_at(context)
         if shared is not None:
-            ctx.extras["shared"] = shared
-            ctx.extras["shared_plans"] = self.plans.setdefault((B,) + key, {})
+            ctx.extras.update(eng.shared_extras(shared))
         logits = eng.model.forward(ctx, eng.cache, None)
         b["logits"] = logits
         self.sampler(logits, b["sampled"], b["request"], b["draw"])
@@ -228,15 +224,16 @@ class DecodeRunner:
         if not self.use_graph:
             self._body(b, B, context)
             return b["sampled"]
-        _, shared_key = self._shared_at(context)
-        key = (B, self.engine.context_bucket(context), shared_key)
+        eng = self.engine
+        shared, shared_key = self._shared_at(context)
+        key = (B, eng.context_bucket(context), shared_key)
         if key not in self.graphs:
             # Warm up outside the capture (lazy initialisation, kernel loading), restoring
             # the state the warm-up advanced, then capture.
             saved = b["ints"].clone()
             cur = torch.cuda.current_stream()
             self.stream.wait_stream(cur)
-            cache = self.engine.cache
+            cache = eng.cache
             with torch.cuda.stream(self.stream):
                 # keys and values are written to the same place twice; a recurrent state
                 # would advance twice, so it is put back after the warm-up
@@ -251,10 +248,10 @@ class DecodeRunner:
                     self._body(b, B, context)
             cur.wait_stream(self.stream)
             b["ints"].copy_(saved)
-            self.graphs[key] = (g, dict(self.plans.get((B,) + shared_key, {})))
-            shared = [k for k in self.graphs if k[2]]
-            if len(shared) > MAX_SHARED_GRAPHS:    # (what batches share seldom comes again)
-                del self.graphs[shared[0]]
+            self.graphs[key] = (g, eng.shared_extras(shared) if shared is not None else None)
+            kept = [k for k in self.graphs if k[2]]
+            if len(kept) > MAX_SHARED_GRAPHS:      # (what batches share seldom comes again)
+                del self.graphs[kept[0]]
         self.graphs[key][0].replay()
         return b["sampled"]
 

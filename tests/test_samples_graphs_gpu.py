@@ -68,3 +68,36 @@ def test_forked_steps_that_gain_nothing_share_captured_steps(model_dirs):
     eng.step([(alone[0], [5]), (alone[1], [6])])
     assert len([k for k in eng._graphs if k[0] == (1, 1)]) == 1
     assert all(torch.isfinite(o).all() for o in outs)
+
+
+def test_a_plan_is_made_once_for_steps_of_a_make_up(model_dirs, monkeypatch):
+    """Steps with drafts that are not captured, and the layers of each, use the plan of the first."""
+    from cretif_b200.csrc import ops
+    from cretif_b200.engine import engine as module
+    made = []
+    real = ops.shared_prefix_plan
+    monkeypatch.setattr(ops, "shared_prefix_plan", lambda *a: (made.append(real(*a)), made[-1])[1])
+    eng = engine(model_dirs, "C", step_graphs=False)
+    a = eng.alloc_slot()
+    eng.step([(a, tiny.tokens("C", 150, 1))])
+    b = eng.fork_slot(a)[0]
+    outs = []
+    for i in range(4):
+        outs.append(eng.step([(a, [5, 7]), (b, [6])], "all"))
+        eng.truncate_slot(a, 150), eng.truncate_slot(b, 150)
+    assert len(made) == 1 and all(torch.equal(outs[0], o) for o in outs)
+    for n in (1, 2):                                        # the other way round, and another number of drafts
+        eng.step([(a, [5] * n), (b, [6, 8, 1])])
+    assert len(made) == 3
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    eng.truncate_slot(a, 150), eng.truncate_slot(b, 150)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):                         # kept plans serve other streams
+        got = eng.step([(a, [5, 7]), (b, [6])], "all")
+    torch.cuda.synchronize()
+    assert torch.equal(got, outs[0]) and len(made) == 3
+    for n in range(1, module.MAX_SHARED_PLANS + 9):
+        eng.truncate_slot(a, 150), eng.truncate_slot(b, 150)
+        eng.step([(a, [5] * (1 + n % 9)), (b, [6] * (2 + n // 9))])
+    assert len(eng._shared_plans) == module.MAX_SHARED_PLANS
