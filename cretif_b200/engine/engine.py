@@ -34,7 +34,7 @@ import torch
 from ..cache import SequenceCache
 from ..config import load_config
 from ..csrc import ops
-from ..parts.attention import shared_pays
+from ..parts import attention
 from ..parts.base import StepContext
 from ..weights import load_weights
 from .model import Model, manifest
@@ -149,6 +149,9 @@ def require_cuda(device) -> torch.device:
 # (a last token and its drafts); longer ones are prompts.
 SHARED_MAX_NEW = 16
 MAX_SHARED_PLANS = 64   # make-ups whose plans an engine keeps
+# What a warm-up, a capture and an instantiation of a decode step cost, in units of attention.SHARED_MIN_BYTES of
+# reading: some 7 ms with 24 to 30 layers, in which 40 GB are read.
+SHARED_CAPTURE = 10_000
 
 Entry = Tuple[int, Sequence[int]]
 
@@ -253,7 +256,17 @@ class Engine:
 
     def shares(self, shared) -> bool:
         """Whether any layer reads what is shared once."""
-        return any(shared_pays(*shared, *heads) for heads in self._shared_heads)
+        return any(attention.shared_pays(*shared, *heads) for heads in self._shared_heads)
+
+    def steps_for_a_graph(self, shared) -> int:
+        """After how many steps of one make-up a graph of its own has paid: what it spares of reading
+        by then is what its capture costs.  Where that is a few steps, none: the ordinary step, which
+        they would run as, may have to be captured too."""
+        spared = sum(n * attention.shared_spares(shared[0], nkv, hd)
+                     for (nh, nkv, hd), n in self._shared_heads.items()
+                     if attention.shared_pays(*shared, nh, nkv, hd))
+        steps = SHARED_CAPTURE * attention.SHARED_MIN_BYTES // max(1, spared)
+        return steps if steps > 4 else 0
 
     def shared_extras(self, shared) -> dict:
         """What a step's context holds of what it shares: that, and the plans made for steps of its make-up

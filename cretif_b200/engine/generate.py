@@ -34,7 +34,9 @@ class GenerationResult:
     finish_reason: Optional[str] = None        # "stop" or "length"
 
 
-MAX_SHARED_GRAPHS = 8   # decode graphs kept of batches that share prefixes
+# Decode graphs kept of batches that share prefixes, the latest used: as many as a full batch has make-ups while its
+# answers end one by one.
+MAX_SHARED_GRAPHS = 64
 MAX_BACKENDS = 4      # sets of decode graphs kept per engine (one per temperature / top_k)
 
 
@@ -185,12 +187,17 @@ class DecodeRunner:
         self.make_up = None if self.shared is None else self.engine.shared_make_up(self.shared)
         self.shares: Dict[int, Optional[tuple]] = {}   # by the bucket of own keys: what the step shares
         self.longest = max(int(p) for p in positions) + 1
+        self.wait = 0 if self.shared is None else self.engine.steps_for_a_graph(self.shared)
+        self.steps = 0
 
     def _shared_at(self, context: int):
         """(what the step shares, or None, and what a plan and a graph that holds it are kept by) when
         the longest sequence holds ``context`` tokens: the groups, and the bucket of the own keys that
-        the plan was made for.  Where own keys have grown so long that no layer shares, nothing."""
-        if self.make_up is None:
+        the plan was made for.  Nothing where own keys have grown so long that no layer shares, and in
+        a make-up's first steps: until what they would have spared makes up for a capture they run
+        as the ordinary step, whose graph serves every make-up (whether this one's is there already or
+        not, and without graphs too: the same call gives the same bits)."""
+        if self.make_up is None or self.steps < self.wait:
             return None, ()
         grown = context - self.longest
         make_up, own = self.make_up
@@ -223,6 +230,7 @@ class DecodeRunner:
         b = self._buffers(B)
         if not self.use_graph:
             self._body(b, B, context)
+            self.steps += 1
             return b["sampled"]
         eng = self.engine
         shared, shared_key = self._shared_at(context)
@@ -252,7 +260,10 @@ class DecodeRunner:
             kept = [k for k in self.graphs if k[2]]
             if len(kept) > MAX_SHARED_GRAPHS:      # (what batches share seldom comes again)
                 del self.graphs[kept[0]]
+        if shared_key:                             # (the latest used last)
+            self.graphs[key] = self.graphs.pop(key)
         self.graphs[key][0].replay()
+        self.steps += 1
         return b["sampled"]
 
 

@@ -168,16 +168,17 @@ class Model:
                     out[(i, k, "shift")] = br.shift.cache_request()
         return out
 
-    def shared_heads(self) -> List[Tuple[int, int, int]]:
+    def shared_heads(self) -> Dict[Tuple[int, int, int], int]:
         """(heads, key/value heads, head size) of the mixers that may take the attention over shared
-        prefixes, each once."""
-        out = set()
-        for part in self._parts:
-            for _, p in part.sub_mixers() if hasattr(part, "sub_mixers") else [(None, part)]:
-                heads = p.shared_heads() if hasattr(p, "shared_heads") else None
-                if heads is not None:
-                    out.add(heads)
-        return sorted(out)
+        prefixes, and how many times a step does so."""
+        out: Dict[Tuple[int, int, int], int] = {}
+        for entry in self.spec.schedule:
+            for br in self.layers[entry.layer].branches:
+                for _, part in self._keepers(0, 0, br.part):
+                    heads = part.shared_heads() if hasattr(part, "shared_heads") else None
+                    if heads is not None:
+                        out[heads] = out.get(heads, 0) + 1
+        return out
 
     @staticmethod
     def _keepers(i: int, k: int, part):

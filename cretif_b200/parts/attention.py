@@ -138,7 +138,7 @@ def shared_pays(groups, news, starts, nh: int, nkv: int, hd: int) -> bool:
     for members, prefix in groups:
         for b in members:
             alone[b] -= prefix
-    spared = sum((len(m) - 1) * p for m, p in groups) * token
+    spared = shared_spares(groups, nkv, hd)
     if wide:
         if max(alone) > 1000 and spared < sum(alone) * token / 2:
             return False
@@ -146,6 +146,11 @@ def shared_pays(groups, news, starts, nh: int, nkv: int, hd: int) -> bool:
     read = (sum(alone) + sum(p for _, p in groups)) * token
     need = (1 if walked else 2) + 6 * max(alone) / 1000 + read / 40e6
     return spared >= need * SHARED_MIN_BYTES
+
+
+def shared_spares(groups, nkv: int, hd: int) -> int:
+    """Bytes of keys and values that a layer reads once instead of once for every member."""
+    return sum((len(m) - 1) * p for m, p in groups) * nkv * hd * 4
 
 
 def shared_takes(hd: int) -> bool:

@@ -70,6 +70,58 @@ def test_forked_steps_that_gain_nothing_share_captured_steps(model_dirs):
     assert all(torch.isfinite(o).all() for o in outs)
 
 
+def test_graphs_of_shared_prefixes_are_kept(model_dirs, captures, monkeypatch):
+    """Where steps share, a make-up that comes again finds its graph; the latest used are kept."""
+    import sys
+    from cretif_b200.parts import attention
+    generate = sys.modules["cretif_b200.engine.generate"]
+    monkeypatch.setattr(attention, "SHARED_MIN_BYTES", 0)   # (a capture costs nothing, all gain)
+    eng = engine(model_dirs, "C")
+    want = run(eng, 150, 24)
+    first = len(captures)
+    assert first > 10
+    assert run(eng, 150, 24) == want and len(captures) == first
+    (runner,) = {b.runner for b in eng._backends.values()}
+    assert len([k for k in runner.graphs if k[2]]) > 10
+    monkeypatch.setattr(generate, "MAX_SHARED_GRAPHS", 5)
+    eng.generate([tiny.tokens("C", 150, 3)], max_tokens=4, temperature=1.5, seed=4, stop_ids=[], samples=24)
+    largest = max(len(k[2][0][0]) for k in runner.graphs if k[2])
+    assert largest == 24
+    for n in range(6):                                      # other make-ups push out the rest, not the one in use
+        eng.generate([tiny.tokens("C", 215 + 64 * n, 3)], max_tokens=3, temperature=1.5, seed=4, stop_ids=[], samples=2)
+        eng.generate([tiny.tokens("C", 150, 3)], max_tokens=3, temperature=1.5, seed=4, stop_ids=[], samples=24)
+    kept = [k for k in runner.graphs if k[2]]
+    assert len(kept) <= 24 + 6 and any(len(k[2][0][0]) == 24 for k in kept)
+
+
+def test_a_make_up_runs_as_the_ordinary_step_until_a_graph_pays(model_dirs, captures, monkeypatch):
+    """What comes of a call does not depend on which graphs are there, or on whether there are any."""
+    from cretif_b200.csrc import ops
+    from cretif_b200.engine import engine as module
+    from cretif_b200.parts import attention
+    eng = engine(model_dirs, "C")
+    prompt = tiny.tokens("C", 150, 3)
+    heads = eng.model.shared_heads()
+    layers = sum(heads.values())
+    ((nh, nkv, hd),) = heads
+    spared = layers * attention.shared_spares([(list(range(6)), 128)], nkv, hd)
+    monkeypatch.setattr(attention, "shared_pays", lambda *a: True)
+    monkeypatch.setattr(module, "SHARED_CAPTURE", 10 * spared / attention.SHARED_MIN_BYTES)
+    steps, real = [], ops.attn_shared
+    monkeypatch.setattr(ops, "attn_shared", lambda *a, **k: (steps.append(1), real(*a, **k))[1])
+
+    def go(**kw):
+        return [r.tokens for r in eng.generate([prompt], max_tokens=30, temperature=1.5, seed=4, stop_ids=[], samples=6, **kw)]
+    first = go()
+    (runner,) = {b.runner for b in eng._backends.values()}
+    assert sorted(bool(k[2]) for k in runner.graphs) == [False, True]
+    n = len(captures)
+    assert go() == first and len(captures) == n             # (the same kernels step for step, no capture)
+    del steps[:]
+    assert go(use_graph=False) == first
+    assert len(steps) == (29 - 10) * layers                 # the first token is the prompt's, ten steps wait
+
+
 def test_a_plan_is_made_once_for_steps_of_a_make_up(model_dirs, monkeypatch):
     """Steps with drafts that are not captured, and the layers of each, use the plan of the first."""
     from cretif_b200.csrc import ops
