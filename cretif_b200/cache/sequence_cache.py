@@ -23,6 +23,7 @@ before anything is launched, in the same spirit.
 """
 from __future__ import annotations
 
+from collections import Counter
 from dataclasses import dataclass, replace
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -505,9 +506,9 @@ class SequenceCache:
                 if held and not self.slots.is_live(s):
                     raise CacheError(f"free slot {s} still maps blocks {held}")
                 mapped.extend(held)
-            for b in set(mapped):
-                if mapped.count(b) != g.pool.holders(b):
-                    raise CacheError(f"block {b} is mapped by {mapped.count(b)} sequences and held by "
-                                     f"{g.pool.holders(b)}")
-            if len(set(mapped)) != g.pool.held_count:
-                raise CacheError(f"{g.pool.held_count} blocks are held but {len(set(mapped))} are mapped")
+            times = Counter(mapped)
+            for b, n in times.items():
+                if n != g.pool.holders(b):
+                    raise CacheError(f"block {b} is mapped by {n} sequences and held by {g.pool.holders(b)}")
+            if len(times) != g.pool.held_count:
+                raise CacheError(f"{g.pool.held_count} blocks are held but {len(times)} are mapped")
