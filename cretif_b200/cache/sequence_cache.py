@@ -280,10 +280,11 @@ class SequenceCache:
                 self._kv_of[cid] = (g, i)
             if req.pool > 0:
                 # Enough for any mixture of live sequences: each may leave its last block of
-                # entries partly empty, and only one with ``pool`` tokens has an entry at all.
+                # entries partly empty, and a fork has filled up a copy of one besides.  (With a block
+                # of tokens of its own, as all that are stepped have, a sequence needs no more blocks of
+                # entries than of tokens.)
                 P = req.pool
-                n_pool = -(-self.max_tokens // (P * block_tokens)) \
-                    + min(self.max_slots, self.max_tokens // P)
+                n_pool = -(-self.max_tokens // (P * block_tokens)) + 2 * self.max_slots
                 pg = _KVGroup(replace(req, window=0, pool=0), cids,
                               max(1, min(self.n_blocks, n_pool)), block_tokens, self.max_slots,
                               max(1, -(-(self.max_len // P) // block_tokens)), dtype, self.device,

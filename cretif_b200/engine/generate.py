@@ -79,8 +79,11 @@ class GenerationLoop:
             if n > self.max_len:
                 raise ValueError(f"request {i}: the prompt has {n} tokens, the longest "
                                  f"sequence allowed is {self.max_len}")
-            whole = self._rounded(self._reserve_len(n, max_tokens))
-            need = whole + (samples - 1) * (whole - n // self.block_tokens * self.block_tokens)
+            reserve = self._reserve_len(n, max_tokens)
+            whole = self._rounded(reserve)
+            need = whole
+            if reserve > n:                            # (answers of one token are drawn from the prompt's logits)
+                need += (samples - 1) * (whole - n // self.block_tokens * self.block_tokens)
             if need > self.capacity_tokens:
                 raise ValueError(f"request {i} needs {need} cache tokens, the cache holds "
                                  f"{self.capacity_tokens}")
@@ -328,10 +331,11 @@ class EngineBackend:
         B = len(self.slots)
         if n > 1:
             logits = logits.repeat_interleave(n, dim=0)
-            for first in range(0, B, n):
+            goes_on = [i for i in range(B) if self.reserve[i] > len(self.prompts[i])]
+            for first in goes_on[::n]:             # (answers of one token have nothing to go on from)
                 self.slots[first + 1:first + n] = eng.fork_slot(self.slots[first], n - 1)
-            for i in range(B):
-                eng.cache.reserve(self.slots[i], self.reserve[i], flush=i + 1 == B)
+            for i in goes_on:
+                eng.cache.reserve(self.slots[i], self.reserve[i], flush=i == goes_on[-1])
         out = torch.empty(B, dtype=torch.int32, device=eng.device)
         req = torch.from_numpy(np.asarray(self.request_ids, dtype=np.int64)).pin_memory().to(
             eng.device, non_blocking=True)
