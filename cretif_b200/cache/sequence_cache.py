@@ -223,6 +223,21 @@ class _KVGroup:
         self.dirty.clear()
 
 
+def _spared_most(rows, members, deep: int = 0):
+    """(blocks spared, [(members, first blocks that they have in common)]) of ``members``, two or more of
+    the tables ``rows`` that begin alike: together, or parted by the block at which they part."""
+    alike = (rows[members] == rows[members[0]]).all(axis=0) & (rows[members[0]] >= 0)
+    n = int(alike.size if alike.all() else np.argmin(alike))
+    together = (members.size - 1) * n, [(members, n)]
+    if n == alike.size or members.size == 2 or deep == 64:
+        return together
+    behind = rows[members, n]
+    blocks, times = np.unique(behind[behind >= 0], return_counts=True)
+    apart = [_spared_most(rows, members[behind == b], deep + 1) for b in blocks[times > 1]]
+    spared = sum(s for s, _ in apart)
+    return together if spared <= together[0] else (spared, [g for _, groups in apart for g in groups])
+
+
 class SequenceCache:
     """Slots, lengths, block tables and storage for all cache ids of a model.
 
@@ -368,22 +383,21 @@ class SequenceCache:
 
     def shared_groups(self, slots: Sequence[int]) -> List[Tuple[List[int], int]]:
         """Which of ``slots`` (by their places in the list) have first blocks in common, and how many
-        tokens those hold: what the attention over shared prefixes is planned for.  Sequences that
-        share more among some of them than all do count with what all do."""
+        tokens those hold: what the attention over shared prefixes is planned for.  A sequence is in
+        one group; where some share more among them than all do, the groups are those that spare the
+        most reading (one of all with what all share, or several of fewer with more)."""
         g = next((g for g in self._kv_groups if g.request.window == 0 and g.tokens_per_entry == 1
                   and g.pool.shared_count), None)
         if g is None or len(slots) < 2:
             return []
-        rows = g.table_host[np.asarray(slots, dtype=np.int64)]
+        at = np.asarray(slots, dtype=np.int64)
+        rows = g.table_host[at, :max(1, int(g.n_blocks_of[at].max()))]
         first = rows[:, 0]
         out = []
         for blk in np.unique(first[first >= 0]):
             members = np.flatnonzero(first == blk)
-            if members.size < 2:
-                continue
-            alike = (rows[members] == rows[members[0]]).all(axis=0) & (rows[members[0]] >= 0)
-            n = int(alike.size if alike.all() else np.argmin(alike))
-            out.append((members.tolist(), n * self.block_tokens))
+            if members.size > 1:
+                out += [(m.tolist(), n * self.block_tokens) for m, n in _spared_most(rows, members)[1]]
         return out
 
     # -- a step ----------------------------------------------------------------
