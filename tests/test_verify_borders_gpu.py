@@ -153,3 +153,45 @@ def test_a_top_k_beyond_the_vocabulary_is_none(ops, temperature):
     for top_k in (2000, 2001, 2 ** 31, 2 ** 32 + 2, 2 ** 40):
         got = verify(ops, s, temperature, top_k, s["draft_logits"])
         assert all(torch.equal(a, b) for a, b in zip(want, got)), top_k
+
+
+@pytest.mark.parametrize("proposed", [True, False])
+@pytest.mark.parametrize("temperature, top_k", [(0.9, 0), (0.9, 30), (0.0, 0)])
+def test_a_draft_outside_the_vocabulary(ops, temperature, top_k, proposed):
+    """At a place that is judged it does not stand and sets the fault word, exactly; behind the last draft, or behind
+    one that does not stand, it is not looked at."""
+    B, K, V = 24, 5, 3001
+    counts = [K - b % 3 for b in range(B)]
+    s = make(B, K, V, counts, seed=17, temperature=temperature, top_k=top_k, like=0.05)
+    if temperature <= 0:                                   # (drafts that are the arg max, some of them)
+        cu = s["cu"].tolist()
+        best = s["logits"].argmax(-1).int()
+        for b in range(B):
+            for j in range(counts[b]):
+                if (b + j) % 4:
+                    s["drafts"][b, j] = best[cu[b] + j]
+    q = s["draft_logits"] if proposed else None
+    accepted, tokens = (t.cpu() for t in verify(ops, s, temperature, top_k, q))
+    judged = behind = 0
+    fault = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for bad in (V, -1, 2 ** 31 - 1):
+        for b in range(B):
+            for j in range(K):
+                if (b + j + bad) % 3:
+                    continue
+                t = {**s, "drafts": s["drafts"].clone()}
+                t["drafts"][b, j] = bad
+                fault.zero_()
+                got_a, got_t = (x.cpu() for x in verify(ops, t, temperature, top_k, q, fault))
+                others = [i for i in range(B) if i != b]
+                assert torch.equal(got_a[others], accepted[others]) and torch.equal(got_t[others], tokens[others])
+                if j < counts[b] and j <= int(accepted[b]):
+                    assert int(fault.item()) == 1 and int(got_a[b]) == j
+                    assert got_t[b, :j].tolist() == s["drafts"][b, :j].tolist() and 0 <= int(got_t[b, j]) < V
+                    assert (got_t[b, j + 1:] == -1).all()
+                    judged += 1
+                else:
+                    assert int(fault.item()) == 0
+                    assert int(got_a[b]) == int(accepted[b]) and torch.equal(got_t[b], tokens[b])
+                    behind += 1
+    assert judged > 10 and behind > 10
