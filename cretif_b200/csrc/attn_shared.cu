@@ -14,10 +14,11 @@ constexpr int kShRows = 32, kShThreads = 256;
 // 32-bit pieces: a block of 256 threads per (item, key/value head), up to 32 rows and 64 keys a step.
 // A warp has rows w, w + 8, w + 16, w + 24, those that there are: a lane two keys of their scores and VD
 // channels of their outputs, so a softmax is the warp's own.  The next step's keys and values are on
-// their way in registers.  (Eight answers at 1,984 tokens: 13.2 us; 16 x 16 threads on 32 rows whatever
-// there were took 25, most of it on the own keys' three rows.)
+// their way in registers.  (Eight answers at 1,984 tokens: 13.5 us; 16 x 16 threads on 32 rows whatever
+// there were took 25, most of it on the own keys' three rows.  One CTA an SM is all that fits: said so, the
+// compiler takes 235 registers instead of 171, and 0.4 us less.)
 template <int VD>
-__global__ void __launch_bounds__(kShThreads)
+__global__ void __launch_bounds__(kShThreads, 1)
 shared_pieces_kernel(const SharedArgs a) {
   extern __shared__ __align__(16) float sh_smem[];
   const int hd = a.hd, ldk = hd + 4, quads = hd >> 2;
@@ -25,28 +26,28 @@ shared_pieces_kernel(const SharedArgs a) {
   float* ks = qs + kShRows * ldk;             // [64][hd + 4]
   float* vs = ks + kShBlk * ldk;              // [64][hd]
   float* ps = vs + kShBlk * hd;               // [32][64]
-  __shared__ int toks[kShRows], firsts[kShRows];   // a row's token, and that token's first piece
+  __shared__ int toks[kShRows], pieces[kShRows];   // a row's token, and this piece of it among all
   const int kvh = blockIdx.y, g = a.nh / a.nkv, tid = threadIdx.x;
   const int warp = tid >> 5, lane = tid & 31;
   constexpr int kRows = kShRows / 8;          // of a warp
   dependent_begin();
 
   // ---- this block's rows and keys
-  int seq, row0, n_rows, row_base = -1, tok0 = 0, key0, key_end, piece;
+  int seq, row0, n_rows, row_base = -1, tok0 = 0, at0 = 0, a_token = 0, key0, key_end;
   if ((int)blockIdx.x < a.n_pre) {
     const SharedPrefixItem it = a.pre[blockIdx.x];
     seq = it.seq; row0 = it.row0; n_rows = it.n_rows; row_base = it.row_base;
-    key0 = it.blk0 * kShBlk; key_end = it.blk1 * kShBlk; piece = it.piece;
+    key0 = it.blk0 * kShBlk; key_end = it.blk1 * kShBlk; at0 = it.piece;
   } else {
     const int x = blockIdx.x - a.n_pre, split = x % a.own_splits;
     const SharedOwnItem it = a.own[x / a.own_splits];
     seq = it.seq; row0 = it.row0; n_rows = it.n_rows; tok0 = it.tok0;
+    at0 = it.first + it.pieces + split; a_token = it.pieces + a.own_splits;
     const int prefix = it.prefix;
     const int end = shared_own_end(a, it, a.tok_pos[tok0 + (row0 + n_rows - 1) / g]);
     const int blocks = (end - prefix + kShBlk - 1) / kShBlk;
     key0 = prefix + (int)((long long)blocks * split / a.own_splits) * kShBlk;
     key_end = min(end, prefix + (int)((long long)blocks * (split + 1) / a.own_splits) * kShBlk);
-    piece = it.pieces + split;
   }
   // a thread's share of a step's tile: keys tid / quads, + step, ...; at most 8 of four channels
   const int slot = a.seq_slot[seq];
@@ -71,7 +72,7 @@ shared_pieces_kernel(const SharedArgs a) {
   if (tid < kShRows) {
     const int r = row0 + tid;
     toks[tid] = tid >= n_rows ? -1 : row_base >= 0 ? a.rows[row_base + r / g] : tok0 + r / g;
-    firsts[tid] = tid >= n_rows ? 0 : row_base >= 0 ? a.rows_first[row_base + r / g] : a.first[tok0 + r / g];
+    pieces[tid] = at0 + (tid >= n_rows ? 0 : row_base >= 0 ? a.rows_first[row_base + r / g] : r / g * a_token);
   }
   __syncthreads();
   for (int i = tid; i < kShRows * quads; i += kShThreads) {
@@ -190,7 +191,7 @@ shared_pieces_kernel(const SharedArgs a) {
   for (int i = 0; i < kRows; ++i)
     if (i < mine) {
       const int r = warp + 8 * i;
-      const size_t row = ((size_t)firsts[r] + piece) * a.nh + kvh * g + (row0 + r) % g;
+      const size_t row = (size_t)pieces[r] * a.nh + kvh * g + (row0 + r) % g;
       if (lane == 0) a.part_ml[row] = make_float2(m[i], l[i]);
       if (has_d) {
         float* to = a.part_o + row * hd + d0;

@@ -2,6 +2,12 @@
 //
 // shared_prefix_tc: the prefix's keys against all rows of a group on the tcgen05 tensor cores.
 // shared_own_mma: a sequence's own keys against its few rows, and the joining of a row's pieces.
+//
+// What is held in fewer than 32 bits: a probability is rounded to bfloat16 where it becomes an operand of P V, as in the
+// framework's other attention kernels, because the tensor cores take a 32-bit operand at an eighth of the rate and in
+// twice the shared memory.  It is off by half a step, 2^-9 at most of each term p |v| of an output; the sums l of
+// the same probabilities are 32-bit and not rounded.  (Error against 64 bits, as a share of the largest output: 2.0 to
+// 2.35e-3 with the output's own rounding, which alone is 1.7e-3.)  Exponentials are ex2.approx.ftz, off by 2^-22.
 #include <cuda.h>
 
 #include "api.h"

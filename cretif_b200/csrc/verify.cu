@@ -749,7 +749,7 @@ verify_draw_kernel(const __grid_constant__ VfArgs a) {
 // above it are few more than k.  They are listed in a second look at the row (from L2) and sorted by
 // (value, id).  Where they are too many for the list (equal logits in masses) the k-th largest is
 // found digit by digit over the whole row.
-// (512 threads: three CTAs of them fit an SM, and one's sort runs under another's loads.  218 rows of 49,152:
+// (512 threads: three CTAs of them fit an SM, and one's sort runs under another's loads.  250 rows of 49,152:
 // 21.4 us, with 1,024 threads, one CTA an SM, 35.)
 constexpr int kVkThreads = 512, kVkWarps = kVkThreads / 32, kVkList = 4096;
 constexpr int kVkMaxima = kVfMaxTopK / kVkThreads;        // maxima a thread keeps: together at least top_k

@@ -146,7 +146,9 @@ def require_cuda(device) -> torch.device:
 
 
 # Steps in which no sequence brings more tokens than this may take the attention over shared prefixes
-# (a last token and its drafts); longer ones are prompts.
+# (a last token and its drafts); longer ones are prompts.  (Against prompt attention, 2 to 32 sequences on 128 to
+# 8,192 tokens: with 16 new tokens each it takes 0.1 to 0.93 of the time, with 17 up to 1.04, with 24 heads of 128 take
+# up to 1.34 times, with 64 most steps on up to 1,024 tokens take more, up to 2.4 times.)
 SHARED_MAX_NEW = 16
 MAX_SHARED_PLANS = 64   # make-ups whose plans an engine keeps
 # What a warm-up, a capture and an instantiation of a decode step cost, in units of attention.SHARED_MIN_BYTES of
