@@ -248,7 +248,8 @@ class Engine:
         brings, cached tokens), or None, also where no layer gains by it: such a step is one like any
         other, and shares their graphs.  Only for bfloat16: in float32 a token's bits do not depend on
         the rest of its step."""
-        if self.dtype != torch.bfloat16 or max(news) > SHARED_MAX_NEW or not self._shared_heads:
+        if self.dtype != torch.bfloat16 or max(news) > SHARED_MAX_NEW or not self._shared_heads \
+                or self.cache.block_tokens != 64:
             return None
         groups = self.cache.shared_groups(slots)
         if not groups:

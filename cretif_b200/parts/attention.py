@@ -128,7 +128,8 @@ def shared_pays(groups, news, starts, nh: int, nkv: int, hd: int) -> bool:
     Several tokens: always (4 tokens each, 8 sequences on 2,048 tokens, prompt attention 22.9 / 10.2; none of 521 steps
     was slower), but for wide heads of few sequences that are short (16 on 16, 3 sequences, up to 16 new tokens on
     448 tokens 11.3 / 15.0): 12 of 439 steps slower, at most 1.4 times.  Of 700 steps drawn afterwards 11 are
-    slower, at most 1.36 times."""
+    slower, at most 1.36 times.  More than eight heads on each of several key/value heads: always, since single
+    tokens would go to the plain kernel (20 and 32 on 2, 2 to 32 sequences, 4 to 100 times as long)."""
     token = nkv * hd * 4                             # bytes of a token's keys and values
     ends = [s + n for s, n in zip(starts, news)]
     walked, wide = ops.shared_prefix_walked(groups, nkv, hd), hd > 64
@@ -138,6 +139,8 @@ def shared_pays(groups, news, starts, nh: int, nkv: int, hd: int) -> bool:
     for members, prefix in groups:
         for b in members:
             alone[b] -= prefix
+    if not decode_takes(nh, nkv):
+        return True
     spared = shared_spares(groups, nkv, hd)
     if wide:
         if max(alone) > 1000 and spared < sum(alone) * token / 2:
@@ -146,6 +149,11 @@ def shared_pays(groups, news, starts, nh: int, nkv: int, hd: int) -> bool:
     read = (sum(alone) + sum(p for _, p in groups)) * token
     need = (1 if walked else 2) + 6 * max(alone) / 1000 + read / 40e6
     return spared >= need * SHARED_MIN_BYTES
+
+
+def decode_takes(nh: int, nkv: int) -> bool:
+    """Whether the decode kernels take these heads: up to eight on a key/value head, or any number on one."""
+    return nh // nkv <= 8 or nkv == 1
 
 
 def shared_spares(groups, nkv: int, hd: int) -> int:
@@ -204,7 +212,7 @@ def run_attention(q, o, ctx, kv, nh, nkv, hd, scale, window, dtype, sink=None, v
             return
     if fast:
         if ctx.is_decode and ops.attn_decode_supported(hd, kv.block_tokens, min(nh // nkv, 8)) \
-                and (nh // nkv <= 8 or nkv == 1):
+                and decode_takes(nh, nkv):
             # the kernel takes up to eight query heads per key/value head; more heads on ONE
             # key/value head (a shared latent) go as groups of eight in one launch whose items
             # are (sequence, group) pairs, where the rows allow that view ...

@@ -153,3 +153,24 @@ def test_a_plan_is_made_once_for_steps_of_a_make_up(model_dirs, monkeypatch):
         eng.truncate_slot(a, 150), eng.truncate_slot(b, 150)
         eng.step([(a, [5] * (1 + n % 9)), (b, [6] * (2 + n // 9))])
     assert len(eng._shared_plans) == module.MAX_SHARED_PLANS
+
+
+@pytest.mark.parametrize("block_tokens", [32, 128])
+def test_blocks_of_another_size_are_shared_in_the_cache_alone(model_dirs, monkeypatch, block_tokens):
+    """The attention over shared prefixes takes blocks of 64: forks on others step as all sequences do."""
+    from cretif_b200.csrc import ops
+    from cretif_b200.parts import attention
+    monkeypatch.setattr(attention, "shared_pays", lambda *a: True)
+    monkeypatch.setattr(ops, "attn_shared", None)
+    eng = engine(model_dirs, "C", block_tokens=block_tokens)
+    prompt = tiny.tokens("C", 300, 3)
+    opts = dict(max_tokens=12, temperature=1.5, seed=4, stop_ids=[])
+    got = [r.tokens for r in eng.generate([prompt], samples=4, **opts)]
+    assert got == [r.tokens for r in eng.generate([prompt] * 4, **opts)]
+    a = eng.alloc_slot()
+    eng.step([(a, prompt)])
+    b = eng.fork_slot(a)[0]
+    for _ in range(3):
+        eng.step([(a, [5, 6]), (b, [7])])
+    assert eng.cache.shared_groups([a, b]) == [([0, 1], 300 // block_tokens * block_tokens)]
+    assert all(k[1] == "last" for k in eng._graphs)

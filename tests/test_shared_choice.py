@@ -25,6 +25,10 @@ MEASURED = [
     (32, 32, 64, 32, 512, 60, 4, 17.2, 84.2),
     (16, 2, 128, 32, 512, 60, 4, 19.3, 53.9),
     (16, 2, 128, 2, 2048, 60, 4, 18.0, 35.5),
+    (32, 2, 64, 2, 64, 30, 1, 3.5, 18.0),
+    (20, 2, 32, 8, 64, 30, 1, 3.2, 12.6),
+    (20, 2, 32, 2, 512, 1000, 1, 9.8, 57.5),
+    (24, 2, 128, 2, 4096, 4000, 1, 18.5, 827.5),
     (16, 16, 128, 3, 448, 30, 16, 15.0, 11.3),
     (16, 16, 128, 6, 320, 10, 8, 12.8, 10.0),
     (32, 8, 128, 4, 320, 60, 3, 12.4, 10.1),
