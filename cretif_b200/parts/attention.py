@@ -113,23 +113,27 @@ SHARED_MIN_BYTES = 4 << 20
 
 
 def shared_pays(groups, news, starts, nh: int, nkv: int, hd: int) -> bool:
-    """Whether a step takes the attention over shared prefixes, by what was measured of both (1,700 steps: 2 to 64
+    """Whether a step takes the attention over shared prefixes, by what was measured of both (1,900 steps: 2 to 64
     sequences, 1 to 29 groups and sequences that share nothing, 4 to 12,000 own tokens, up to 16 new ones, 9 head
-    layouts; a sequence's tokens are ``starts`` + ``news``).
+    layouts; a sequence's tokens are ``starts`` + ``news``).  Counted is a choice that is slower by more than 5 %.
 
     Single tokens, heads of up to 64: a second launch for the prefix, and own keys, which the ordinary kernel
     deals out over more CTAs, cost what 4 MB and 24 MB a thousand tokens of reading do; so does a tenth of what
     is read either way.  (ordinary / shared, us: 9 heads on 3, 8 sequences on 2,048 tokens 6.9 / 7.8, 32 on 1,024 8.5 / 7.9;
-    32 on 32, 8 on 2,048 26.2 / 10.6, 6 on 576 and 1,700 own tokens 18.0 / 25.8.)  Of 415 steps 9 are slower than the
-    other kernel would be by more than 5 %, at most 1.35 times, and 38 are left to the ordinary kernel that would
-    gain.  Wider heads: the ordinary kernel needs more for few keys, so all walked prefixes gain (16 on 2, 32
-    sequences on 256 tokens 17.9 / 8.2), others from 8 MB on, long own keys that are twice what is spared excepted (16 on
-    16, 10 sequences, 3 of them on 4,800 tokens, 5,700 own ones 91 / 146).  Of 325 steps 15 are slower, at most 1.5 times.
-    Several tokens: always (4 tokens each, 8 sequences on 2,048 tokens, prompt attention 22.9 / 10.2; none of 521 steps
-    was slower), but for wide heads of few sequences that are short (16 on 16, 3 sequences, up to 16 new tokens on
-    448 tokens 11.3 / 15.0): 12 of 439 steps slower, at most 1.4 times.  Of 700 steps drawn afterwards 11 are
-    slower, at most 1.36 times.  More than eight heads on each of several key/value heads: always, since single
-    tokens would go to the plain kernel (20 and 32 on 2, 2 to 32 sequences, 4 to 100 times as long)."""
+    32 on 32, 8 on 2,048 26.2 / 10.6, 6 on 576 and 1,700 own tokens 18.0 / 25.8.)  Taken though slower: 9 of 415 steps, up
+    to 1.35 times; left though faster: 40.
+    Wider heads: with 16 items (key/value heads x sequences) the ordinary kernel needs twice as long as with fewer, so all
+    gain (16 on 2, sharing 64 tokens: 4 sequences 6.7 / 4.7, 8 12.9 / 4.7; 32 on 256 17.9 / 8.2), but for long own keys that
+    are twice what is spared, in too few items to fill the chip and too many to be cut into ranges (16 on 16, 10
+    sequences, 3 of them on 4,800 tokens, 5,700 own ones 91 / 146).  With fewer items little walked gains, and what the
+    ordinary kernel has to deal out in more ranges than a cluster's (from 8,192 tokens on 41 / 17).  21 of 546 steps, up to
+    1.54 times, and 28.
+    Several tokens: always (4 tokens each, 8 sequences on 2,048 tokens, prompt attention 22.9 / 10.2; 0 of 521 steps), but
+    for wide heads of few sequences that are short (16 on 16, 3 sequences, up to 16 new tokens on 448 tokens 11.3 /
+    15.0): 12 of 439 steps, up to 1.4 times, and 1.
+    More than eight heads on each of several key/value heads: always, since single tokens would go to the plain kernel
+    (20 and 32 on 2, 2 to 32 sequences, 4 to 100 times as long).
+    Of 1,200 steps drawn afterwards 34 are taken though slower, up to 1.67 times, and 37 left though faster."""
     token = nkv * hd * 4                             # bytes of a token's keys and values
     ends = [s + n for s, n in zip(starts, news)]
     walked, wide = ops.shared_prefix_walked(groups, nkv, hd), hd > 64
@@ -143,9 +147,11 @@ def shared_pays(groups, news, starts, nh: int, nkv: int, hd: int) -> bool:
         return True
     spared = shared_spares(groups, nkv, hd)
     if wide:
-        if max(alone) > 1000 and spared < sum(alone) * token / 2:
-            return False
-        return spared >= (0 if walked else 2) * SHARED_MIN_BYTES
+        items = nkv * len(ends)
+        if items < 16:
+            return max(ends) >= 8192 or (walked and max(ends) <= 200) or spared >= 8 * SHARED_MIN_BYTES
+        # (own keys in too few items to fill the chip and too many to be cut into ranges)
+        return not (48 <= items < 200 and max(alone) > 1000 and spared < sum(alone) * token / 2)
     read = (sum(alone) + sum(p for _, p in groups)) * token
     need = (1 if walked else 2) + 6 * max(alone) / 1000 + read / 40e6
     return spared >= need * SHARED_MIN_BYTES
