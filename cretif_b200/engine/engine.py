@@ -420,11 +420,11 @@ class Engine:
         so the capture's context is the finished step's, rebuilt on a buffer of its own."""
         if n_want * self.vocab_size * 4 > self.graph_max_logit_bytes:
             return
+        if len(self._seen) >= 4096 and key not in self._seen:
+            self._seen.clear()                      # (shapes that never come again, for the most part)
         self._seen[key] = self._seen.get(key, 0) + 1
         if self._seen[key] < 2:
             return
-        if len(self._seen) > 4096:
-            self._seen.clear()
         meta = torch.zeros(self._last_meta_len, dtype=torch.int32, device=self.device)
         saved = {s: int(self.cache.lengths[s]) for s in ran.seq_slot_host}
         for s, n in zip(ran.seq_slot_host, ran.seq_new_host):

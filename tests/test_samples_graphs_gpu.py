@@ -174,3 +174,18 @@ def test_blocks_of_another_size_are_shared_in_the_cache_alone(model_dirs, monkey
         eng.step([(a, [5, 6]), (b, [7])])
     assert eng.cache.shared_groups([a, b]) == [([0, 1], 300 // block_tokens * block_tokens)]
     assert all(k[1] == "last" for k in eng._graphs)
+
+
+def test_shapes_that_never_come_again_are_forgotten(model_dirs):
+    """Steps with drafts are of ever new shapes: how many of them an engine remembers is bounded."""
+    eng = engine(model_dirs, "C")
+    a, b = eng.alloc_slot(), eng.alloc_slot()
+    eng._seen.update({("a shape", i): 1 for i in range(4096)})
+    eng.step([(a, [1, 2, 3]), (b, [4])])
+    assert len(eng._seen) == 1
+    eng.step([(a, [1, 2, 3]), (b, [4])])
+    assert len(eng._graphs) == 1
+    eng._seen.update({("a shape", i): 1 for i in range(4095)})
+    for n in range(1, 12):
+        eng.step([(a, [1] * n), (b, [4] * 9)])
+        assert len(eng._seen) <= 4096
